@@ -10,12 +10,15 @@ from .api import (  # noqa: F401
     Gguf,
     LayerTensors,
     MoeContext,
+    RouteRule,
     argmax_f16,
     bread_dequant_rows,
+    bread_matmul,
     bread_matvec,
     bread_matvec_f32,
     bread_rmsnorm_f32,
     layer_seeds,
+    route_select,
     row_bytes,
     shape,
     shape_bytes,

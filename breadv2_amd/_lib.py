@@ -36,6 +36,15 @@ PATH_GROUPED = 2
 PATH_PER_TOKEN = 3
 PATH_SMALL = 4
 
+# BREAD_ACT_*, BREAD_SCORE_*
+ACT_NONE = 0
+ACT_SILU = 1
+ACT_GELU = 2
+ACT_GELU_TANH = 3
+ACT_RELU = 4
+SCORE_SOFTMAX = 0
+SCORE_SIGMOID = 1
+
 QK_K = 256
 Q4K_BLOCK_BYTES = 144
 Q6K_BLOCK_BYTES = 210
@@ -96,6 +105,50 @@ class MoeLayer(ctypes.Structure):
     ]
 
 
+class MatmulOpts(ctypes.Structure):
+    _fields_ = [
+        ("bias", c_void_p),
+        ("residual", c_void_p),
+        ("act", c_int),
+        ("y_type", c_int),
+        ("x_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+    ]
+
+
+class RouteRuleDesc(ctypes.Structure):
+    _fields_ = [
+        ("bias", c_void_p),
+        ("score", c_int),
+        ("n_groups", c_int),
+        ("top_groups", c_int),
+        ("group_top", c_int),
+        ("renorm", c_int),
+        ("scale", c_float),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p),
+        ("logits_stride", ctypes.c_int64),
+        ("logits_type", c_int),
+        ("vocab", c_int),
+        ("n_rows", c_int),
+        ("n_requests", c_int),
+        ("tokens", c_void_p),
+        ("offsets", c_void_p),
+        ("u", c_void_p),
+        ("draft_probs", c_void_p),
+        ("draft_probs_stride", ctypes.c_int64),
+        ("temperature", c_void_p),
+        ("eos", c_int32),
+        ("n_accept", c_void_p),
+        ("next", c_void_p),
+        ("logprob", c_void_p),
+    ]
+
+
 class GgufTensor(ctypes.Structure):
     _fields_ = [
         ("name", c_char_p),
@@ -116,6 +169,8 @@ SIGNATURES = {
     "bread_set_exit_on_error": (None, [c_int]),
     "bread_matvec": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "bread_matvec_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "bread_matmul": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "bread_dequant_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "bread_moe_shape_default": (None, [POINTER(MoeShape)]),
     "bread_moe_ctx_create": (c_int, [POINTER(MoeShape), c_int, POINTER(c_void_p)]),
@@ -128,6 +183,10 @@ SIGNATURES = {
         c_int,
         [POINTER(MoeShape), POINTER(MoeLayer), c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    "bread_route_select": (
+        c_int, [c_void_p, c_void_p, ctypes.c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "bread_route_by_rule": (
+        c_int, [c_void_p, POINTER(MoeLayer), c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "bread_route_layer": (
         c_int,
         [c_void_p, POINTER(MoeLayer), c_void_p, POINTER(c_int32), POINTER(c_float), POINTER(c_float), c_void_p],
@@ -140,6 +199,11 @@ SIGNATURES = {
         c_int,
         [c_void_p, POINTER(MoeLayer), c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    "bread_moe_forward_by_rule": (
+        c_int,
+        [c_void_p, POINTER(MoeLayer), c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "bread_spec_verify": (c_int, [c_void_p, c_void_p, c_void_p]),
     "bread_moe_forward_f16": (
         c_int,
         [c_void_p, POINTER(MoeLayer), c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],

@@ -24,6 +24,7 @@ PATH_DECODE = _lib.PATH_DECODE
 PATH_GROUPED = _lib.PATH_GROUPED
 PATH_PER_TOKEN = _lib.PATH_PER_TOKEN
 PATH_SMALL = _lib.PATH_SMALL
+QTYPE_F16 = _lib.QTYPE_F16
 
 
 def _p(t: torch.Tensor | None):
@@ -34,6 +35,21 @@ def _s(stream) -> ctypes.c_void_p:
     if stream is None:
         stream = torch.cuda.current_stream()
     return ctypes.c_void_p(stream.cuda_stream)
+
+
+def _need(cond: bool, what: str) -> None:
+    if not cond:
+        raise ValueError(what)
+
+
+def _on(stream, *tensors) -> int:
+    """The raw stream a call on these tensors goes to (default: torch's current
+    one).  A launch goes to the current device, so the tensors have to be there."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+    return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
 
 
 _HIP = None
@@ -73,6 +89,48 @@ def bread_matvec(w, x, y, rows: int, cols: int, qtype: int, stream=None) -> None
 
 def bread_matvec_f32(w, x, y, rows: int, cols: int, qtype: int, stream=None) -> None:
     check(lib.bread_matvec_f32(_p(w), _p(x), _p(y), rows, cols, qtype, _s(stream)), "bread_matvec_f32")
+
+
+ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU,
+        "gelu_tanh": _lib.ACT_GELU_TANH, "relu": _lib.ACT_RELU}
+
+
+def _rows_of(t: torch.Tensor, name: str, cols: int) -> int:
+    """Elements from one row of a 2-d tensor to the next (rows themselves dense)."""
+    _need(t.dim() == 2 and t.shape[1] == cols, f"{name} must be 2-d with {cols} columns, is {tuple(t.shape)}")
+    _need(cols <= 1 or t.stride(1) == 1, f"{name}'s rows must be dense")
+    if t.shape[0] <= 1:
+        return cols
+    _need(t.stride(0) >= cols, f"{name}'s rows overlap")
+    return t.stride(0)
+
+
+def bread_matmul(w, x, y, rows: int, cols: int, qtype: int, bias=None, act=None, residual=None, stream=None) -> None:
+    """y[t] = act(W x[t] + bias) + residual[t] for the rows t of x: torch.float16
+    [n_tokens][cols], y (and residual, which may be y) float16 or float32
+    [n_tokens][rows], bias float32 [rows]; rows of x and y may be strided.
+    act: None, "silu", "gelu", "gelu_tanh" or "relu"."""
+    _need(x.dtype == torch.float16, "x must be float16")
+    _need(y.dtype in (torch.float16, torch.float32), "y must be float16 or float32")
+    _need(act in ACTS, f"unknown activation {act!r}")
+    _need(x.dim() == 2 and y.dim() == 2 and x.shape[0] == y.shape[0], "x and y must have a row a token")
+    xs, ys = _rows_of(x, "x", cols), _rows_of(y, "y", rows)
+    _need(qtype not in _WEIGHT_BLOCKS or cols <= 0 or rows < 0 or
+          w.numel() * w.element_size() >= rows * (-(-cols // _WEIGHT_BLOCKS[qtype][0])) * _WEIGHT_BLOCKS[qtype][1],
+          "w holds fewer than rows x cols weights")
+    o = _lib.MatmulOpts(None, None, ACTS[act], _lib.QTYPE_F32 if y.dtype == torch.float32 else QTYPE_F16, xs, ys)
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == rows,
+              "bias must be float32 [rows]")
+        o.bias = bias.data_ptr()
+    if residual is not None:
+        _need(residual.dtype == y.dtype and residual.shape == y.shape and _rows_of(residual, "residual", rows) == ys,
+              "residual must have y's type, shape and stride")
+        o.residual = residual.data_ptr()
+    st = _on(stream, w, x, y, bias, residual)
+    rc = lib.bread_matmul(w.data_ptr(), x.data_ptr(), y.data_ptr(), rows, cols, qtype, x.shape[0], ctypes.byref(o), st)
+    if rc:
+        check(rc, "bread_matmul")
 
 
 def bread_dequant_rows(w, qtype: int, rows: int, cols: int, out=None, stream=None) -> torch.Tensor:
@@ -117,6 +175,7 @@ def shape(hidden=2048, expert_inter=512, shared_inter=512, n_experts=256, top_k=
 # the specialised kernels take; each entry may be Q4_K or Q6_K.
 STANDARD_TYPES = (QTYPE_Q4_K, QTYPE_Q4_K, QTYPE_Q6_K, QTYPE_Q4_K, QTYPE_Q4_K, QTYPE_Q6_K)
 BLOCK_BYTES = {QTYPE_Q4_K: 144, QTYPE_Q6_K: 210}
+_WEIGHT_BLOCKS = {QTYPE_Q4_K: (256, 144), QTYPE_Q6_K: (256, 210), QTYPE_Q8_0: (32, 34), QTYPE_F16: (1, 2)}
 
 
 def row_bytes(qtype: int, cols: int) -> int:
@@ -160,6 +219,44 @@ def route_noalloc(s: MoeShape, layer: MoeLayer, x: torch.Tensor, n_tokens: int, 
     check(lib.bread_route_noalloc(ctypes.byref(s), ctypes.byref(layer), _p(x), n_tokens, _p(idx), _p(w), _p(gsh),
                                   _s(stream)), "bread_route_noalloc")
     return idx, w, gsh
+
+
+class RouteRule:
+    """bread_route_rule_t: how experts are chosen from router logits (scores by
+    "softmax" or "sigmoid", a bias float32 [n_experts] that only steers the
+    choice, top_groups of n_groups groups by their group_top largest choices,
+    weights renormalised and scaled).  Holds the bias tensor."""
+
+    def __init__(self, score: str = "softmax", bias: torch.Tensor | None = None, n_groups: int = 1,
+                 top_groups: int = 1, group_top: int = 1, renorm: bool = True, scale: float = 1.0):
+        _need(score in ("softmax", "sigmoid"), f"unknown score {score!r}")
+        _need(bias is None or (bias.dtype == torch.float32 and bias.dim() == 1 and bias.is_contiguous()),
+              "bias must be float32 [n_experts]")
+        self.bias = bias
+        self.desc = _lib.RouteRuleDesc(
+            None if bias is None else bias.data_ptr(),
+            _lib.SCORE_SIGMOID if score == "sigmoid" else _lib.SCORE_SOFTMAX, n_groups, top_groups, group_top,
+            int(renorm), scale)
+
+    def check(self, n_experts: int) -> None:
+        _need(self.bias is None or self.bias.numel() == n_experts, "the rule's bias must have n_experts values")
+
+
+def route_select(logits: torch.Tensor, top_k: int, rule: RouteRule, stream=None):
+    """bread_route_select over the rows of a 2-d float32 device tensor (rows
+    may be strided): (indices int32, weights float32), each [n_tokens][top_k]."""
+    _need(logits.dtype == torch.float32 and logits.dim() == 2, "logits must be float32 [n_tokens][n_experts]")
+    T, E = logits.shape
+    rule.check(E)
+    ls = _rows_of(logits, "logits", E)
+    st = _on(stream, logits, rule.bias)
+    idx = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
+    w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    rc = lib.bread_route_select(ctypes.byref(rule.desc), logits.data_ptr(), ls, E, top_k, T, idx.data_ptr(),
+                                w.data_ptr(), st)
+    if rc:
+        check(rc, "bread_route_select")
+    return idx, w
 
 
 @dataclass
@@ -456,6 +553,73 @@ class MoeContext:
         check(lib.bread_moe_forward(self._h, ctypes.byref(layer), _p(x), _p(hidden), n_tokens, _p(idx), _p(w),
                                     _p(gsh), _s(stream)), "bread_moe_forward")
         return idx, w, gsh
+
+    def route_by_rule(self, layer: MoeLayer, rule: RouteRule, x: torch.Tensor, n_tokens: int, stream=None):
+        """bread_route_by_rule: route() with the experts and weights of a rule."""
+        K = self.shape.top_k
+        rule.check(self.shape.n_experts)
+        st = _on(stream, x, rule.bias)
+        idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
+        w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
+        gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+        check(lib.bread_route_by_rule(self._h, ctypes.byref(layer), ctypes.byref(rule.desc), _p(x), n_tokens, _p(idx),
+                                      _p(w), _p(gsh), st), "bread_route_by_rule")
+        return idx, w, gsh
+
+    def forward_by_rule(self, layer: MoeLayer, rule: RouteRule, x: torch.Tensor, hidden: torch.Tensor, n_tokens: int,
+                        want_routing: bool = False, stream=None):
+        """bread_moe_forward_by_rule: forward() with the experts and weights of a rule."""
+        K = self.shape.top_k
+        rule.check(self.shape.n_experts)
+        st = _on(stream, x, hidden, rule.bias)
+        idx = w = gsh = None
+        if want_routing:
+            idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
+            w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
+            gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+        check(lib.bread_moe_forward_by_rule(self._h, ctypes.byref(layer), ctypes.byref(rule.desc), _p(x), _p(hidden),
+                                            n_tokens, _p(idx), _p(w), _p(gsh), st), "bread_moe_forward_by_rule")
+        return idx, w, gsh
+
+    def spec_verify(self, logits: torch.Tensor, tokens: torch.Tensor, offsets: torch.Tensor, u: torch.Tensor,
+                    draft_probs: torch.Tensor | None = None, temperature: torch.Tensor | None = None, eos: int = -1,
+                    want_logprob: bool = True, stream=None):
+        """bread_spec_verify: (accepted drafts int32 [n_requests], next tokens int32
+        [n_requests], log-probabilities float32 [n_rows] or None).  logits
+        [n_rows][vocab] float16 or float32, tokens int32 and u float32 [n_rows],
+        offsets int32 [n_requests + 1], draft_probs float32
+        [n_rows - n_requests][vocab] or None, temperature float32 [n_requests]."""
+        _need(logits.dim() == 2 and logits.dtype in (torch.float16, torch.float32),
+              "logits must be float16 or float32 [n_rows][vocab]")
+        R, V = logits.shape
+        for t, name, kind in ((tokens, "tokens", torch.int32), (offsets, "offsets", torch.int32),
+                              (u, "u", torch.float32)):
+            _need(t.dtype == kind and t.dim() == 1 and t.is_contiguous(), f"{name} must be dense, 1-d and {kind}")
+        B = offsets.numel() - 1
+        _need(B >= 0 and tokens.numel() == R and u.numel() == R, "offsets, tokens or u do not fit the rows of logits")
+        a = _lib.VerifyArgs()
+        a.logits, a.logits_stride = logits.data_ptr(), _rows_of(logits, "logits", V)
+        a.logits_type = _lib.QTYPE_F32 if logits.dtype == torch.float32 else QTYPE_F16
+        a.vocab, a.n_rows, a.n_requests, a.eos = V, R, B, eos
+        if draft_probs is not None and R > B:
+            _need(draft_probs.dtype == torch.float32 and draft_probs.dim() == 2 and draft_probs.shape[0] == R - B,
+                  "draft_probs must be float32 [n_rows - n_requests][vocab]")
+            a.draft_probs, a.draft_probs_stride = draft_probs.data_ptr(), _rows_of(draft_probs, "draft_probs", V)
+        if temperature is not None:
+            _need(temperature.dtype == torch.float32 and temperature.is_contiguous() and temperature.numel() == B,
+                  "temperature must be float32 [n_requests]")
+            a.temperature = temperature.data_ptr()
+        st = _on(stream, logits, tokens, offsets, u, draft_probs, temperature)
+        out = torch.empty((2, B), dtype=torch.int32, device=logits.device)
+        logp = torch.empty((R,), dtype=torch.float32, device=logits.device) if want_logprob else None
+        a.tokens, a.offsets, a.u = tokens.data_ptr(), offsets.data_ptr(), u.data_ptr()
+        a.n_accept, a.next = out.data_ptr(), out.data_ptr() + 4 * B
+        if logp is not None:
+            a.logprob = logp.data_ptr()
+        rc = lib.bread_spec_verify(self._h, ctypes.byref(a), st)
+        if rc:
+            check(rc, "bread_spec_verify")
+        return out[0], out[1], logp
 
     def expert_block(self, layer: MoeLayer, x: torch.Tensor, hidden: torch.Tensor, n_tokens: int,
                      idx: torch.Tensor, w: torch.Tensor, stream=None) -> None:

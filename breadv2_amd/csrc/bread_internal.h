@@ -50,6 +50,7 @@ enum : uint32_t {
     BREAD_DEV_ERR_PAIR = 8u,    // small batch: a wait on the partner wave ran out
     BREAD_DEV_ERR_LOCAL = 16u,  // decode: a wait on another wave of the workgroup ran out
     BREAD_DEV_ERR_INDEX = 32u,  // expert block: a caller's expert index outside [0, n_experts)
+    BREAD_DEV_ERR_OFFSET = 64u, // verification: a request's row offsets are not those of n_rows rows
 };
 
 // Routing outcomes counted on the device (bread_moe_ctx_route_stats).
@@ -122,6 +123,7 @@ struct bread_moe_ctx {
     size_t trace_words;
     bread_grouped_ws gws;
     bread_small_ws sws;
+    uint32_t *vcount;  // [max_tokens] finished workgroups of a verification's request, zero between calls
     int64_t spin_limit = -1;  // sleeps a bounded wait allows; < 0: each kernel's default
 };
 
@@ -184,8 +186,17 @@ int bread_validate_layer(const bread_moe_shape_t *s, const bread_moe_layer_t *L)
 // Launchers implemented in the .hip translation units.
 int bread_launch_route(bread_moe_ctx_t *ctx, const bread_moe_layer_t *L, const float *x,
                        int n_tokens, int32_t *idx, float *w, float *gsh, hipStream_t st);
+// With a rule (NULL: route_layer's own) the router's logits are summed in the
+// reference's order and the rule selects from them.
 int bread_launch_moe_multi(bread_moe_ctx_t *ctx, const bread_moe_layer_t *L, const float *x,
-                           float *hidden, int n_tokens, hipStream_t st);
+                           float *hidden, int n_tokens, hipStream_t st, const bread_route_rule_t *rule = nullptr);
+// Routing by a rule (route_rule.hip): from logits, and from activations
+// (logits in the reference's order into the context's buffer).
+int bread_validate_rule(const bread_route_rule_t *r, int E, int K);
+int bread_launch_route_rule(const bread_route_rule_t *r, const float *logits, int64_t stride, int E, int K, int T,
+                            int32_t *idx, float *w, hipStream_t st);
+int bread_launch_route_by_rule(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const bread_route_rule_t *r,
+                               const float *x, int T, int32_t *idx, float *w, float *gsh, hipStream_t st);
 int bread_launch_topk(const float *logits, int E, int K, int T, int32_t *idx, float *w, hipStream_t st);
 // Router logits in the reference's sequential order (route.hip): logits
 // [T][E]; with shg_row also the shared-gate score of every token into gsh.
@@ -203,13 +214,13 @@ int bread_grouped_alloc(bread_moe_ctx_t *ctx);
 void bread_grouped_free(bread_moe_ctx_t *ctx);
 bool bread_grouped_supported(const bread_moe_shape_t &s, const bread_moe_layer_t *L);
 int bread_launch_moe_grouped(bread_moe_ctx_t *ctx, const bread_moe_layer_t *L, const float *x, float *hidden,
-                             int n_tokens, hipStream_t st);
+                             int n_tokens, hipStream_t st, const bread_route_rule_t *rule = nullptr);
 int bread_small_alloc(bread_moe_ctx_t *ctx);
 void bread_small_free(bread_moe_ctx_t *ctx);
 bool bread_small_supported(const bread_moe_shape_t &s, const bread_moe_layer_t *L);
 int bread_small_max_tokens();
 int bread_launch_moe_small(bread_moe_ctx_t *ctx, const bread_moe_layer_t *L, const float *x, float *hidden,
-                           int n_tokens, hipStream_t st);
+                           int n_tokens, hipStream_t st, const bread_route_rule_t *rule = nullptr);
 // One token (token index tok of the call: its routing lands at record tok
 // of the context's routing buffers).
 int bread_launch_moe_decode(bread_moe_ctx_t *ctx, const bread_moe_layer_t *L, const float *x,

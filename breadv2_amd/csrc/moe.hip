@@ -143,6 +143,8 @@ extern "C" int bread_moe_ctx_create(const bread_moe_shape_t *shape, int max_toke
     if (e == hipSuccess) e = hipMalloc((void **)&c->xbuf, bread_decode_xbuf_floats() * sizeof(float));
     if (e == hipSuccess) e = hipMalloc((void **)&c->hbuf, bread_decode_hbuf_floats() * sizeof(float));
     if (e == hipSuccess) e = hipMalloc((void **)&c->dsync, sizeof(bread_decode_sync));
+    if (e == hipSuccess) e = hipMalloc((void **)&c->vcount, T * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMemset(c->vcount, 0, T * sizeof(uint32_t));
     if (e == hipSuccess && bread_decode_reset(c) != BREAD_OK) e = hipErrorUnknown;
     if (e == hipSuccess) e = hipMalloc(&c->d_layers, (size_t)c->max_layers * bread_decode_layer_record_bytes());
     if (e == hipSuccess) {
@@ -182,6 +184,7 @@ extern "C" int bread_moe_ctx_destroy(bread_moe_ctx_t *c)
     (void)hipFree(c->xbuf);
     (void)hipFree(c->hbuf);
     (void)hipFree(c->dsync);
+    (void)hipFree(c->vcount);
     (void)hipFree(c->d_layers);
     bread_grouped_free(c);
     bread_small_free(c);
@@ -538,10 +541,11 @@ static void launch_down(const bread_moe_ctx_t *c, const bread_moe_layer_t *L, co
 }
 
 int bread_launch_moe_multi(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const float *x, float *hidden, int T,
-                           hipStream_t st)
+                           hipStream_t st, const bread_route_rule_t *rule)
 {
     const bread_moe_shape_t &s = c->shape;
-    int rc = bread_launch_route(c, L, x, T, c->idx, c->w, c->gsh, st);
+    int rc = rule ? bread_launch_route_by_rule(c, L, rule, x, T, c->idx, c->w, c->gsh, st)
+                  : bread_launch_route(c, L, x, T, c->idx, c->w, c->gsh, st);
     if (rc) return rc;
     const int Imax = s.expert_inter > s.shared_inter ? s.expert_inter : s.shared_inter;
     const uint64_t gu_waves = (uint64_t)T * (s.top_k + 1) * Imax;
@@ -650,12 +654,11 @@ static bool grouped_takes_mix(const bread_moe_shape_t &s, const bread_moe_layer_
            ((uintptr_t)hidden & 15) == 0;
 }
 
-extern "C" int bread_moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const float *x, float *hidden,
-                                 int T, int32_t *idx, float *w, float *gsh, bread_stream_t stream)
+// bread_moe_forward, and with a rule bread_moe_forward_by_rule
+static int moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const bread_route_rule_t *rule, const float *x,
+                       float *hidden, int T, int32_t *idx, float *w, float *gsh, bread_stream_t stream)
 {
-    int rc = check_tokens(c, L, x, T);
-    if (rc) return rc;
-    BREAD_REQUIRE(hidden, BREAD_ERR_ARG, "NULL hidden");
+    int rc = BREAD_OK;
     if (T == 0) return BREAD_OK;
     hipStream_t st = to_hip(stream);
     c->last_stream = st;
@@ -666,26 +669,28 @@ extern "C" int bread_moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L,
     switch (c->path) {
     case BREAD_PATH_DECODE:
         BREAD_REQUIRE(T == 1, BREAD_ERR_SHAPE, "the decode path takes one token");
+        BREAD_REQUIRE(!rule, BREAD_ERR_SHAPE, "the decode path routes by softmax only");
         rc = bread_launch_moe_decode(c, L, x, hidden, st);
         if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, "bread_moe_forward", "shape not supported by the decode kernel");
         break;
     case BREAD_PATH_GROUPED:
-        rc = bread_launch_moe_grouped(c, L, x, hidden, T, st);
+        rc = bread_launch_moe_grouped(c, L, x, hidden, T, st, rule);
         if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, "bread_moe_forward", "shape not supported by the grouped path");
         break;
     case BREAD_PATH_PER_TOKEN:
-        rc = bread_launch_moe_multi(c, L, x, hidden, T, st);
+        rc = bread_launch_moe_multi(c, L, x, hidden, T, st, rule);
         break;
     case BREAD_PATH_SMALL:
-        rc = bread_launch_moe_small(c, L, x, hidden, T, st);
+        rc = bread_launch_moe_small(c, L, x, hidden, T, st, rule);
         if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, "bread_moe_forward", "shape not supported by the small-batch path");
         break;
     default:
-        rc = (T == 1) ? bread_launch_moe_decode(c, L, x, hidden, st) : BREAD_ERR_SHAPE;
-        if (rc == BREAD_ERR_SHAPE && T <= bread_small_auto_tokens()) rc = bread_launch_moe_small(c, L, x, hidden, T, st);
+        rc = (T == 1 && !rule) ? bread_launch_moe_decode(c, L, x, hidden, st) : BREAD_ERR_SHAPE;
+        if (rc == BREAD_ERR_SHAPE && T <= bread_small_auto_tokens())
+            rc = bread_launch_moe_small(c, L, x, hidden, T, st, rule);
         if (rc == BREAD_ERR_SHAPE && (bread_standard_qtypes(L) || grouped_takes_mix(c->shape, L, T, hidden)))
-            rc = bread_launch_moe_grouped(c, L, x, hidden, T, st);
-        if (rc == BREAD_ERR_SHAPE) rc = bread_launch_moe_multi(c, L, x, hidden, T, st);
+            rc = bread_launch_moe_grouped(c, L, x, hidden, T, st, rule);
+        if (rc == BREAD_ERR_SHAPE) rc = bread_launch_moe_multi(c, L, x, hidden, T, st, rule);
     }
     if (rc) return rc;
     const int K = c->shape.top_k;
@@ -693,6 +698,40 @@ extern "C" int bread_moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L,
     if (w) BREAD_HIP(hipMemcpyAsync(w, c->w, (size_t)T * K * sizeof(float), hipMemcpyDeviceToDevice, st));
     if (gsh) BREAD_HIP(hipMemcpyAsync(gsh, c->gsh, (size_t)T * sizeof(float), hipMemcpyDeviceToDevice, st));
     return BREAD_OK;
+}
+
+extern "C" int bread_moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const float *x, float *hidden,
+                                 int T, int32_t *idx, float *w, float *gsh, bread_stream_t stream)
+{
+    const int rc = check_tokens(c, L, x, T);
+    if (rc) return rc;
+    BREAD_REQUIRE(hidden, BREAD_ERR_ARG, "NULL hidden");
+    return moe_forward(c, L, nullptr, x, hidden, T, idx, w, gsh, stream);
+}
+
+extern "C" int bread_moe_forward_by_rule(bread_moe_ctx_t *c, const bread_moe_layer_t *L,
+                                         const bread_route_rule_t *rule, const float *x, float *hidden, int T,
+                                         int32_t *idx, float *w, float *gsh, bread_stream_t stream)
+{
+    int rc = check_tokens(c, L, x, T);
+    if (rc) return rc;
+    BREAD_REQUIRE(hidden, BREAD_ERR_ARG, "NULL hidden");
+    rc = bread_validate_rule(rule, c->shape.n_experts, c->shape.top_k);
+    if (rc) return rc;
+    return moe_forward(c, L, rule, x, hidden, T, idx, w, gsh, stream);
+}
+
+extern "C" int bread_route_by_rule(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const bread_route_rule_t *rule,
+                                   const float *x, int T, int32_t *idx, float *w, float *gsh, bread_stream_t stream)
+{
+    int rc = check_tokens(c, L, x, T);
+    if (rc) return rc;
+    BREAD_REQUIRE(idx && w && gsh, BREAD_ERR_ARG, "NULL output");
+    rc = bread_validate_rule(rule, c->shape.n_experts, c->shape.top_k);
+    if (rc) return rc;
+    if (T == 0) return BREAD_OK;
+    c->last_stream = to_hip(stream);
+    return bread_launch_route_by_rule(c, L, rule, x, T, idx, w, gsh, to_hip(stream));
 }
 
 // The routed experts with the caller's routing (the reference's expert-block

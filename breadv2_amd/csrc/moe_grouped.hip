@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256) void k_mt_topk_xprep(const float *__restrict__
 {
     __shared__ __attribute__((aligned(16))) float s_e[WAVE * MAXV];
     const int t = (int)blockIdx.x;
-    if (wave_id() == 0) {
+    if (logits && wave_id() == 0) {  // NULL: the caller has routed
         int ik;
         float wk;
         topk_wave_exact<MAXV>(logits + (size_t)t * E, E, K, s_e, ik, wk);
@@ -1325,7 +1325,7 @@ bool bread_grouped_supported(const bread_moe_shape_t &s, const bread_moe_layer_t
 }
 
 int bread_launch_moe_grouped(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const float *x, float *hidden, int T,
-                             hipStream_t st)
+                             hipStream_t st, const bread_route_rule_t *rule)
 {
     const bread_moe_shape_t &s = c->shape;
     if (!bread_grouped_supported(s, L)) return BREAD_ERR_SHAPE;
@@ -1341,17 +1341,24 @@ int bread_launch_moe_grouped(bread_moe_ctx_t *c, const bread_moe_layer_t *L, con
     const bool standard = bread_standard_qtypes(L);
     const uint16_t *shg = (const uint16_t *)L->shexp_gate;
     float *gsh = standard ? c->gsh : nullptr;
-    {
+    const float *logits = c->logits;
+    if (rule) {
+        const int rc = bread_launch_route_by_rule(c, L, rule, x, T, c->idx, c->w, c->gsh, st);
+        if (rc) return rc;
+        logits = nullptr;
+        gsh = nullptr;
+        shg = nullptr;
+    } else {
         const int rc = bread_launch_route_logits((const float *)L->router, standard ? nullptr : shg, x, c->logits,
                                                  standard ? nullptr : c->gsh, H, E, T, !standard, st);
         if (rc) return rc;
     }
     if (!standard) shg = nullptr;
     if ((E + WAVE - 1) / WAVE <= 4)
-        hipLaunchKernelGGL(k_mt_topk_xprep<4>, dim3(T), dim3(256), 0, st, c->logits, E, K, c->idx, c->w, x, shg, H, !standard,
+        hipLaunchKernelGGL(k_mt_topk_xprep<4>, dim3(T), dim3(256), 0, st, logits, E, K, c->idx, c->w, x, shg, H, !standard,
                            (uint4 *)g.xop, (uint4 *)g.xsum, g.xexp, gsh);
     else
-        hipLaunchKernelGGL(k_mt_topk_xprep<16>, dim3(T), dim3(256), 0, st, c->logits, E, K, c->idx, c->w, x, shg, H, !standard,
+        hipLaunchKernelGGL(k_mt_topk_xprep<16>, dim3(T), dim3(256), 0, st, logits, E, K, c->idx, c->w, x, shg, H, !standard,
                            (uint4 *)g.xop, (uint4 *)g.xsum, g.xexp, gsh);
     BREAD_HIP(hipGetLastError());
     hipLaunchKernelGGL(k_mt_bucket, dim3(1), dim3(1024), 0, st, c->idx, T, K, E, g.pair_tok, g.pos_of,

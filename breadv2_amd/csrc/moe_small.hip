@@ -149,6 +149,19 @@ __device__ void sb_number_slots(const int *sidx, int E, int K, int T, int32_t *_
     for (int t = tid; t < T; t += RT_THREADS) slot_pair[t] = t * (K + 1);  // slot t / SB_CH, place t % SB_CH
 }
 
+// The slots of experts that are already chosen.  One workgroup.
+__global__ __launch_bounds__(RT_THREADS) void k_sb_slots(const int32_t *__restrict__ idx, int E, int K, int T,
+                                                         int32_t *__restrict__ slot_expert,
+                                                         int32_t *__restrict__ slot_cnt,
+                                                         int32_t *__restrict__ slot_pair,
+                                                         int32_t *__restrict__ n_slots)
+{
+    __shared__ int sidx[SB_MAX_T * MAX_K];
+    for (int i = threadIdx.x; i < T * K; i += RT_THREADS) sidx[i] = idx[i];
+    __syncthreads();
+    sb_number_slots(sidx, E, K, T, slot_expert, slot_cnt, slot_pair, n_slots);
+}
+
 // Softmax / top-k per token with the host's arithmetic (topk_wave_exact) on
 // the reference-order logits, then the slots.  One workgroup.
 template <int MAXV>
@@ -1105,7 +1118,7 @@ void bread_small_free(bread_moe_ctx_t *c)
 }
 
 int bread_launch_moe_small(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const float *x, float *hidden, int T,
-                           hipStream_t st)
+                           hipStream_t st, const bread_route_rule_t *rule)
 {
     const bread_moe_shape_t &s = c->shape;
     if (T < 1 || T > SB_MAX_T || T > c->max_tokens || !bread_small_supported(s, L)) return BREAD_ERR_SHAPE;
@@ -1128,7 +1141,15 @@ int bread_launch_moe_small(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const
     // k_route_fast writes
     const bool cert = bread_route_certified_ok(c, T);
     const bool sw = cert && H == SW_H && I == SW_I && Ish == SW_I && K <= SW_K && T <= SW_MAX_T;
-    if (cert) {
+    if (rule) {
+        // the rule's experts from the reference-order logits; at the decode
+        // shape k_route_fast then writes the activations in fixed point
+        int rc = bread_launch_route_by_rule(c, L, rule, x, T, c->idx, c->w, c->gsh, st);
+        if (rc == BREAD_OK && sw) rc = bread_launch_route_fast(c, L, x, T, c->gsh, c->h, g.xq, st);
+        if (rc) return rc;
+        hipLaunchKernelGGL(k_sb_slots, dim3(1), dim3(RT_THREADS), 0, st, c->idx, E, K, T, g.slot_expert, g.slot_cnt,
+                           g.slot_pair, g.n_slots);
+    } else if (cert) {
         float *radii = c->h;
         const int rc = bread_launch_route_fast(c, L, x, T, c->gsh, radii, sw ? g.xq : nullptr, st);
         if (rc) return rc;

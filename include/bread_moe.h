@@ -99,6 +99,40 @@ int bread_matvec_f32(const void *w, const float *x, float *y, int rows, int cols
 int bread_dequant_rows(const void *w, int qtype, int rows, int cols, float *out,
                        bread_stream_t stream);
 
+/* Activations of bread_matmul's epilogue. */
+#define BREAD_ACT_NONE      0
+#define BREAD_ACT_SILU      1 /* v / (1 + exp(-v)) */
+#define BREAD_ACT_GELU      2 /* v (1 + erf(v / sqrt 2)) / 2 */
+#define BREAD_ACT_GELU_TANH 3 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+#define BREAD_ACT_RELU      4
+
+typedef struct {
+    const float *bias;    /* fp32 [rows], or NULL */
+    const void *residual; /* y's type and stride, or NULL; may be y itself */
+    int act;              /* BREAD_ACT_* */
+    int y_type;           /* BREAD_QTYPE_F16 or BREAD_QTYPE_F32 */
+    int64_t x_stride;     /* elements from one token's row to the next; 0: cols */
+    int64_t y_stride;     /* the same for y and residual; 0: rows */
+} bread_matmul_opts_t;
+
+/* Several tokens through one weight matrix:
+ *   y[t][r] = act(sum_c dequant(W[r,c]) * x[t][c] + bias[r]) + residual[t][r]
+ * for t < n_tokens, r < rows.  The several-token form of bread_matvec, which
+ * the reference calls once per token (main.cu:615-639): W is read once for a
+ * few tokens, and its tiles are shared by many.  qtype is 12 (Q4_K), 14 (Q6_K),
+ * 8 (Q8_0) or 1 (F16); cols must be a multiple of 256 (K-quants), 32 (Q8_0) or
+ * 8 (F16).  x is fp16, bias fp32, y and residual are fp16 or fp32 (y_type).
+ * Products are exact and sums fp32 (fp16 results from Q6_K: weights whose
+ * integer part, scale times code, exceeds 2048 are rounded to 11 bits), and y
+ * is rounded once.  opts NULL: fp16 y, packed rows, no epilogue.  w must be
+ * 16-byte aligned (Q6_K and Q8_0: 4-byte), x 16-byte aligned with a stride
+ * that is a multiple of 8.  y must not overlap x, w or bias, and residual is y
+ * or does not overlap it.  Elements of y between one row's end and the next
+ * row's start are left as they were.  n_tokens or rows 0: nothing is done.  No
+ * workspace: calls on different streams may overlap. */
+int bread_matmul(const void *w, const uint16_t *x, void *y, int rows, int cols, int qtype, int n_tokens,
+                 const bread_matmul_opts_t *opts, bread_stream_t stream);
+
 /* ------------------------------------------------------------------ */
 /* MoE layer                                                           */
 /* ------------------------------------------------------------------ */
@@ -195,7 +229,8 @@ int bread_stack_loop_tokens(void);
  * kernel's wait on a partner wave expired (the workgroup then writes none of
  * its rows of hidden), 16 = a decode workgroup's wait on another of its own
  * waves expired, 32 = bread_moe_expert_block met an expert index outside
- * [0, n_experts).  Outputs of a launch that set a bit are unspecified.  Clears
+ * [0, n_experts), 64 = bread_spec_verify met row offsets that do not fit its
+ * rows (that request gets 0 accepted drafts and token 0).  Outputs of a launch that set a bit are unspecified.  Clears
  * the word and resets the decode exchange state, so the context is usable
  * again. */
 int bread_moe_ctx_check(bread_moe_ctx_t *ctx, int *device_error);
@@ -233,6 +268,45 @@ int bread_route(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer, const floa
  * share the workspace and race; serialise them (one stream, or events). */
 int bread_route_noalloc(const bread_moe_shape_t *shape, const bread_moe_layer_t *layer, const float *d_x,
                         int n_tokens, int32_t *d_idx, float *d_w, float *d_gsh, bread_stream_t stream);
+
+/* Scores of bread_route_rule_t. */
+#define BREAD_SCORE_SOFTMAX 0
+#define BREAD_SCORE_SIGMOID 1
+
+/* A routing rule.  With l the router logits of a token (fp32),
+ *   s_e = softmax(l)_e or 1 / (1 + exp(-l_e));   c_e = s_e + bias_e
+ * the experts form n_groups equal consecutive groups; a group's score is the
+ * sum of its group_top largest c (the only one's in groups of one); the
+ * top_groups groups with the largest scores stay; the top_k experts with the
+ * largest c among them are chosen, in that order, ties everywhere to the lower
+ * index; the weight of rank k is its s (never c), divided by the chosen ones'
+ * sum if renorm, times scale.  Scores and choices are compared in 64 bits.  A
+ * logit of NaN or -inf has score 0; +inf logits share softmax evenly; where
+ * the chosen scores sum to zero, renorm gives weights of zero.
+ * route_layer's own rule (one_layer.cu:983-985) is softmax, no bias, one
+ * group, renorm, scale 1. */
+typedef struct {
+    const float *bias; /* device fp32 [n_experts], or NULL */
+    int score;         /* BREAD_SCORE_* */
+    int n_groups;      /* divides n_experts; 1: no groups */
+    int top_groups;    /* 1 to n_groups, holding at least top_k experts */
+    int group_top;     /* 1 or 2 */
+    int renorm;
+    float scale;
+} bread_route_rule_t;
+
+/* Experts and weights of n_tokens tokens from their router logits by a rule.
+ * d_logits fp32, n_experts (up to 1024) of a token every `stride` floats (0:
+ * n_experts); d_idx int32 and d_w fp32 [n_tokens][top_k], top_k up to 32.  No
+ * workspace: calls on different streams may overlap. */
+int bread_route_select(const bread_route_rule_t *rule, const float *d_logits, int64_t stride, int n_experts,
+                       int top_k, int n_tokens, int32_t *d_idx, float *d_w, bread_stream_t stream);
+
+/* bread_route by a rule: logits in the reference's order (bit-identical to
+ * its host's), then bread_route_select; d_gsh as there. */
+int bread_route_by_rule(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer, const bread_route_rule_t *rule,
+                        const float *d_x, int n_tokens, int32_t *d_idx, float *d_w, float *d_gsh,
+                        bread_stream_t stream);
 
 /* route_layer-compatible shim: one token, results copied to host arrays
  * (idx[K], w[K]) and the raw shared-gate logit returned in *gsh_logit.
@@ -279,6 +353,13 @@ int bread_route_layer_f16(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer, 
 int bread_moe_forward(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer,
                       const float *d_x_normed, float *d_hidden, int n_tokens,
                       int32_t *d_idx, float *d_w, float *d_gsh, bread_stream_t stream);
+
+/* bread_moe_forward with the experts and weights of bread_route_by_rule.  The
+ * decode kernel has route_layer's rule built in, so a single token takes the
+ * small-batch path here; BREAD_PATH_DECODE returns BREAD_ERR_SHAPE. */
+int bread_moe_forward_by_rule(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer,
+                              const bread_route_rule_t *rule, const float *d_x_normed, float *d_hidden,
+                              int n_tokens, int32_t *d_idx, float *d_w, float *d_gsh, bread_stream_t stream);
 
 /* The routed experts of the MoE block with the caller's routing:
  *   hidden[t] += sum_k w[t][k] * expert_{idx[t][k]}(x_t)
@@ -351,6 +432,57 @@ int bread_argmax_f16(const uint16_t *d_logits, int n, int n_tokens, int32_t *d_o
  * last accepted draft, since the reference stops stepping there. */
 int bread_spec_accept(const int32_t *pred, const int32_t *draft, int n_draft, int32_t eos, int max_accept,
                       int *n_accept, int32_t *next);
+
+/* Verification of drafted tokens by sampling, for many requests at once: the
+ * acceptance of main_speculative.cu:477-497 for requests that sample, with
+ * the random numbers given.  Request b has the rows offsets[b] to
+ * offsets[b + 1] - 1 (at least one; offsets[0] = 0, offsets[n_requests] =
+ * n_rows): tokens[r] is the token that was run at row r (the request's first:
+ * its last confirmed token; the others: its drafts in order) and logits[r]
+ * the target's logits after it.  With p_r = softmax(logits[r] /
+ * temperature[b]) and q_r the probabilities that the draft tokens[r + 1] was
+ * drawn from, draft tokens[r + 1] stands when u[r] * q_r(draft) < p_r(draft).
+ * Drafts are judged in order; the request stops at row r
+ *   - where a draft falls: next is drawn from max(p_r - q_r, 0) (from p_r if
+ *     that is zero everywhere);
+ *   - where the draft that stands is eos: next is eos, which n_accept does not
+ *     count (as bread_spec_accept);
+ *   - at its last row: next is drawn from p_r.
+ * n_accept[b] = r - offsets[b].  "Drawn": the lowest token whose cumulative
+ * weight exceeds u[last row of b] times the whole.  Probabilities and sums are
+ * held in 64 bits.
+ * A temperature that is not above 0 is greedy: p_r is 1 at the lowest index of
+ * the largest logit, and the request ends as bread_spec_accept's.  A logit of
+ * NaN counts as -inf (a masked token), +inf logits share p evenly; where
+ * nothing is left no draft stands and next is 0.  Draft probabilities that are
+ * not above 0 (NaN too) count as 0.  Drafts outside [0, vocab) fall.
+ * logprob (optional): log p_r(tokens[r + 1]) for every row with a draft after
+ * it, and in each request's last row log p(next) at the row it stopped at; for
+ * greedy requests at temperature 1.
+ * Every buffer is on the device.  n_rows <= the context's max_tokens; the
+ * partial sums live in its scratch (BREAD_ERR_CAPACITY if a vocabulary is too
+ * large for it: 16 bytes for every 8192 tokens of each row, and 8 of each
+ * request).  Offsets that do not fit set bit 64 of the error word. */
+typedef struct {
+    const void *logits;        /* [n_rows][vocab], fp16 or fp32 */
+    int64_t logits_stride;     /* elements from one row to the next; 0: vocab */
+    int logits_type;           /* BREAD_QTYPE_F16 or BREAD_QTYPE_F32 */
+    int vocab;                 /* up to 2^24 */
+    int n_rows, n_requests;
+    const int32_t *tokens;     /* [n_rows] */
+    const int32_t *offsets;    /* [n_requests + 1] */
+    const float *u;            /* [n_rows], uniform in [0, 1) */
+    const float *draft_probs;  /* fp32 [n_rows - n_requests][vocab], q_r of request b in row r - b; NULL: drafts
+                                  that were looked up, q_r is 1 at the draft */
+    int64_t draft_probs_stride; /* 0: vocab */
+    const float *temperature;  /* [n_requests], or NULL: 1 */
+    int32_t eos;               /* end token, -1: none */
+    int32_t *n_accept;         /* [n_requests] out */
+    int32_t *next;             /* [n_requests] out */
+    float *logprob;            /* [n_rows] out, or NULL */
+} bread_verify_t;
+
+int bread_spec_verify(bread_moe_ctx_t *ctx, const bread_verify_t *args, bread_stream_t stream);
 
 /* One decode token through a stack of MoE layers in a single launch:
  *   for l < n_layers:  x = RMSNorm(hidden) * layers[l].post_norm_w  (eps = shape.rms_eps);
