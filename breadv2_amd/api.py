@@ -42,14 +42,14 @@ def _need(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _on(stream, *tensors) -> int:
-    """The raw stream a call on these tensors goes to (default: torch's current
-    one).  A launch goes to the current device, so the tensors have to be there."""
+def _on(stream, tensors) -> int:
+    """The raw stream a call on these tensors (or None) goes to (default: torch's
+    current one).  A launch goes to the current device, so they have to be there."""
     dev = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
-    return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
 
 
 _HIP = None
@@ -93,16 +93,21 @@ def bread_matvec_f32(w, x, y, rows: int, cols: int, qtype: int, stream=None) -> 
 
 ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU,
         "gelu_tanh": _lib.ACT_GELU_TANH, "relu": _lib.ACT_RELU}
+_Y_TYPES = {torch.float16: _lib.QTYPE_F16, torch.float32: _lib.QTYPE_F32}
 
 
 def _rows_of(t: torch.Tensor, name: str, cols: int) -> int:
     """Elements from one row of a 2-d tensor to the next (rows themselves dense)."""
-    _need(t.dim() == 2 and t.shape[1] == cols, f"{name} must be 2-d with {cols} columns, is {tuple(t.shape)}")
-    _need(cols <= 1 or t.stride(1) == 1, f"{name}'s rows must be dense")
+    if t.dim() != 2 or t.shape[1] != cols:
+        raise ValueError(f"{name} must be 2-d with {cols} columns, is {tuple(t.shape)}")
+    step, one = t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"{name}'s rows must be dense")
     if t.shape[0] <= 1:
         return cols
-    _need(t.stride(0) >= cols, f"{name}'s rows overlap")
-    return t.stride(0)
+    if step < cols:
+        raise ValueError(f"{name}'s rows overlap")
+    return step
 
 
 def bread_matmul(w, x, y, rows: int, cols: int, qtype: int, bias=None, act=None, residual=None, stream=None) -> None:
@@ -110,25 +115,34 @@ def bread_matmul(w, x, y, rows: int, cols: int, qtype: int, bias=None, act=None,
     [n_tokens][cols], y (and residual, which may be y) float16 or float32
     [n_tokens][rows], bias float32 [rows]; rows of x and y may be strided.
     act: None, "silu", "gelu", "gelu_tanh" or "relu"."""
-    _need(x.dtype == torch.float16, "x must be float16")
-    _need(y.dtype in (torch.float16, torch.float32), "y must be float16 or float32")
-    _need(act in ACTS, f"unknown activation {act!r}")
-    _need(x.dim() == 2 and y.dim() == 2 and x.shape[0] == y.shape[0], "x and y must have a row a token")
+    a = ACTS.get(act)
+    if a is None:
+        raise ValueError(f"unknown activation {act!r}")
+    if x.dtype != torch.float16:
+        raise ValueError("x must be float16")
+    kind = y.dtype
+    y_type = _Y_TYPES.get(kind)
+    if y_type is None:
+        raise ValueError("y must be float16 or float32")
     xs, ys = _rows_of(x, "x", cols), _rows_of(y, "y", rows)
-    _need(qtype not in _WEIGHT_BLOCKS or cols <= 0 or rows < 0 or
-          w.numel() * w.element_size() >= rows * (-(-cols // _WEIGHT_BLOCKS[qtype][0])) * _WEIGHT_BLOCKS[qtype][1],
-          "w holds fewer than rows x cols weights")
-    o = _lib.MatmulOpts(None, None, ACTS[act], _lib.QTYPE_F32 if y.dtype == torch.float32 else QTYPE_F16, xs, ys)
+    T = x.shape[0]
+    if y.shape[0] != T:
+        raise ValueError("x and y must have a row a token")
+    block = _WEIGHT_BLOCKS.get(qtype)
+    if block and rows > 0 and cols > 0 and w.numel() * w.element_size() < rows * -(-cols // block[0]) * block[1]:
+        raise ValueError("w holds fewer than rows x cols weights")
+    bp = rp = None
     if bias is not None:
-        _need(bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == rows,
-              "bias must be float32 [rows]")
-        o.bias = bias.data_ptr()
+        if bias.dtype != torch.float32 or not bias.is_contiguous() or bias.numel() != rows:
+            raise ValueError("bias must be float32 [rows]")
+        bp = bias.data_ptr()
     if residual is not None:
-        _need(residual.dtype == y.dtype and residual.shape == y.shape and _rows_of(residual, "residual", rows) == ys,
-              "residual must have y's type, shape and stride")
-        o.residual = residual.data_ptr()
-    st = _on(stream, w, x, y, bias, residual)
-    rc = lib.bread_matmul(w.data_ptr(), x.data_ptr(), y.data_ptr(), rows, cols, qtype, x.shape[0], ctypes.byref(o), st)
+        if residual.dtype != kind or residual.shape[0] != T or _rows_of(residual, "residual", rows) != ys:
+            raise ValueError("residual must have y's type, shape and stride")
+        rp = residual.data_ptr()
+    st = _on(stream, (w, x, y, bias, residual))
+    rc = lib.bread_matmul(w.data_ptr(), x.data_ptr(), y.data_ptr(), rows, cols, qtype, T,
+                          ctypes.byref(_lib.MatmulOpts(bp, rp, a, y_type, xs, ys)), st)
     if rc:
         check(rc, "bread_matmul")
 
@@ -237,23 +251,25 @@ class RouteRule:
             None if bias is None else bias.data_ptr(),
             _lib.SCORE_SIGMOID if score == "sigmoid" else _lib.SCORE_SOFTMAX, n_groups, top_groups, group_top,
             int(renorm), scale)
+        self.ref = ctypes.byref(self.desc)
 
     def check(self, n_experts: int) -> None:
-        _need(self.bias is None or self.bias.numel() == n_experts, "the rule's bias must have n_experts values")
+        if self.bias is not None and self.bias.shape[0] != n_experts:
+            raise ValueError("the rule's bias must have n_experts values")
 
 
 def route_select(logits: torch.Tensor, top_k: int, rule: RouteRule, stream=None):
     """bread_route_select over the rows of a 2-d float32 device tensor (rows
     may be strided): (indices int32, weights float32), each [n_tokens][top_k]."""
-    _need(logits.dtype == torch.float32 and logits.dim() == 2, "logits must be float32 [n_tokens][n_experts]")
+    if logits.dtype != torch.float32 or logits.dim() != 2:
+        raise ValueError("logits must be float32 [n_tokens][n_experts]")
     T, E = logits.shape
     rule.check(E)
     ls = _rows_of(logits, "logits", E)
-    st = _on(stream, logits, rule.bias)
+    st = _on(stream, (logits, rule.bias))
     idx = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
     w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
-    rc = lib.bread_route_select(ctypes.byref(rule.desc), logits.data_ptr(), ls, E, top_k, T, idx.data_ptr(),
-                                w.data_ptr(), st)
+    rc = lib.bread_route_select(rule.ref, logits.data_ptr(), ls, E, top_k, T, idx.data_ptr(), w.data_ptr(), st)
     if rc:
         check(rc, "bread_route_select")
     return idx, w
@@ -558,11 +574,11 @@ class MoeContext:
         """bread_route_by_rule: route() with the experts and weights of a rule."""
         K = self.shape.top_k
         rule.check(self.shape.n_experts)
-        st = _on(stream, x, rule.bias)
+        st = _on(stream, (x, rule.bias))
         idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
         w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
         gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
-        check(lib.bread_route_by_rule(self._h, ctypes.byref(layer), ctypes.byref(rule.desc), _p(x), n_tokens, _p(idx),
+        check(lib.bread_route_by_rule(self._h, ctypes.byref(layer), rule.ref, _p(x), n_tokens, _p(idx),
                                       _p(w), _p(gsh), st), "bread_route_by_rule")
         return idx, w, gsh
 
@@ -571,13 +587,13 @@ class MoeContext:
         """bread_moe_forward_by_rule: forward() with the experts and weights of a rule."""
         K = self.shape.top_k
         rule.check(self.shape.n_experts)
-        st = _on(stream, x, hidden, rule.bias)
+        st = _on(stream, (x, hidden, rule.bias))
         idx = w = gsh = None
         if want_routing:
             idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
             w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
             gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
-        check(lib.bread_moe_forward_by_rule(self._h, ctypes.byref(layer), ctypes.byref(rule.desc), _p(x), _p(hidden),
+        check(lib.bread_moe_forward_by_rule(self._h, ctypes.byref(layer), rule.ref, _p(x), _p(hidden),
                                             n_tokens, _p(idx), _p(w), _p(gsh), st), "bread_moe_forward_by_rule")
         return idx, w, gsh
 
@@ -589,37 +605,41 @@ class MoeContext:
         [n_rows][vocab] float16 or float32, tokens int32 and u float32 [n_rows],
         offsets int32 [n_requests + 1], draft_probs float32
         [n_rows - n_requests][vocab] or None, temperature float32 [n_requests]."""
-        _need(logits.dim() == 2 and logits.dtype in (torch.float16, torch.float32),
-              "logits must be float16 or float32 [n_rows][vocab]")
+        z_type = _Y_TYPES.get(logits.dtype)
+        if z_type is None or logits.dim() != 2:
+            raise ValueError("logits must be float16 or float32 [n_rows][vocab]")
         R, V = logits.shape
-        for t, name, kind in ((tokens, "tokens", torch.int32), (offsets, "offsets", torch.int32),
-                              (u, "u", torch.float32)):
-            _need(t.dtype == kind and t.dim() == 1 and t.is_contiguous(), f"{name} must be dense, 1-d and {kind}")
-        B = offsets.numel() - 1
-        _need(B >= 0 and tokens.numel() == R and u.numel() == R, "offsets, tokens or u do not fit the rows of logits")
-        a = _lib.VerifyArgs()
-        a.logits, a.logits_stride = logits.data_ptr(), _rows_of(logits, "logits", V)
-        a.logits_type = _lib.QTYPE_F32 if logits.dtype == torch.float32 else QTYPE_F16
-        a.vocab, a.n_rows, a.n_requests, a.eos = V, R, B, eos
+        B = offsets.shape[0] - 1
+        for t, name, kind, n in ((tokens, "tokens", torch.int32, R), (offsets, "offsets", torch.int32, B + 1),
+                                 (u, "u", torch.float32, R)):
+            if t.dtype != kind or t.shape != (n,) or n > 1 and t.stride(0) != 1:
+                raise ValueError(f"{name} must be dense {kind} [{n}]")
+        if B < 0:
+            raise ValueError("offsets must hold n_requests + 1 values")
+        qp = tp = lp = None
+        qs = 0
         if draft_probs is not None and R > B:
-            _need(draft_probs.dtype == torch.float32 and draft_probs.dim() == 2 and draft_probs.shape[0] == R - B,
-                  "draft_probs must be float32 [n_rows - n_requests][vocab]")
-            a.draft_probs, a.draft_probs_stride = draft_probs.data_ptr(), _rows_of(draft_probs, "draft_probs", V)
+            if draft_probs.dtype != torch.float32 or draft_probs.shape != (R - B, V):
+                raise ValueError("draft_probs must be float32 [n_rows - n_requests][vocab]")
+            qp, qs = draft_probs.data_ptr(), _rows_of(draft_probs, "draft_probs", V)
         if temperature is not None:
-            _need(temperature.dtype == torch.float32 and temperature.is_contiguous() and temperature.numel() == B,
-                  "temperature must be float32 [n_requests]")
-            a.temperature = temperature.data_ptr()
-        st = _on(stream, logits, tokens, offsets, u, draft_probs, temperature)
-        out = torch.empty((2, B), dtype=torch.int32, device=logits.device)
-        logp = torch.empty((R,), dtype=torch.float32, device=logits.device) if want_logprob else None
-        a.tokens, a.offsets, a.u = tokens.data_ptr(), offsets.data_ptr(), u.data_ptr()
-        a.n_accept, a.next = out.data_ptr(), out.data_ptr() + 4 * B
-        if logp is not None:
-            a.logprob = logp.data_ptr()
+            if temperature.dtype != torch.float32 or temperature.shape != (B,) or B > 1 and temperature.stride(0) != 1:
+                raise ValueError("temperature must be dense float32 [n_requests]")
+            tp = temperature.data_ptr()
+        st = _on(stream, (logits, tokens, offsets, u, draft_probs, temperature))
+        accepted = torch.empty((B,), dtype=torch.int32, device=logits.device)
+        following = torch.empty((B,), dtype=torch.int32, device=logits.device)
+        logp = None
+        if want_logprob:
+            logp = torch.empty((R,), dtype=torch.float32, device=logits.device)
+            lp = logp.data_ptr()
+        a = _lib.VerifyArgs(logits.data_ptr(), _rows_of(logits, "logits", V), z_type, V, R, B, tokens.data_ptr(),
+                            offsets.data_ptr(), u.data_ptr(), qp, qs, tp, eos, accepted.data_ptr(),
+                            following.data_ptr(), lp)
         rc = lib.bread_spec_verify(self._h, ctypes.byref(a), st)
         if rc:
             check(rc, "bread_spec_verify")
-        return out[0], out[1], logp
+        return accepted, following, logp
 
     def expert_block(self, layer: MoeLayer, x: torch.Tensor, hidden: torch.Tensor, n_tokens: int,
                      idx: torch.Tensor, w: torch.Tensor, stream=None) -> None:

@@ -21,8 +21,10 @@ namespace {
 
 constexpr int SV_THREADS = 256;
 constexpr int SV_WAVES = SV_THREADS / WAVE;
-constexpr int SV_PER = 32;                    // logits a thread
-constexpr int SV_CHUNK = SV_THREADS * SV_PER;  // logits a workgroup
+// Logits a thread (PER): 32 once there is work for the whole GPU, 8 below that, where the time is one
+// workgroup's chain of loads and exponentials.  A workgroup's chunk of a row is SV_THREADS times as many.
+constexpr int SV_MANY = 32, SV_FEW = 8;
+constexpr int SV_MAX_CHUNKS = 2048;  // of a row: 2^24 logits in chunks of 8192
 
 // One chunk of a row: the largest logit and the sum of exp((l - max) / T).
 struct SvPart {
@@ -53,40 +55,52 @@ __device__ __forceinline__ float num(float v)
     return v != v ? -__builtin_inff() : v;
 }
 
-template <typename LT>
-__device__ __forceinline__ float logit(const void *base, size_t i)
+// 2^y for y <= 0, to 8e-14 of itself: 2^n p(y - n) with n the nearest whole number and p the polynomial of
+// degree 9 that is 1 at 0 and nearest to 2^f on [-1/2, 1/2] in relative error (by Remez exchange).  1 for 0, and
+// 0 below -1075, for -inf and for NaN (-inf times 1 / an infinite temperature).  18 instructions, where
+// the library's exp takes twice as many.
+__device__ __forceinline__ double exp2_neg(double y)
 {
-    if constexpr (sizeof(LT) == 2) return num(h2f(static_cast<const uint16_t *>(base)[i]));
-    else return num(static_cast<const float *>(base)[i]);
+    y = fmax(y, -1100.0);
+    const double n = __builtin_rint(y), f = y - n;
+    double p = 0x1.89c489e9e3ae4p-24;
+    p = fma(p, f, 0x1.63d0ec28f10f2p-20);
+    p = fma(p, f, 0x1.fffd75179b1a0p-17);
+    p = fma(p, f, 0x1.4308acc67a164p-13);
+    p = fma(p, f, 0x1.5d87ebe42d79dp-10);
+    p = fma(p, f, 0x1.3b2ab717fb0b6p-7);
+    p = fma(p, f, 0x1.c6b08d7a95072p-5);
+    p = fma(p, f, 0x1.ebfbdff823df0p-3);
+    p = fma(p, f, 0x1.62e42fefa08dcp-1);
+    p = fma(p, f, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
-// exp((l - m) / T) for l <= m: 1 where they are equal, infinite ones too; 0 for l = -inf
-__device__ __forceinline__ double weight(float l, float m, double inv_t)
+constexpr double LOG2E = 1.4426950408889634;
+
+// exp((l - m) / T) for l <= m, c2 = log2(e) / T: 1 where they are equal, infinite ones too; 0 for l = -inf
+__device__ __forceinline__ double weight(float l, float m, double c2)
 {
-    // (infinite differences are settled here: an infinite temperature makes inv_t 0)
-    if (l == -__builtin_inff() || (m == __builtin_inff() && l != m)) return 0.0;
-    return l == m ? 1.0 : exp(((double)l - (double)m) * inv_t);
+    if (__builtin_isinf(m)) return l == m && m > 0.f ? 1.0 : 0.0;
+    return exp2_neg(((double)l - (double)m) * c2);
 }
 
-// Eight logits from element i on, of which those at V and beyond read as -inf
+// Eight values from element i on, of which those at V and beyond read as `none`
 template <typename LT>
-__device__ __forceinline__ void load8(const void *base, size_t row, int i, int V, float (&v)[8])
+__device__ __forceinline__ void load8(const LT *row, int i, int V, float none, float (&v)[8])
 {
+    LT h[8];
     if (i + 8 <= V) {
-        if constexpr (sizeof(LT) == 2) {
-            uint16_t h[8];
-            __builtin_memcpy(h, static_cast<const uint16_t *>(base) + row + i, 16);
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = num(h2f(h[k]));
-        } else {
-            float f[8];
-            __builtin_memcpy(f, static_cast<const float *>(base) + row + i, 32);
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = num(f[k]);
-        }
+        __builtin_memcpy(h, row + i, sizeof(h));  // aligned to an element
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = i + k < V ? logit<LT>(base, row + i + k) : -__builtin_inff();
+        for (int k = 0; k < 8; k++) h[k] = i + k < V ? row[i + k] : LT(0);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        if constexpr (sizeof(LT) == 2) v[k] = num(h2f(h[k]));
+        else v[k] = num(h[k]);
+        if (i + k >= V) v[k] = none;
     }
 }
 
@@ -107,10 +121,11 @@ __device__ __forceinline__ int request_of(const int32_t *off, int B, int row)
     return n;
 }
 
-__device__ __forceinline__ double inverse(const float *temp, int b)
+// log2(e) / temperature; a greedy request's log-probabilities are those of temperature 1
+__device__ __forceinline__ double scale2(const float *temp, int b)
 {
     const float t = temp ? temp[b] : 1.0f;
-    return t > 0.f ? 1.0 / (double)t : 1.0;
+    return t > 0.f ? LOG2E / (double)t : LOG2E;
 }
 
 __device__ __forceinline__ bool greedy(const float *temp, int b)
@@ -119,22 +134,24 @@ __device__ __forceinline__ bool greedy(const float *temp, int b)
 }
 
 // Workgroup b: chunk b % nchunk of row b / nchunk.
-template <typename LT>
+template <typename LT, int PER>
 __global__ __launch_bounds__(SV_THREADS) void k_sv_stats(const SvArgs a)
 {
     __shared__ float s_m[SV_WAVES];
     __shared__ double s_s[SV_WAVES];
     __shared__ int s_i[SV_WAVES];
     const int row = (int)blockIdx.x / a.nchunk, ch = (int)blockIdx.x % a.nchunk, tid = (int)threadIdx.x, wv = wave_id();
-    const size_t base = (size_t)row * a.stride;
-    float v[SV_PER / 8][8], m = -__builtin_inff();
+    const LT *z = static_cast<const LT *>(a.logits) + (size_t)row * a.stride;
+    float v[PER / 8][8], m = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < SV_PER / 8; j++) {
-        load8<LT>(a.logits, base, ch * SV_CHUNK + (j * SV_THREADS + tid) * 8, a.V, v[j]);
+    for (int j = 0; j < PER / 8; j++)
+        load8<LT>(z, ch * (SV_THREADS * PER) + (j * SV_THREADS + tid) * 8, a.V, -__builtin_inff(), v[j]);
+    const int b = request_of(a.off, a.B, row);
+    const double c2 = scale2(a.temp, b);
+#pragma unroll
+    for (int j = 0; j < PER / 8; j++)
 #pragma unroll
         for (int k = 0; k < 8; k++) m = fmaxf(m, v[j][k]);
-    }
-    const double inv_t = inverse(a.temp, request_of(a.off, a.B, row));
     m = wave_max(m);
     if (lane_id() == 0) s_m[wv] = m;
     __syncthreads();
@@ -142,12 +159,23 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_stats(const SvArgs a)
     for (int k = 0; k < SV_WAVES; k++) m = fmaxf(m, s_m[k]);
     double s = 0.0;
     int arg = 0x7FFFFFFF;
+    if (__builtin_isinf(m)) {
 #pragma unroll
-    for (int j = SV_PER / 8 - 1; j >= 0; j--)
+        for (int j = 0; j < PER / 8; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += weight(v[j][k], m, c2);
+    } else {
+        const double md = (double)m;
+#pragma unroll
+        for (int j = 0; j < PER / 8; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += exp2_neg(((double)v[j][k] - md) * c2);
+    }
+#pragma unroll
+    for (int j = PER / 8 - 1; j >= 0; j--)
 #pragma unroll
         for (int k = 7; k >= 0; k--) {
-            const int i = ch * SV_CHUNK + (j * SV_THREADS + tid) * 8 + k;
-            s += weight(v[j][k], m, inv_t);
+            const int i = ch * (SV_THREADS * PER) + (j * SV_THREADS + tid) * 8 + k;
             if (v[j][k] == m && i < a.V) arg = i;
         }
     s = sum_f64(s);
@@ -173,14 +201,14 @@ struct SvRow {
     int arg;
 };
 
-__device__ __forceinline__ SvRow row_stats(const SvArgs &a, int row, double inv_t)
+__device__ __forceinline__ SvRow row_stats(const SvArgs &a, int row, double c2)
 {
     const SvPart *p = a.part + (size_t)row * a.nchunk;
     SvRow r{0.0, -__builtin_inff(), 0x7FFFFFFF};
     for (int c = lane_id(); c < a.nchunk; c += WAVE) r.max = fmaxf(r.max, p[c].max);
     r.max = wave_max(r.max);
     for (int c = lane_id(); c < a.nchunk; c += WAVE) {
-        r.sum += p[c].sum * weight(p[c].max, r.max, inv_t);
+        r.sum += p[c].sum * weight(p[c].max, r.max, c2);
         if (p[c].max == r.max) r.arg = min(r.arg, p[c].arg);
     }
     r.sum = sum_f64(r.sum);
@@ -188,10 +216,10 @@ __device__ __forceinline__ SvRow row_stats(const SvArgs &a, int row, double inv_
     return r;
 }
 
-__device__ __forceinline__ float log_p(float l, const SvRow &r, double inv_t)
+__device__ __forceinline__ float log_p(float l, const SvRow &r, double c2)
 {
     if (!(r.sum > 0.0) || l == -__builtin_inff() || (r.max == __builtin_inff() && l != r.max)) return -__builtin_inff();
-    return (float)((l == r.max ? 0.0 : ((double)l - (double)r.max) * inv_t) - log(r.sum));
+    return (float)((l == r.max ? 0.0 : ((double)l - (double)r.max) * (c2 / LOG2E)) - log(r.sum));
 }
 
 // What is left of token i's weight e (its probability times the row's sum) when
@@ -201,30 +229,42 @@ struct SvLeft {
     const float *q;  // the draft's row of probabilities, or NULL
     int one;         // the looked-up draft, or -1
     double sum;
-    __device__ __forceinline__ double operator()(double e, int i) const
+    __device__ __forceinline__ double operator()(double e, int i, float x) const
     {
         if (q) {
-            const float x = q[i];
             const double d = e - (x > 0.f ? (double)x * sum : 0.0);
             return d > 0.0 ? d : 0.0;
         }
         return i == one ? 0.0 : e;
+    }
+    // What eight tokens from i on leave (those at V and beyond: nothing)
+    template <typename LT>
+    __device__ __forceinline__ void eight(const LT *z, int i, int V, float m, double c2, double (&d)[8]) const
+    {
+        float l[8], x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        load8<LT>(z, i, V, -__builtin_inff(), l);
+        if (q) load8<float>(q, i, V, 0.f, x);
+#pragma unroll
+        for (int k = 0; k < 8; k++) d[k] = (*this)(weight(l[k], m, c2), i + k, x[k]);
     }
 };
 
 // Workgroup i: chunk i % nchunk for request i / nchunk.  Every workgroup of a request judges its drafts, then sums
 // one chunk of what is left at the row where it stopped; the last one to finish
 // draws the token.
-template <typename LT>
+template <typename LT, int PER>
 __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
 {
     __shared__ int s_stop[SV_WAVES], s_pass[SV_WAVES];
     __shared__ SvRow s_row[SV_WAVES];
-    __shared__ double s_d[SV_WAVES];
+    __shared__ double s_d[SV_WAVES], s_tot[SV_MAX_CHUNKS];
     __shared__ int s_win, s_last;
     const int b = (int)blockIdx.x / a.nchunk, ch = (int)blockIdx.x % a.nchunk;
     const int tid = (int)threadIdx.x, wv = wave_id(), lane = lane_id();
     const int r0 = a.off[b], r1 = a.off[b + 1];
+    const bool gr = greedy(a.temp, b);
+    const double c2 = scale2(a.temp, b);
+    const LT *z0 = static_cast<const LT *>(a.logits);
     // rows of no request's, or draft rows past the probabilities': nothing is judged
     if (r0 < b || r1 <= r0 || r1 > a.R || r1 - 2 - b >= a.R - a.B) {
         if (ch == 0 && tid == 0) {
@@ -234,25 +274,32 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
         }
         return;
     }
-    const bool gr = greedy(a.temp, b);
-    const double inv_t = inverse(a.temp, b);
     // wave w judges the rows r0 + w, r0 + w + 4, ...; its first that stops
     int stop = 0x7FFFFFFF, pass = 0;
     SvRow mine{0.0, 0.f, 0};
     for (int r = r0 + wv; r < r1; r += SV_WAVES) {
         if (stop != 0x7FFFFFFF && !(ch == 0 && a.logp)) break;
-        const SvRow s = row_stats(a, r, inv_t);
+        bool in = false;
+        int d = -1;
+        float l = -__builtin_inff(), qd = 1.0f, u = 0.f;
+        if (r + 1 < r1) {
+            d = a.tokens[r + 1];
+            u = a.u[r];
+            in = d >= 0 && d < a.V;
+            if (in) {
+                if constexpr (sizeof(LT) == 2) l = num(h2f(z0[(size_t)r * a.stride + d]));
+                else l = num(z0[(size_t)r * a.stride + d]);
+                if (a.q) qd = a.q[(size_t)(r - b) * a.qstride + d];
+            }
+        }
+        const SvRow s = row_stats(a, r, c2);
         bool ok = false, ends = true;
         if (r + 1 < r1) {
-            const int d = a.tokens[r + 1];
-            const bool in = d >= 0 && d < a.V;
-            const float l = in ? logit<LT>(a.logits, (size_t)r * a.stride + d) : -__builtin_inff();
-            double p = in && s.sum > 0.0 ? weight(l, s.max, inv_t) / s.sum : 0.0;
+            double p = in && s.sum > 0.0 ? weight(l, s.max, c2) / s.sum : 0.0;
             if (gr) p = in && d == s.arg && s.sum > 0.0 ? 1.0 : 0.0;
-            const float qd = a.q && in ? a.q[(size_t)(r - b) * a.qstride + d] : 1.0f;
-            ok = (double)a.u[r] * (qd > 0.f ? (double)qd : 0.0) < p;
+            ok = (double)u * (qd > 0.f ? (double)qd : 0.0) < p;
             ends = d == a.eos;
-            if (ch == 0 && a.logp && lane == 0) a.logp[r] = log_p(l, s, inv_t);
+            if (ch == 0 && a.logp && lane == 0) a.logp[r] = log_p(l, s, c2);
         }
         if (stop == 0x7FFFFFFF && (!ok || ends)) {
             stop = r;
@@ -272,14 +319,19 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
         if (s_stop[k] < s_stop[at]) at = k;
     const int row = s_stop[at];
     const SvRow rs = s_row[at];
-    const size_t base = (size_t)row * a.stride;
+    const LT *z = z0 + (size_t)row * a.stride;
     const bool ended = s_pass[at];  // the end token stood
     auto answer = [&](int token) {
         a.accepted[b] = row - r0;
         a.next[b] = token;
-        if (a.logp)
-            a.logp[r1 - 1] = token >= 0 && token < a.V ? log_p(logit<LT>(a.logits, base + token), rs, inv_t)
-                                                       : -__builtin_inff();
+        if (a.logp) {
+            float l = -__builtin_inff();
+            if (token >= 0 && token < a.V) {
+                if constexpr (sizeof(LT) == 2) l = num(h2f(z[token]));
+                else l = num(z[token]);
+            }
+            a.logp[r1 - 1] = log_p(l, rs, c2);
+        }
     };
     if (ended || gr || !(rs.sum > 0.0)) {
         if (ch == 0 && tid == 0) answer(ended ? a.tokens[row + 1] : rs.sum > 0.0 ? rs.arg : 0);
@@ -292,13 +344,11 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
     }
     double s = 0.0;
 #pragma unroll
-    for (int j = 0; j < SV_PER / 8; j++) {
-        const int i0 = ch * SV_CHUNK + (j * SV_THREADS + tid) * 8;
-        float v[8];
-        load8<LT>(a.logits, base, i0, a.V, v);
+    for (int j = 0; j < PER / 8; j++) {
+        double d[8];
+        left.template eight<LT>(z, ch * (SV_THREADS * PER) + (j * SV_THREADS + tid) * 8, a.V, rs.max, c2, d);
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (i0 + k < a.V) s += left(weight(v[k], rs.max, inv_t), i0 + k);
+        for (int k = 0; k < 8; k++) s += d[k];
     }
     s = sum_f64(s);
     if (lane == 0) s_d[wv] = s;
@@ -310,64 +360,76 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
         const uint32_t n = __hip_atomic_fetch_add(&a.count[b], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         s_last = n + 1 == (uint32_t)a.nchunk;
         if (s_last) __hip_atomic_store(&a.count[b], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_win = 0x7FFFFFFF;
     }
     __syncthreads();
     if (!s_last) return;
-    // chunk sums in order: the chunk that holds the border (each thread looks at all of them)
-    auto chunk_sum = [&](int c, bool whole) {
-        if (!whole)
-            return __hip_atomic_load(&a.tot[(size_t)b * a.nchunk + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const SvPart &p = a.part[(size_t)row * a.nchunk + c];
-        return p.sum * weight(p.max, rs.max, inv_t);
+    for (int c = tid; c < a.nchunk; c += SV_THREADS)
+        s_tot[c] = __hip_atomic_load(&a.tot[(size_t)b * a.nchunk + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    // every wave sums the chunks, 64 at a time
+    auto whole_sum = [&] {
+        double t = 0.0;
+        for (int c = lane; c < a.nchunk; c += WAVE) t += s_tot[c];
+        return sum_f64(t);
     };
-    double total = 0.0;
-    for (int c = 0; c < a.nchunk; c++) total += chunk_sum(c, false);
-    const bool whole = !(total > 0.0);  // the draft's probabilities cover the target's: draw from the target's
-    if (whole) {
+    double total = whole_sum();
+    if (!(total > 0.0)) {  // the draft's probabilities cover the target's: draw from the target's
         left = SvLeft{nullptr, -1, rs.sum};
-        total = 0.0;
-        for (int c = 0; c < a.nchunk; c++) total += chunk_sum(c, true);
-    }
-    const double border = (double)a.u[r1 - 1] * total;
-    double before = 0.0;
-    int hit = -1, last_some = 0;
-    double last_before = 0.0;
-    for (int c = 0; c < a.nchunk; c++) {
-        const double x = chunk_sum(c, whole);
-        if (x > 0.0) {
-            last_some = c;
-            last_before = before;
+        __syncthreads();
+        for (int c = tid; c < a.nchunk; c += SV_THREADS) {
+            const SvPart &p = a.part[(size_t)row * a.nchunk + c];
+            s_tot[c] = p.sum * weight(p.max, rs.max, c2);
         }
-        if (hit < 0 && before + x > border) hit = c;
-        if (hit < 0) before += x;
+        __syncthreads();
+        total = whole_sum();
     }
-    if (hit < 0) {  // by rounding: the last token with any weight
-        hit = last_some;
+    // the chunk that the border lies in, and the weight before it; where rounding puts the border past the
+    // end, the last chunk with any weight
+    const double border = (double)a.u[r1 - 1] * total;
+    double before = 0.0, sum = 0.0;
+    int hit = -1, last = 0;
+    double last_before = 0.0;
+    for (int c0 = 0; c0 < a.nchunk && hit < 0; c0 += WAVE) {
+        const double x = c0 + lane < a.nchunk ? s_tot[c0 + lane] : 0.0;
+        const double inc = sum + wave_scan_incl_f64(x);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0);
+        const uint64_t over = __builtin_amdgcn_ballot_w64(x > 0.0 && inc > border);
+        if (over) {
+            hit = c0 + (int)__builtin_ctzll(over);
+            before = readlane_f64(inc - x, hit & 63);
+        } else if (some) {
+            const int w = 63 - (int)__builtin_clzll(some);
+            last = c0 + w;
+            last_before = readlane_f64(inc - x, w);
+        }
+        sum = readlane_f64(inc, 63);
+    }
+    if (hit < 0) {
+        hit = last;
         before = last_before;
     }
-    // inside the chunk: thread t owns 32 consecutive tokens
-    const int i0 = hit * SV_CHUNK + tid * SV_PER;
-    double x[SV_PER], own = 0.0;
+    // inside the chunk: thread t owns PER consecutive tokens
+    const int i0 = hit * (SV_THREADS * PER) + tid * PER;
+    double x[PER], own = 0.0;
 #pragma unroll
-    for (int j = 0; j < SV_PER / 8; j++) {
-        float v[8];
-        load8<LT>(a.logits, base, i0 + 8 * j, a.V, v);
+    for (int j = 0; j < PER / 8; j++) {
+        double d[8];
+        left.template eight<LT>(z, i0 + 8 * j, a.V, rs.max, c2, d);
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int i = i0 + 8 * j + k;
-            x[8 * j + k] = i < a.V ? left(weight(v[k], rs.max, inv_t), i) : 0.0;
-            own += x[8 * j + k];
+            x[8 * j + k] = d[k];
+            own += d[k];
         }
     }
     const double inc = wave_scan_incl_f64(own);
     if (lane == WAVE - 1) s_d[wv] = inc;
-    if (tid == 0) s_win = 0x7FFFFFFF;
     __syncthreads();
     double cum = before + (inc - own);
     for (int k = 0; k < wv; k++) cum += s_d[k];
     int win = 0x7FFFFFFF, some = -1;
 #pragma unroll
-    for (int k = 0; k < SV_PER; k++) {
+    for (int k = 0; k < PER; k++) {
         cum += x[k];
         if (x[k] > 0.0) {
             some = i0 + k;
@@ -386,13 +448,13 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
     if (tid == 0) answer(s_win < 0 ? rs.arg : s_win);
 }
 
-template <typename LT>
+template <typename LT, int PER>
 int launch(const SvArgs &a, hipStream_t st)
 {
     bread_clear_stale_error();
-    hipLaunchKernelGGL(k_sv_stats<LT>, dim3((unsigned)(a.R * a.nchunk)), dim3(SV_THREADS), 0, st, a);
+    hipLaunchKernelGGL((k_sv_stats<LT, PER>), dim3((unsigned)(a.R * a.nchunk)), dim3(SV_THREADS), 0, st, a);
     BREAD_HIP(hipGetLastError());
-    hipLaunchKernelGGL(k_sv_finish<LT>, dim3((unsigned)(a.B * a.nchunk)), dim3(SV_THREADS), 0, st, a);
+    hipLaunchKernelGGL((k_sv_finish<LT, PER>), dim3((unsigned)(a.B * a.nchunk)), dim3(SV_THREADS), 0, st, a);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
 }
@@ -427,7 +489,6 @@ extern "C" int bread_spec_verify(bread_moe_ctx_t *c, const bread_verify_t *v, br
     a.stride = v->logits_stride ? v->logits_stride : v->vocab;
     a.R = v->n_rows;
     a.B = v->n_requests;
-    a.nchunk = (int)(((int64_t)a.V + SV_CHUNK - 1) / SV_CHUNK);
     a.tokens = v->tokens;
     a.off = v->offsets;
     a.u = v->u;
@@ -439,9 +500,15 @@ extern "C" int bread_spec_verify(bread_moe_ctx_t *c, const bread_verify_t *v, br
     const bread_moe_shape_t &s = c->shape;
     const size_t Imax = (size_t)(s.expert_inter > s.shared_inter ? s.expert_inter : s.shared_inter);
     const size_t have = (size_t)c->max_tokens * (s.top_k + 1) * Imax * sizeof(float);
-    const size_t parts = (size_t)a.R * a.nchunk * sizeof(SvPart), tots = (size_t)a.B * a.nchunk * sizeof(double);
-    BREAD_REQUIRE((int64_t)a.R * a.nchunk < (1ll << 31) && parts + tots <= have, BREAD_ERR_CAPACITY,
+    auto chunks = [&](int per) { return (int)(((int64_t)a.V + SV_THREADS * per - 1) / (SV_THREADS * per)); };
+    auto bytes = [&](int per) {
+        return (size_t)chunks(per) * ((size_t)a.R * sizeof(SvPart) + (size_t)a.B * sizeof(double));
+    };
+    BREAD_REQUIRE(bytes(SV_MANY) <= have && (int64_t)a.R * chunks(SV_MANY) < (1ll << 31), BREAD_ERR_CAPACITY,
                   "the context's scratch is too small for this vocabulary: create it for more tokens");
+    const bool few = (int64_t)a.R * chunks(SV_FEW) <= 2048 && chunks(SV_FEW) <= SV_MAX_CHUNKS && bytes(SV_FEW) <= have;
+    a.nchunk = chunks(few ? SV_FEW : SV_MANY);
+    const size_t parts = (size_t)a.R * a.nchunk * sizeof(SvPart);
     a.part = reinterpret_cast<SvPart *>(c->h);
     a.tot = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(c->h) + parts);
     a.count = c->vcount;
@@ -451,5 +518,6 @@ extern "C" int bread_spec_verify(bread_moe_ctx_t *c, const bread_verify_t *v, br
     a.logp = v->logprob;
     const hipStream_t st = to_hip(stream);
     c->last_stream = st;
-    return v->logits_type == BREAD_QTYPE_F16 ? launch<uint16_t>(a, st) : launch<float>(a, st);
+    if (v->logits_type == BREAD_QTYPE_F16) return few ? launch<uint16_t, SV_FEW>(a, st) : launch<uint16_t, SV_MANY>(a, st);
+    return few ? launch<float, SV_FEW>(a, st) : launch<float, SV_MANY>(a, st);
 }
