@@ -24,6 +24,7 @@ constexpr int SV_WAVES = SV_THREADS / WAVE;
 // Logits a thread (PER): 32 once there is work for the whole GPU, 8 below that, where the time is one
 // workgroup's chain of loads and exponentials.  A workgroup's chunk of a row is SV_THREADS times as many.
 constexpr int SV_MANY = 32, SV_FEW = 8;
+constexpr int SV_CHAINS = 4;  // exponentials side by side
 constexpr int SV_MAX_CHUNKS = 2048;  // of a row: 2^24 logits in chunks of 8192
 
 // One chunk of a row: the largest logit and the sum of exp((l - max) / T).
@@ -31,6 +32,13 @@ struct SvPart {
     double sum;
     float max;
     int arg;  // lowest index of the largest logit
+};
+
+// Where a request's draft fell against a draft model's probabilities: what is left there is drawn by k_sv_left.
+struct SvStop {
+    double sum;  // of the row's weights
+    float max;
+    int row;     // -1: the request has its token
 };
 
 struct SvArgs {
@@ -42,6 +50,7 @@ struct SvArgs {
     int64_t qstride;
     int32_t eos;
     SvPart *part;      // [R][nchunk]
+    SvStop *stop;      // [B]
     double *tot;       // [B][nchunk]
     uint32_t *count;   // [B], zero between calls
     uint32_t *err;
@@ -49,58 +58,123 @@ struct SvArgs {
     float *logp;       // may be NULL
 };
 
+// The larger of two, a number against NaN (fmaxf's rule, without the compiler's two extra instructions to quiet
+// its arguments first)
+__device__ __forceinline__ float max2(float a, float b)
+{
+    float d;
+    asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+    return d;
+}
+
 // A logit as a number: NaN counts as -inf
 __device__ __forceinline__ float num(float v)
 {
-    return v != v ? -__builtin_inff() : v;
+    return max2(v, -__builtin_inff());
 }
 
-// 2^y for y <= 0, to 8e-14 of itself: 2^n p(y - n) with n the nearest whole number and p the polynomial of
-// degree 9 that is 1 at 0 and nearest to 2^f on [-1/2, 1/2] in relative error (by Remez exchange).  1 for 0, and
-// 0 below -1075, for -inf and for NaN (-inf times 1 / an infinite temperature).  18 instructions, where
-// the library's exp takes twice as many.
-__device__ __forceinline__ double exp2_neg(double y)
+template <typename LT>
+__device__ __forceinline__ float logit(LT v)
 {
-    y = fmax(y, -1100.0);
-    const double n = __builtin_rint(y), f = y - n;
-    double p = 0x1.89c489e9e3ae4p-24;
-    p = fma(p, f, 0x1.63d0ec28f10f2p-20);
-    p = fma(p, f, 0x1.fffd75179b1a0p-17);
-    p = fma(p, f, 0x1.4308acc67a164p-13);
-    p = fma(p, f, 0x1.5d87ebe42d79dp-10);
-    p = fma(p, f, 0x1.3b2ab717fb0b6p-7);
-    p = fma(p, f, 0x1.c6b08d7a95072p-5);
-    p = fma(p, f, 0x1.ebfbdff823df0p-3);
-    p = fma(p, f, 0x1.62e42fefa08dcp-1);
-    p = fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, (int)n);
+    if constexpr (sizeof(LT) == 2) return num(h2f(v));
+    else return num(v);
 }
+
+// 2^y for y <= 0 by 2^n p(f), n the nearest whole number to y, f = y - n and p the polynomial of degree 9 that is 1
+// at 0 and has the least largest relative error on [-1/2, 1/2], 8e-14 (by Remez exchange).  The coefficients stay
+// in scalar registers: left to itself the compiler moves each to vector registers for every use, two moves for a
+// multiply-add (with the quieting of max's arguments 31 instructions a logit in k_sv_stats, 18 in its loop now).
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+struct Exp2 {
+    double c[9];
+    __device__ __forceinline__ Exp2()
+        : c{0x1.62e42fefa08dcp-1, 0x1.ebfbdff823df0p-3, 0x1.c6b08d7a95072p-5, 0x1.3b2ab717fb0b6p-7, 0x1.5d87ebe42d79dp-10,
+            0x1.4308acc67a164p-13, 0x1.fffd75179b1a0p-17, 0x1.63d0ec28f10f2p-20, 0x1.89c489e9e3ae4p-24}
+    {
+#pragma unroll
+        for (int k = 0; k < 8; k++) asm("" : "+s"(c[k]));
+        asm("" : "+v"(c[8]));  // an instruction takes one scalar operand
+    }
+    __device__ __forceinline__ double part(double f) const
+    {
+        double p = c[8];
+#pragma unroll
+        for (int k = 7; k >= 0; k--) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p) : "v"(p), "v"(f), "s"(c[k]));
+        return fma(p, f, 1.0);
+    }
+    // any y: 1 for 0, and 0 below -1075, for -inf and for NaN (-inf times 1 / an infinite temperature)
+    __device__ __forceinline__ double operator()(double y) const
+    {
+        y = fmax(y, -1100.0);
+        const double n = __builtin_rint(y);
+        return __builtin_amdgcn_ldexp(part(y - n), (int)n);
+    }
+    // The sum of N of them, each y in [-1000, 1]: n comes out of the low bits of y + 1.5 2^52 and goes to the
+    // exponent.  N chains at a time, so that no instruction waits for the one before it.
+    template <int N>
+    __device__ __forceinline__ double sum_mid(const double (&y)[N]) const
+    {
+        double t[N], f[N], p[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) t[i] = y[i] + 0x1.8p52;
+#pragma unroll
+        for (int i = 0; i < N; i++) f[i] = y[i] - (t[i] - 0x1.8p52);
+#pragma unroll
+        for (int i = 0; i < N; i++) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p[i]) : "v"(c[8]), "v"(f[i]), "s"(c[7]));
+#pragma unroll
+        for (int k = 6; k >= 0; k--)
+#pragma unroll
+            for (int i = 0; i < N; i++) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p[i]) : "v"(p[i]), "v"(f[i]), "s"(c[k]));
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            u32x2 q = __builtin_bit_cast(u32x2, fma(p[i], f[i], 1.0));
+            q.y += __builtin_bit_cast(u32x2, t[i]).x << 20;
+            s += __builtin_bit_cast(double, q);
+        }
+        return s;
+    }
+};
 
 constexpr double LOG2E = 1.4426950408889634;
 
 // exp((l - m) / T) for l <= m, c2 = log2(e) / T: 1 where they are equal, infinite ones too; 0 for l = -inf
-__device__ __forceinline__ double weight(float l, float m, double c2)
+__device__ __forceinline__ double weight(const Exp2 &e2, float l, float m, double c2)
 {
     if (__builtin_isinf(m)) return l == m && m > 0.f ? 1.0 : 0.0;
-    return exp2_neg(((double)l - (double)m) * c2);
+    return e2(((double)l - (double)m) * c2);
 }
+
+// Eight logits (or probabilities) as they are stored
+template <typename LT> struct Eight;
+
+template <> struct Eight<uint16_t> {
+    uint32_t w[4];
+    __device__ __forceinline__ float value(int k) const { return h2f(w[k / 2] >> (16 * (k & 1))); }
+    __device__ __forceinline__ void set(int k, uint16_t v)
+    {
+        w[k / 2] = (k & 1) ? (w[k / 2] & 0xFFFFu) | ((uint32_t)v << 16) : v;
+    }
+    static constexpr uint16_t NONE = 0xFC00;  // -inf
+};
+
+template <> struct Eight<float> {
+    float w[8];
+    __device__ __forceinline__ float value(int k) const { return w[k]; }
+    __device__ __forceinline__ void set(int k, float v) { w[k] = v; }
+    static constexpr float NONE = -__builtin_inff();
+};
 
 // Eight values from element i on, of which those at V and beyond read as `none`
 template <typename LT>
-__device__ __forceinline__ void load8(const LT *row, int i, int V, float none, float (&v)[8])
+__device__ __forceinline__ void load8(const LT *row, int i, int V, LT none, Eight<LT> &v)
 {
-    LT h[8];
     if (i + 8 <= V) {
-        __builtin_memcpy(h, row + i, sizeof(h));  // aligned to an element
+        __builtin_memcpy(&v, row + i, sizeof(v));  // aligned to an element
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) h[k] = i + k < V ? row[i + k] : LT(0);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        if constexpr (sizeof(LT) == 2) v[k] = num(h2f(h[k]));
-        else v[k] = num(h[k]);
-        if (i + k >= V) v[k] = none;
+        for (int k = 0; k < 8; k++) v.set(k, i + k < V ? row[i + k] : none);
     }
 }
 
@@ -133,65 +207,125 @@ __device__ __forceinline__ bool greedy(const float *temp, int b)
     return temp && !(temp[b] > 0.f);
 }
 
-// Workgroup b: chunk b % nchunk of row b / nchunk.
+__device__ __forceinline__ uint32_t max2_f16(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+    return d;
+}
+
+// The largest of the values and m, numbers against NaN
+__device__ __forceinline__ float max8(const Eight<float> &v, float m)
+{
+#pragma unroll
+    for (int k = 0; k < 8; k++) m = max2(m, v.w[k]);
+    return m;
+}
+
+__device__ __forceinline__ float max8(const Eight<uint16_t> &v, float m)
+{
+    const uint32_t p = max2_f16(max2_f16(v.w[0], v.w[1]), max2_f16(v.w[2], v.w[3]));
+    return max2(max2(m, h2f(p)), h2f(p >> 16));
+}
+
+// The values, those below `least` and NaN raised to it
+__device__ __forceinline__ Eight<float> raise8(const Eight<float> &v, float least)
+{
+    Eight<float> r;
+#pragma unroll
+    for (int k = 0; k < 8; k++) r.w[k] = max2(v.w[k], least);
+    return r;
+}
+
+__device__ __forceinline__ Eight<uint16_t> raise8(const Eight<uint16_t> &v, float least)
+{
+    const uint32_t h = f2h(least), hh = h | (h << 16);
+    Eight<uint16_t> r;
+#pragma unroll
+    for (int k = 0; k < 4; k++) r.w[k] = max2_f16(v.w[k], hh);
+    return r;
+}
+
+// A chunk a wave (chunk i % nchunk of row i / nchunk), 32 logits a lane at a time and the next ones on their way:
+// the largest so far, and in each lane its own sum relative to it; a larger one scales the sum down.
+// Bound by the 64-bit exponentials: 64 requests with 8 drafts over 248,320 tokens, 143M logits, 119 us on MI355X
+// (2.4 TB/s).  With a chunk a workgroup, 32 logits a thread, a third of the instructions went into its two
+// reductions: 149 us.
 template <typename LT, int PER>
 __global__ __launch_bounds__(SV_THREADS) void k_sv_stats(const SvArgs a)
 {
-    __shared__ float s_m[SV_WAVES];
-    __shared__ double s_s[SV_WAVES];
-    __shared__ int s_i[SV_WAVES];
-    const int row = (int)blockIdx.x / a.nchunk, ch = (int)blockIdx.x % a.nchunk, tid = (int)threadIdx.x, wv = wave_id();
+    constexpr int STEPS = PER * SV_WAVES / 32, STEP = 32 * WAVE;
+    const Exp2 e2;
+    const int lane = lane_id(), at = (int)blockIdx.x * SV_WAVES + wave_id();
+    if (at >= a.R * a.nchunk) return;
+    const int row = at / a.nchunk, i0 = (at - row * a.nchunk) * (STEPS * STEP) + lane * 8;
     const LT *z = static_cast<const LT *>(a.logits) + (size_t)row * a.stride;
-    float v[PER / 8][8], m = -__builtin_inff();
+    Eight<LT> v[4], nx[4];
+    auto load = [&](Eight<LT>(&d)[4], int i) {
 #pragma unroll
-    for (int j = 0; j < PER / 8; j++)
-        load8<LT>(z, ch * (SV_THREADS * PER) + (j * SV_THREADS + tid) * 8, a.V, -__builtin_inff(), v[j]);
+        for (int j = 0; j < 4; j++) load8<LT>(z, i + j * (8 * WAVE), a.V, Eight<LT>::NONE, d[j]);
+    };
+    load(nx, i0);
     const int b = request_of(a.off, a.B, row);
     const double c2 = scale2(a.temp, b);
-#pragma unroll
-    for (int j = 0; j < PER / 8; j++)
-#pragma unroll
-        for (int k = 0; k < 8; k++) m = fmaxf(m, v[j][k]);
-    m = wave_max(m);
-    if (lane_id() == 0) s_m[wv] = m;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < SV_WAVES; k++) m = fmaxf(m, s_m[k]);
-    double s = 0.0;
+    const bool gr = greedy(a.temp, b);
+    float m = -__builtin_inff(), least = 0.f;
+    double s = 0.0, mc = 0.0;
+    bool plain = false;
     int arg = 0x7FFFFFFF;
-    if (__builtin_isinf(m)) {
+    for (int step = 0; step < STEPS; step++) {
 #pragma unroll
-        for (int j = 0; j < PER / 8; j++)
+        for (int j = 0; j < 4; j++) v[j] = nx[j];
+        if (step + 1 < STEPS) load(nx, i0 + (step + 1) * STEP);
+        float ms = -__builtin_inff();
 #pragma unroll
-            for (int k = 0; k < 8; k++) s += weight(v[j][k], m, c2);
-    } else {
-        const double md = (double)m;
-#pragma unroll
-        for (int j = 0; j < PER / 8; j++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) s += exp2_neg(((double)v[j][k] - md) * c2);
-    }
-#pragma unroll
-    for (int j = PER / 8 - 1; j >= 0; j--)
-#pragma unroll
-        for (int k = 7; k >= 0; k--) {
-            const int i = ch * (SV_THREADS * PER) + (j * SV_THREADS + tid) * 8 + k;
-            if (v[j][k] == m && i < a.V) arg = i;
+        for (int j = 0; j < 4; j++) ms = max8(v[j], ms);
+        ms = wave_max(ms);
+        if (ms > m) {
+            s *= weight(e2, m, ms, c2);
+            m = ms;
+            arg = 0x7FFFFFFF;
+            // Logits whose 2^y would have y < -1000 or so, masked ones and NaN too, are raised to `least` and count
+            // as 2^-200 or less next to a sum of at least 1; above it the exponent can be added to the bits.  An
+            // unusual temperature or size, where fp16 (or fp32) has no such value, takes the general form.
+            least = m - 900.f / (float)c2;
+            if constexpr (sizeof(LT) == 2) least = h2f(f2h(least));
+            const double yl = ((double)least - (double)m) * c2;
+            plain = yl >= -1000.0 && yl <= -200.0 && least > -60000.f;
+            mc = -(double)m * c2;
         }
+        if (plain) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const Eight<LT> r = raise8(v[j], least);
+#pragma unroll
+                for (int k = 0; k < 8; k += SV_CHAINS) {
+                    double y[SV_CHAINS];
+#pragma unroll
+                    for (int i = 0; i < SV_CHAINS; i++) y[i] = fma((double)r.value(k + i), c2, mc);
+                    s += e2.sum_mid(y);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) s += weight(e2, num(v[j].value(k)), m, c2);
+        }
+        if (gr && arg == 0x7FFFFFFF) {  // (of the lane; the first step that has the largest has the lane's lowest)
+#pragma unroll
+            for (int j = 3; j >= 0; j--)
+#pragma unroll
+                for (int k = 7; k >= 0; k--) {
+                    const int i = i0 + step * STEP + j * (8 * WAVE) + k;
+                    if (num(v[j].value(k)) == m && i < a.V) arg = i;
+                }
+        }
+    }
     s = sum_f64(s);
-    for (int o = WAVE / 2; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o));
-    if (lane_id() == 0) {
-        s_s[wv] = s;
-        s_i[wv] = arg;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        for (int k = 1; k < SV_WAVES; k++) {
-            s += s_s[k];
-            arg = min(arg, s_i[k]);
-        }
-        a.part[(size_t)row * a.nchunk + ch] = SvPart{s, m, arg};
-    }
+    if (gr)
+        for (int o = WAVE / 2; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o));
+    if (lane == 0) a.part[at] = SvPart{s, m, arg};
 }
 
 // A row's statistics from its chunks, by one wave
@@ -201,14 +335,14 @@ struct SvRow {
     int arg;
 };
 
-__device__ __forceinline__ SvRow row_stats(const SvArgs &a, int row, double c2)
+__device__ __forceinline__ SvRow row_stats(const SvArgs &a, const Exp2 &e2, int row, double c2)
 {
     const SvPart *p = a.part + (size_t)row * a.nchunk;
     SvRow r{0.0, -__builtin_inff(), 0x7FFFFFFF};
     for (int c = lane_id(); c < a.nchunk; c += WAVE) r.max = fmaxf(r.max, p[c].max);
     r.max = wave_max(r.max);
     for (int c = lane_id(); c < a.nchunk; c += WAVE) {
-        r.sum += p[c].sum * weight(p[c].max, r.max, c2);
+        r.sum += p[c].sum * weight(e2, p[c].max, r.max, c2);
         if (p[c].max == r.max) r.arg = min(r.arg, p[c].arg);
     }
     r.sum = sum_f64(r.sum);
@@ -239,35 +373,162 @@ struct SvLeft {
     }
     // What eight tokens from i on leave (those at V and beyond: nothing)
     template <typename LT>
-    __device__ __forceinline__ void eight(const LT *z, int i, int V, float m, double c2, double (&d)[8]) const
+    __device__ __forceinline__ void eight(const Exp2 &e2, const LT *z, int i, int V, float m, double c2, double (&d)[8]) const
     {
-        float l[8], x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        load8<LT>(z, i, V, -__builtin_inff(), l);
+        Eight<LT> l;
+        Eight<float> x{};
+        load8<LT>(z, i, V, Eight<LT>::NONE, l);
         if (q) load8<float>(q, i, V, 0.f, x);
 #pragma unroll
-        for (int k = 0; k < 8; k++) d[k] = (*this)(weight(l[k], m, c2), i + k, x[k]);
+        for (int k = 0; k < 8; k++) d[k] = (*this)(weight(e2, num(l.value(k)), m, c2), i + k, x.w[k]);
     }
 };
 
-// Workgroup i: chunk i % nchunk for request i / nchunk.  Every workgroup of a request judges its drafts, then sums
-// one chunk of what is left at the row where it stopped; the last one to finish
-// draws the token.
+// The chunk that the border lies in and the weight before it, from the chunks' weights in LDS; where rounding
+// puts the border past the end, the last chunk with any weight.  By every wave alike.
+__device__ __forceinline__ void find_chunk(const double *tot, int nchunk, double border, int &hit, double &before)
+{
+    const int lane = lane_id();
+    double sum = 0.0, last_before = 0.0;
+    int last = 0;
+    for (int c0 = 0; c0 < nchunk; c0 += WAVE) {
+        const double x = c0 + lane < nchunk ? tot[c0 + lane] : 0.0;
+        const double inc = sum + wave_scan_incl_f64(x);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0);
+        const uint64_t over = __builtin_amdgcn_ballot_w64(x > 0.0 && inc > border);
+        if (over) {
+            const int w = (int)__builtin_ctzll(over);
+            hit = c0 + w;
+            before = readlane_f64(inc - x, w);
+            return;
+        }
+        if (some) {
+            const int w = 63 - (int)__builtin_clzll(some);
+            last = c0 + w;
+            last_before = readlane_f64(inc - x, w);
+        }
+        sum = readlane_f64(inc, 63);
+    }
+    hit = last;
+    before = last_before;
+}
+
+__device__ __forceinline__ double whole_sum(const double *tot, int nchunk)
+{
+    double t = 0.0;
+    for (int c = lane_id(); c < nchunk; c += WAVE) t += tot[c];
+    return sum_f64(t);
+}
+
+// Sum over the workgroup, in every thread (s_d: one double a wave)
+__device__ __forceinline__ double block_sum(double v, double *s_d)
+{
+    v = sum_f64(v);
+    __syncthreads();
+    if (lane_id() == 0) s_d[wave_id()] = v;
+    __syncthreads();
+    v = s_d[0];
+#pragma unroll
+    for (int k = 1; k < SV_WAVES; k++) v += s_d[k];
+    return v;
+}
+
 template <typename LT, int PER>
-__global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
+__device__ __forceinline__ double chunk_left(const Exp2 &e2, const SvLeft &left, const LT *z, int ch, int V, float max, double c2)
+{
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < PER / 8; j++) {
+        double d[8];
+        left.template eight<LT>(e2, z, ch * (SV_THREADS * PER) + (j * SV_THREADS + (int)threadIdx.x) * 8, V, max, c2, d);
+#pragma unroll
+        for (int k = 0; k < 8; k++) s += d[k];
+    }
+    return s;
+}
+
+// The token at the border, by the workgroup, from the chunks' weights in tot (LDS): the first whose cumulative
+// weight exceeds u times the whole; -1 where there is no weight.
+template <typename LT, int PER>
+__device__ __forceinline__ int draw(const Exp2 &e2, const SvLeft &left, const LT *z, const double *tot, int nchunk, double border, int V,
+                                    float max, double c2, double *s_d, int *s_win)
+{
+    const int tid = (int)threadIdx.x;
+    int hit;
+    double before;
+    find_chunk(tot, nchunk, border, hit, before);
+    // thread t owns PER consecutive tokens of the chunk
+    const int i0 = hit * (SV_THREADS * PER) + tid * PER;
+    double x[PER], own = 0.0;
+#pragma unroll
+    for (int j = 0; j < PER / 8; j++) {
+        double d[8];
+        left.template eight<LT>(e2, z, i0 + 8 * j, V, max, c2, d);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            x[8 * j + k] = d[k];
+            own += d[k];
+        }
+    }
+    const double inc = wave_scan_incl_f64(own);
+    __syncthreads();
+    if (lane_id() == WAVE - 1) s_d[wave_id()] = inc;
+    if (tid == 0) *s_win = 0x7FFFFFFF;
+    __syncthreads();
+    double cum = before + (inc - own);
+    for (int k = 0; k < wave_id(); k++) cum += s_d[k];
+    int win = 0x7FFFFFFF, some = -1;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        cum += x[k];
+        if (x[k] > 0.0) {
+            some = i0 + k;
+            if (win == 0x7FFFFFFF && cum > border) win = i0 + k;
+        }
+    }
+    if (win != 0x7FFFFFFF) atomicMin(s_win, win);
+    __syncthreads();
+    if (*s_win == 0x7FFFFFFF) {  // by rounding: the last token of the chunk with any weight
+        __syncthreads();
+        if (tid == 0) *s_win = -1;
+        __syncthreads();
+        atomicMax(s_win, some);
+        __syncthreads();
+    }
+    return *s_win;
+}
+
+// The request's answer, by one thread
+template <typename LT>
+__device__ __forceinline__ void answer(const SvArgs &a, int b, int row, const LT *z, const SvRow &rs, double c2, int token)
+{
+    a.accepted[b] = row - a.off[b];
+    a.next[b] = token;
+    if (a.logp)
+        a.logp[a.off[b + 1] - 1] = log_p(token >= 0 && token < a.V ? logit(z[token]) : -__builtin_inff(), rs, c2);
+}
+
+// Workgroup b: judges request b's drafts, and draws its token unless a draft
+// fell against a draft model's probabilities (k_sv_left then draws it).  Its
+// time is a chain of loads: offsets, then tokens and chunk statistics, then
+// the drafts' logits, then the chunk that holds the token.
+template <typename LT, int PER>
+__global__ __launch_bounds__(SV_THREADS) void k_sv_judge(const SvArgs a)
 {
     __shared__ int s_stop[SV_WAVES], s_pass[SV_WAVES];
     __shared__ SvRow s_row[SV_WAVES];
     __shared__ double s_d[SV_WAVES], s_tot[SV_MAX_CHUNKS];
-    __shared__ int s_win, s_last;
-    const int b = (int)blockIdx.x / a.nchunk, ch = (int)blockIdx.x % a.nchunk;
-    const int tid = (int)threadIdx.x, wv = wave_id(), lane = lane_id();
+    __shared__ int s_win;
+    const Exp2 e2;
+    const int b = (int)blockIdx.x, tid = (int)threadIdx.x, wv = wave_id(), lane = lane_id();
     const int r0 = a.off[b], r1 = a.off[b + 1];
     const bool gr = greedy(a.temp, b);
     const double c2 = scale2(a.temp, b);
     const LT *z0 = static_cast<const LT *>(a.logits);
+    if (tid == 0) a.stop[b].row = -1;
     // rows of no request's, or draft rows past the probabilities': nothing is judged
     if (r0 < b || r1 <= r0 || r1 > a.R || r1 - 2 - b >= a.R - a.B) {
-        if (ch == 0 && tid == 0) {
+        if (tid == 0) {
             __hip_atomic_fetch_or(a.err, BREAD_DEV_ERR_OFFSET, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             a.accepted[b] = 0;
             a.next[b] = 0;
@@ -278,7 +539,7 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
     int stop = 0x7FFFFFFF, pass = 0;
     SvRow mine{0.0, 0.f, 0};
     for (int r = r0 + wv; r < r1; r += SV_WAVES) {
-        if (stop != 0x7FFFFFFF && !(ch == 0 && a.logp)) break;
+        if (stop != 0x7FFFFFFF && !a.logp) break;
         bool in = false;
         int d = -1;
         float l = -__builtin_inff(), qd = 1.0f, u = 0.f;
@@ -287,19 +548,18 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
             u = a.u[r];
             in = d >= 0 && d < a.V;
             if (in) {
-                if constexpr (sizeof(LT) == 2) l = num(h2f(z0[(size_t)r * a.stride + d]));
-                else l = num(z0[(size_t)r * a.stride + d]);
+                l = logit(z0[(size_t)r * a.stride + d]);
                 if (a.q) qd = a.q[(size_t)(r - b) * a.qstride + d];
             }
         }
-        const SvRow s = row_stats(a, r, c2);
+        const SvRow s = row_stats(a, e2, r, c2);
         bool ok = false, ends = true;
         if (r + 1 < r1) {
-            double p = in && s.sum > 0.0 ? weight(l, s.max, c2) / s.sum : 0.0;
+            double p = in && s.sum > 0.0 ? weight(e2, l, s.max, c2) / s.sum : 0.0;
             if (gr) p = in && d == s.arg && s.sum > 0.0 ? 1.0 : 0.0;
             ok = (double)u * (qd > 0.f ? (double)qd : 0.0) < p;
             ends = d == a.eos;
-            if (ch == 0 && a.logp && lane == 0) a.logp[r] = log_p(l, s, c2);
+            if (a.logp && lane == 0) a.logp[r] = log_p(l, s, c2);
         }
         if (stop == 0x7FFFFFFF && (!ok || ends)) {
             stop = r;
@@ -321,140 +581,104 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_finish(const SvArgs a)
     const SvRow rs = s_row[at];
     const LT *z = z0 + (size_t)row * a.stride;
     const bool ended = s_pass[at];  // the end token stood
-    auto answer = [&](int token) {
-        a.accepted[b] = row - r0;
-        a.next[b] = token;
-        if (a.logp) {
-            float l = -__builtin_inff();
-            if (token >= 0 && token < a.V) {
-                if constexpr (sizeof(LT) == 2) l = num(h2f(z[token]));
-                else l = num(z[token]);
-            }
-            a.logp[r1 - 1] = log_p(l, rs, c2);
-        }
-    };
     if (ended || gr || !(rs.sum > 0.0)) {
-        if (ch == 0 && tid == 0) answer(ended ? a.tokens[row + 1] : rs.sum > 0.0 ? rs.arg : 0);
+        if (tid == 0) answer(a, b, row, z, rs, c2, ended ? a.tokens[row + 1] : rs.sum > 0.0 ? rs.arg : 0);
         return;
     }
-    SvLeft left{nullptr, -1, rs.sum};
-    if (row + 1 < r1) {
-        if (a.q) left.q = a.q + (size_t)(row - b) * a.qstride;
-        else left.one = a.tokens[row + 1];
+    const bool fell = row + 1 < r1;
+    if (fell && a.q) {
+        if (tid == 0) a.stop[b] = SvStop{rs.sum, rs.max, row};
+        return;
     }
-    double s = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER / 8; j++) {
-        double d[8];
-        left.template eight<LT>(z, ch * (SV_THREADS * PER) + (j * SV_THREADS + tid) * 8, a.V, rs.max, c2, d);
-#pragma unroll
-        for (int k = 0; k < 8; k++) s += d[k];
+    // the row's own weights, without the draft that was looked up
+    const SvLeft left{nullptr, fell ? a.tokens[row + 1] : -1, rs.sum};
+    for (int c = tid; c < a.nchunk; c += SV_THREADS) {
+        const SvPart &p = a.part[(size_t)row * a.nchunk + c];
+        s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
     }
-    s = sum_f64(s);
-    if (lane == 0) s_d[wv] = s;
-    __syncthreads();
+    double total = rs.sum;
+    if (left.one >= 0 && left.one < a.V) {
+        // summed again rather than subtracted: the draft may be nearly all there was
+        const int c = left.one / (SV_THREADS * PER);
+        const double x = block_sum(chunk_left<LT, PER>(e2, left, z, c, a.V, rs.max, c2), s_d);
+        if (tid == 0) s_tot[c] = x;
+        __syncthreads();
+        total = whole_sum(s_tot, a.nchunk);
+    } else {
+        __syncthreads();
+    }
+    SvLeft from = left;
+    if (!(total > 0.0)) {  // the draft was all there was
+        from.one = -1;
+        __syncthreads();
+        for (int c = tid; c < a.nchunk; c += SV_THREADS) {
+            const SvPart &p = a.part[(size_t)row * a.nchunk + c];
+            s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
+        }
+        __syncthreads();
+        total = whole_sum(s_tot, a.nchunk);
+    }
+    const int token = draw<LT, PER>(e2, from, z, s_tot, a.nchunk, (double)a.u[r1 - 1] * total, a.V, rs.max, c2, s_d, &s_win);
+    if (tid == 0) answer(a, b, row, z, rs, c2, token);
+}
+
+// Workgroup i: what is left of chunk i % nchunk at the row where a draft of
+// request i / nchunk fell; the request's last one to finish draws the token.
+template <typename LT, int PER>
+__global__ __launch_bounds__(SV_THREADS) void k_sv_left(const SvArgs a)
+{
+    __shared__ double s_d[SV_WAVES], s_tot[SV_MAX_CHUNKS];
+    __shared__ int s_win, s_last;
+    const Exp2 e2;
+    const int b = (int)blockIdx.x / a.nchunk, ch = (int)blockIdx.x % a.nchunk;
+    const int tid = (int)threadIdx.x;
+    const SvStop st = a.stop[b];
+    if (st.row < 0) return;
+    const double c2 = scale2(a.temp, b);
+    const LT *z = static_cast<const LT *>(a.logits) + (size_t)st.row * a.stride;
+    SvLeft left{a.q + (size_t)(st.row - b) * a.qstride, -1, st.sum};
+    const double s = block_sum(chunk_left<LT, PER>(e2, left, z, ch, a.V, st.max, c2), s_d);
     if (tid == 0) {
-        for (int k = 1; k < SV_WAVES; k++) s += s_d[k];
         __hip_atomic_store(&a.tot[(size_t)b * a.nchunk + ch], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // the last workgroup of the request sees every sum, and leaves the counter at zero
-        const uint32_t n = __hip_atomic_fetch_add(&a.count[b], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        // the store has reached where every workgroup sees it before the counter moves; the last workgroup of the
+        // request then sees every sum, and leaves the counter at zero
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint32_t n = __hip_atomic_fetch_add(&a.count[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         s_last = n + 1 == (uint32_t)a.nchunk;
         if (s_last) __hip_atomic_store(&a.count[b], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_win = 0x7FFFFFFF;
     }
     __syncthreads();
     if (!s_last) return;
     for (int c = tid; c < a.nchunk; c += SV_THREADS)
         s_tot[c] = __hip_atomic_load(&a.tot[(size_t)b * a.nchunk + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    // every wave sums the chunks, 64 at a time
-    auto whole_sum = [&] {
-        double t = 0.0;
-        for (int c = lane; c < a.nchunk; c += WAVE) t += s_tot[c];
-        return sum_f64(t);
-    };
-    double total = whole_sum();
+    double total = whole_sum(s_tot, a.nchunk);
     if (!(total > 0.0)) {  // the draft's probabilities cover the target's: draw from the target's
-        left = SvLeft{nullptr, -1, rs.sum};
+        left.q = nullptr;
         __syncthreads();
         for (int c = tid; c < a.nchunk; c += SV_THREADS) {
-            const SvPart &p = a.part[(size_t)row * a.nchunk + c];
-            s_tot[c] = p.sum * weight(p.max, rs.max, c2);
+            const SvPart &p = a.part[(size_t)st.row * a.nchunk + c];
+            s_tot[c] = p.sum * weight(e2, p.max, st.max, c2);
         }
         __syncthreads();
-        total = whole_sum();
+        total = whole_sum(s_tot, a.nchunk);
     }
-    // the chunk that the border lies in, and the weight before it; where rounding puts the border past the
-    // end, the last chunk with any weight
-    const double border = (double)a.u[r1 - 1] * total;
-    double before = 0.0, sum = 0.0;
-    int hit = -1, last = 0;
-    double last_before = 0.0;
-    for (int c0 = 0; c0 < a.nchunk && hit < 0; c0 += WAVE) {
-        const double x = c0 + lane < a.nchunk ? s_tot[c0 + lane] : 0.0;
-        const double inc = sum + wave_scan_incl_f64(x);
-        const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0);
-        const uint64_t over = __builtin_amdgcn_ballot_w64(x > 0.0 && inc > border);
-        if (over) {
-            hit = c0 + (int)__builtin_ctzll(over);
-            before = readlane_f64(inc - x, hit & 63);
-        } else if (some) {
-            const int w = 63 - (int)__builtin_clzll(some);
-            last = c0 + w;
-            last_before = readlane_f64(inc - x, w);
-        }
-        sum = readlane_f64(inc, 63);
-    }
-    if (hit < 0) {
-        hit = last;
-        before = last_before;
-    }
-    // inside the chunk: thread t owns PER consecutive tokens
-    const int i0 = hit * (SV_THREADS * PER) + tid * PER;
-    double x[PER], own = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER / 8; j++) {
-        double d[8];
-        left.template eight<LT>(z, i0 + 8 * j, a.V, rs.max, c2, d);
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            x[8 * j + k] = d[k];
-            own += d[k];
-        }
-    }
-    const double inc = wave_scan_incl_f64(own);
-    if (lane == WAVE - 1) s_d[wv] = inc;
-    __syncthreads();
-    double cum = before + (inc - own);
-    for (int k = 0; k < wv; k++) cum += s_d[k];
-    int win = 0x7FFFFFFF, some = -1;
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-        cum += x[k];
-        if (x[k] > 0.0) {
-            some = i0 + k;
-            if (win == 0x7FFFFFFF && cum > border) win = i0 + k;
-        }
-    }
-    atomicMin(&s_win, win);
-    __syncthreads();
-    if (s_win == 0x7FFFFFFF) {  // by rounding: the last token of the chunk with any weight
-        __syncthreads();
-        if (tid == 0) s_win = -1;
-        __syncthreads();
-        atomicMax(&s_win, some);
-        __syncthreads();
-    }
-    if (tid == 0) answer(s_win < 0 ? rs.arg : s_win);
+    const double border = (double)a.u[a.off[b + 1] - 1] * total;
+    const int token = draw<LT, PER>(e2, left, z, s_tot, a.nchunk, border, a.V, st.max, c2, s_d, &s_win);
+    if (tid == 0) answer(a, b, st.row, z, SvRow{st.sum, st.max, 0}, c2, token < 0 ? 0 : token);
 }
 
 template <typename LT, int PER>
 int launch(const SvArgs &a, hipStream_t st)
 {
     bread_clear_stale_error();
-    hipLaunchKernelGGL((k_sv_stats<LT, PER>), dim3((unsigned)(a.R * a.nchunk)), dim3(SV_THREADS), 0, st, a);
+    const int all = a.R * a.nchunk;
+    hipLaunchKernelGGL((k_sv_stats<LT, PER>), dim3((unsigned)((all + SV_WAVES - 1) / SV_WAVES)), dim3(SV_THREADS), 0, st, a);
     BREAD_HIP(hipGetLastError());
-    hipLaunchKernelGGL((k_sv_finish<LT, PER>), dim3((unsigned)(a.B * a.nchunk)), dim3(SV_THREADS), 0, st, a);
+    hipLaunchKernelGGL((k_sv_judge<LT, PER>), dim3((unsigned)a.B), dim3(SV_THREADS), 0, st, a);
+    BREAD_HIP(hipGetLastError());
+    if (!a.q) return BREAD_OK;
+    hipLaunchKernelGGL((k_sv_left<LT, PER>), dim3((unsigned)(a.B * a.nchunk)), dim3(SV_THREADS), 0, st, a);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
 }
@@ -502,15 +726,16 @@ extern "C" int bread_spec_verify(bread_moe_ctx_t *c, const bread_verify_t *v, br
     const size_t have = (size_t)c->max_tokens * (s.top_k + 1) * Imax * sizeof(float);
     auto chunks = [&](int per) { return (int)(((int64_t)a.V + SV_THREADS * per - 1) / (SV_THREADS * per)); };
     auto bytes = [&](int per) {
-        return (size_t)chunks(per) * ((size_t)a.R * sizeof(SvPart) + (size_t)a.B * sizeof(double));
+        return (size_t)chunks(per) * ((size_t)a.R * sizeof(SvPart) + (size_t)a.B * sizeof(double)) +
+               (size_t)a.B * sizeof(SvStop);
     };
     BREAD_REQUIRE(bytes(SV_MANY) <= have && (int64_t)a.R * chunks(SV_MANY) < (1ll << 31), BREAD_ERR_CAPACITY,
                   "the context's scratch is too small for this vocabulary: create it for more tokens");
     const bool few = (int64_t)a.R * chunks(SV_FEW) <= 2048 && chunks(SV_FEW) <= SV_MAX_CHUNKS && bytes(SV_FEW) <= have;
     a.nchunk = chunks(few ? SV_FEW : SV_MANY);
-    const size_t parts = (size_t)a.R * a.nchunk * sizeof(SvPart);
     a.part = reinterpret_cast<SvPart *>(c->h);
-    a.tot = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(c->h) + parts);
+    a.stop = reinterpret_cast<SvStop *>(a.part + (size_t)a.R * a.nchunk);
+    a.tot = reinterpret_cast<double *>(a.stop + a.B);
     a.count = c->vcount;
     a.err = &c->dsync->error.v;
     a.accepted = v->n_accept;

@@ -461,8 +461,8 @@ int bread_spec_accept(const int32_t *pred, const int32_t *draft, int n_draft, in
  * greedy requests at temperature 1.
  * Every buffer is on the device.  n_rows <= the context's max_tokens; the
  * partial sums live in its scratch (BREAD_ERR_CAPACITY if a vocabulary is too
- * large for it: 16 bytes for every 8192 tokens of each row, and 8 of each
- * request).  Offsets that do not fit set bit 64 of the error word. */
+ * large for it: 16 bytes for every 8192 tokens of each row, and 16, and 8 for
+ * every 8192 tokens, of each request).  Offsets that do not fit set bit 64 of the error word. */
 typedef struct {
     const void *logits;        /* [n_rows][vocab], fp16 or fp32 */
     int64_t logits_stride;     /* elements from one row to the next; 0: vocab */
