@@ -4,10 +4,10 @@
 // W is Q4_K, Q6_K, Q8_0 or fp16, x fp16, sums fp32, y fp16 or fp32.  The
 // reference runs one bread_matvec (kernels.cu:289) per token.
 //
-// k_mm_rows: a workgroup takes 16 weight rows at a time against up to 64
-// tokens; its waves split the columns 256 at a time and join their sums in
-// LDS.  Weights go from memory to registers once, as integers that fp16 holds
-// exactly (a block's scale is applied to the fp32 sum): the products are exact.
+// Weights are unpacked to integers that fp16 holds exactly, and a block's scale
+// is applied to the fp32 sum: the products are exact.  k_mm_rows is for a few
+// tokens (16 weight rows a workgroup at a time, the columns split over its
+// waves), k_mm_tile for more (tiles of tokens by weight rows).
 #include "bread_internal.h"
 #include "q4k_mfma.h"
 
@@ -32,12 +32,29 @@ struct MmArgs {
 // Epilogue
 // ---------------------------------------------------------------------------
 
+// 1 / (1 + exp(-v)): 1 and 0 far out
+__device__ __forceinline__ float sigmoid(float v)
+{
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+}
+
+// The activations to a few 2^-24 of v.  GELU by Abramowitz and Stegun 7.1.26, erfc(x) = exp(-x^2) times a
+// polynomial of 1 / (1 + 0.3275911 x) to 1.5e-7: a third of the library erf's instructions.
 __device__ __forceinline__ float activate(float v, int act)
 {
     switch (act) {
-    case BREAD_ACT_SILU: return v / (1.0f + expf(-v));
-    case BREAD_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    case BREAD_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+    case BREAD_ACT_SILU: return v * sigmoid(v);
+    case BREAD_ACT_GELU: {
+        const float x = fabsf(v) * 0.70710678f;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+        float p = fmaf(1.061405429f, t, -1.453152027f);
+        p = fmaf(p, t, 1.421413741f);
+        p = fmaf(p, t, -0.284496736f);
+        p = fmaf(p, t, 0.254829592f);
+        const float half = 0.5f * p * t * __builtin_amdgcn_exp2f(-1.44269504f * x * x);  // erfc(x) / 2
+        return v * (v < 0.f ? half : 1.0f - half);
+    }
+    case BREAD_ACT_GELU_TANH: return v * sigmoid(1.59576912f * (v + 0.044715f * v * v * v));
     case BREAD_ACT_RELU: return v < 0.f ? 0.f : v;  // NaN stays NaN
     }
     return v;
@@ -54,6 +71,39 @@ __device__ __forceinline__ void put(const MmArgs &a, int t, int r, float v)
     } else {
         if (a.res) v += h2f(static_cast<const uint16_t *>(a.res)[o]);
         static_cast<uint16_t *>(a.y)[o] = f2h(v);
+    }
+}
+
+// Four consecutive rows of a token (y is aligned to an element only)
+__device__ __forceinline__ void put4(const MmArgs &a, int t, int r, const float (&in)[4])
+{
+    if (r + 4 > a.rows) {
+        for (int k = 0; k < 4 && r + k < a.rows; k++) put(a, t, r + k, k == 0 ? in[0] : k == 1 ? in[1] : k == 2 ? in[2] : in[3]);
+        return;
+    }
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = activate(a.bias ? in[k] + a.bias[r + k] : in[k], a.act);
+    const size_t o = (size_t)t * a.ys + r;
+    if (a.y32) {
+        float *y = static_cast<float *>(a.y) + o;
+        if (a.res) {
+            float x[4];
+            __builtin_memcpy(x, static_cast<const float *>(a.res) + o, 16);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] += x[k];
+        }
+        __builtin_memcpy(y, v, 16);
+    } else {
+        uint16_t *y = static_cast<uint16_t *>(a.y) + o, h[4];
+        if (a.res) {
+            __builtin_memcpy(h, static_cast<const uint16_t *>(a.res) + o, 8);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] += h2f(h[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) h[k] = f2h(v[k]);
+        __builtin_memcpy(y, h, 8);
     }
 }
 
@@ -351,6 +401,497 @@ __global__ __launch_bounds__(MR_THREADS) void k_mm_rows(const MmArgs a, int ny, 
     }
 }
 
+// ---------------------------------------------------------------------------
+// Tiles of tokens by weight rows
+// ---------------------------------------------------------------------------
+// k_mm_tile: a wave computes 32 WM tokens by 32 WN rows on v_mfma_f32_32x32x16_f16, MW by NW waves a workgroup.
+// Activations go through LDS (64 columns of the workgroup's tokens at a time, two buffers); weights go from
+// memory to the registers of the lanes that hold their rows, a superblock ahead, and are unpacked there: lane l
+// holds row l % 32 and the half kh = l / 32 of each MFMA's 16 columns, and which columns of a superblock these
+// are is free as long as the activations follow, so that a lane unpacks consecutive bytes.
+//
+// Operands are exact integers as above.  Q4_K and Q6_K: the accumulators are kept in units of the superblock's
+// d, rescaled once a superblock (acc *= d_before / d; a superblock of d = 0 keeps the unit and adds zeros), which
+// needs no second set of accumulators; the min terms sum_j m_j X_j, X_j the activations' sums over a sub-block, are
+// one more MFMA a superblock, with X_j / 32 as a high and a low fp16 part (2^-22 of X_j).  Q8_0: a block of 32 is two
+// MFMAs, whose sum is scaled and added.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(const uint4 &x, h8 w, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x), w, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 zero16()
+{
+    return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+
+// acc += f p, and acc *= f.  The accumulators are named as one register tuple afterwards: as loose values the
+// compiler gives them new registers at every use and moves hundreds of them to memory and back.
+__device__ __forceinline__ void add16(f32x16 &acc, float f, const f32x16 &p)
+{
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = fmaf(f, p[e], acc[e]);
+    asm volatile("" : "+v"(acc));
+}
+
+__device__ __forceinline__ void scale16(f32x16 &acc, float f)
+{
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] *= f;
+    asm volatile("" : "+v"(acc));
+}
+
+// Column of unit u (8 columns) of stage st inside a superblock; unit 4 kh + s is step s of half kh (Q8_0: unit
+// 4 b + 2 kh + s is step 2 b + s, so that a step's halves lie in one block).
+template <int QT>
+__device__ __forceinline__ int unit_column(int st, int u)
+{
+    if (QT == BREAD_QTYPE_Q8_0) return 64 * st + 8 * u;
+    return 128 * (u >> 2) + 32 * st + 8 * (u & 3);
+}
+
+template <int QT>
+__device__ __forceinline__ int step_unit(int kh, int s)
+{
+    return QT == BREAD_QTYPE_Q8_0 ? 4 * (s >> 1) + 2 * kh + (s & 1) : 4 * kh + s;
+}
+
+// A weight row's superblock in LDS, PIECES pieces of 16 bytes as they were loaded (piece p from byte
+// source(p)), STRIDE bytes from one row to the next; and what a lane keeps of it in registers, its half kh.
+template <int QT> struct Share;
+
+template <> struct Share<BREAD_QTYPE_Q4_K> {
+    static constexpr int BYTES = Q4K_BYTES, PIECES = 9, STRIDE = 144;
+    static __device__ __forceinline__ int source(int p) { return 16 * p; }
+    uint4 q[2];      // stages 0 and 1, then 2 and 3
+    uint32_t dd;     // d and dmin
+    uint32_t sc, m;  // scales and mins of the half's four sub-blocks, a byte each
+    h2 S, N;
+    __device__ __forceinline__ void half(const uint8_t *b, int kh, int at)
+    {
+        q[0] = ld_b128(b + 16 + 64 * kh + 32 * at);
+        q[1] = ld_b128(b + 32 + 64 * kh + 32 * at);
+    }
+    __device__ __forceinline__ float take(const uint8_t *b, int kh)
+    {
+        const uint4 head = ld_b128(b);
+        half(b, kh, 0);
+        dd = head.x;
+        const uint32_t s0 = head.y, s1 = head.z, s2 = head.w;
+        sc = kh ? (s2 & 0x0F0F0F0Fu) | ((s0 >> 2) & 0x30303030u) : s0 & 0x3F3F3F3Fu;
+        m = kh ? ((s2 >> 4) & 0x0F0F0F0Fu) | ((s1 >> 2) & 0x30303030u) : s1 & 0x3F3F3F3Fu;
+        return h2f(dd & 0xFFFFu);
+    }
+    __device__ __forceinline__ float dmin() const { return h2f(dd >> 16); }
+    __device__ __forceinline__ void clear() { sc = 0u; }
+    __device__ __forceinline__ void stage(int st)
+    {
+        S = both((float)byte_of(sc, st));
+        N = S * both(-1024.f);
+    }
+    __device__ __forceinline__ h8 step(int st, int s) const
+    {
+        const uint4 &v = q[s >> 1];
+        return q4m_b8(word(v, 2 * (s & 1)), word(v, 2 * (s & 1) + 1), st & 1, S, N);
+    }
+    // the mins as the operand against (X_j / 32 in two parts, the second times 2^11)
+    __device__ __forceinline__ h8 mins() const
+    {
+        const h2 a = magic_lo(m) + both(-1024.f), b = magic_hi(m) + both(-1024.f), f = both(0x1p-11f);
+        return join(a, b, a * f, b * f);
+    }
+};
+
+template <> struct Share<BREAD_QTYPE_Q6_K> {
+    // the last piece ends with the superblock (d is its last two bytes)
+    static constexpr int BYTES = Q6K_BYTES, PIECES = 14, STRIDE = 224;
+    static __device__ __forceinline__ int source(int p) { return p < 13 ? 16 * p : 194; }
+    uint4 l[4], h[2];
+    uint2 sc;
+    h2 S[2];
+    __device__ __forceinline__ float take(const uint8_t *b, int kh)
+    {
+#pragma unroll
+        for (int k = 0; k < 4; k++) l[k] = ld_b128(b + 64 * kh + 16 * k);
+        h[0] = ld_b128(b + 128 + 32 * kh);
+        h[1] = ld_b128(b + 144 + 32 * kh);
+        sc = *reinterpret_cast<const uint2 *>(b + 192 + 8 * kh);
+        return h2f(*reinterpret_cast<const uint16_t *>(b + 222));
+    }
+    __device__ __forceinline__ void clear() { sc = make_uint2(0u, 0u); }
+    // stage st is quarter st: low bytes l[2 (st & 1) ..], their high nibbles from stage 2 on
+    __device__ __forceinline__ void stage(int st)
+    {
+        const uint32_t v = (st < 2 ? sc.x : sc.y) >> (16 * (st & 1));
+        S[0] = both((float)(int8_t)(v & 0xFFu));
+        S[1] = both((float)(int8_t)((v >> 8) & 0xFFu));
+    }
+    __device__ __forceinline__ void codes(int st, int s, uint32_t &v0, uint32_t &v1) const
+    {
+        const int k = 2 * (s & 1);
+        const uint4 &lv = l[2 * (st & 1) + (s >> 1)], &hv = h[s >> 1];
+        v0 = ((word(lv, k) >> (4 * (st >> 1))) & 0x0F0F0F0Fu) | (((word(hv, k) >> (2 * st)) & 0x03030303u) << 4);
+        v1 = ((word(lv, k + 1) >> (4 * (st >> 1))) & 0x0F0F0F0Fu) | (((word(hv, k + 1) >> (2 * st)) & 0x03030303u) << 4);
+    }
+    __device__ __forceinline__ h8 scaled(uint32_t v0, uint32_t v1, h2 off, int s) const
+    {
+        const h2 f = S[s >> 1];
+        return join((magic_lo(v0) + off) * f, (magic_hi(v0) + off) * f, (magic_lo(v1) + off) * f,
+                    (magic_hi(v1) + off) * f);
+    }
+    __device__ __forceinline__ h8 step(int st, int s) const
+    {
+        uint32_t v0, v1;
+        codes(st, s, v0, v1);
+        return scaled(v0, v1, both(-1056.f), s);
+    }
+    // the codes without their low bits, and the low bits alone
+    __device__ __forceinline__ void step2(int st, int s, h8 &hi, h8 &lo) const
+    {
+        uint32_t v0, v1;
+        codes(st, s, v0, v1);
+        hi = scaled(v0 & 0x3E3E3E3Eu, v1 & 0x3E3E3E3Eu, both(-1056.f), s);
+        lo = scaled(v0 & 0x01010101u, v1 & 0x01010101u, both(-1024.f), s);
+    }
+};
+
+template <> struct Share<BREAD_QTYPE_Q8_0> {
+    // 69 dwords from one row to the next: the lanes' dwords lie in different banks
+    static constexpr int BYTES = 8 * Q80_BYTES, PIECES = 17, STRIDE = 276;
+    static __device__ __forceinline__ int source(int p) { return 16 * p; }
+    // four blocks at a time: stages 0 and 1, then 2 and 3
+    uint32_t q[4][4];
+    float d[4];
+    __device__ __forceinline__ void half(const uint8_t *b, int kh, int at)
+    {
+        const int k0 = 4 * at;
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(b) + 4 * kh;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            // block k's bytes begin at 34 k + 2: at a dword for odd k, between two for even k
+            const int at = (34 * (k0 + k) + 2) / 4;
+            uint32_t v[5];
+#pragma unroll
+            for (int i = 0; i < 5; i++) v[i] = i < 4 || !(k & 1) ? w[at + i] : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; i++) q[k][i] = (k & 1) ? v[i] : __builtin_amdgcn_alignbyte(v[i + 1], v[i], 2);
+            d[k] = h2f(reinterpret_cast<const uint16_t *>(b)[17 * (k0 + k)]);
+        }
+    }
+    __device__ __forceinline__ float take(const uint8_t *b, int kh)
+    {
+        half(b, kh, 0);
+        return 1.0f;
+    }
+    __device__ __forceinline__ void stage(int) {}
+    __device__ __forceinline__ h8 step(int st, int s) const
+    {
+        const uint32_t(&v)[4] = q[2 * (st & 1) + (s >> 1)];
+        const uint32_t v0 = v[2 * (s & 1)] ^ 0x80808080u, v1 = v[2 * (s & 1) + 1] ^ 0x80808080u;
+        const h2 off = both(-1152.f);
+        return join(magic_lo(v0) + off, magic_hi(v0) + off, magic_lo(v1) + off, magic_hi(v1) + off);
+    }
+};
+
+// fp16 rows go through LDS like the activations, 64 columns at a time
+template <> struct Share<BREAD_QTYPE_F16> {
+    static constexpr int BYTES = 512, PIECES = 8, STRIDE = 128;
+};
+
+template <int QT, int WM, int WN, int MW, int NW, int KW, bool EXACT>
+__global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a, int mt, int nt)
+{
+    using W = Share<QT>;
+    constexpr int TM = 32 * WM * MW, TN = 32 * WN * NW, THREADS = WAVE * MW * NW;
+    constexpr int XL = TM * 8 / THREADS, WP = TN * W::PIECES, WL = (WP + THREADS - 1) / THREADS;
+    constexpr bool DENSE = QT == BREAD_QTYPE_F16;
+    constexpr int AHEAD = WM * WN > 4 ? 1 : 2;  // stages of activations on their way, and of operands made: registers
+    constexpr bool UNIT = QT == BREAD_QTYPE_Q4_K || QT == BREAD_QTYPE_Q6_K;
+    __shared__ uint4 xs_all[KW][2][TM * 8];
+    // Q4_K: X_j / 32 of every token by superblock parity and half, four high parts, then four low ones
+    __shared__ __attribute__((aligned(16))) uint16_t xm_all[KW][2][QT == BREAD_QTYPE_Q4_K ? TM : 1][2][8];
+    __shared__ __attribute__((aligned(16))) uint8_t ws_all[KW][DENSE ? 2 : 1][TN * W::STRIDE];
+    const int kg = wave_id() / (MW * NW), wv = wave_id() - kg * (MW * NW);  // group of the superblocks, wave in it
+    const int tid = (int)threadIdx.x - kg * THREADS, l = lane_id(), c = l & 31, kh = l >> 5;
+    auto &xs = xs_all[kg];
+    auto &ws = ws_all[kg];
+    auto &xm = xm_all[kg];
+    // the workgroups of one XCD (blockIdx % 8, each with an L2 of its own) take neighbouring tiles
+    const int all = mt * nt, per = (all + 7) / 8;
+    const int ti = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+    if (((int)blockIdx.x >> 3) >= per || ti >= all) return;
+    const int m0 = (ti % mt) * TM, n0 = (ti / mt) * TN;
+    const int wm = wv % MW, wn = wv / MW;
+    const int nsb = (a.cols + 255) / 256, rounds = (nsb + KW - 1) / KW;
+    // activations: the thread's units i THREADS + tid of a stage, unit u of token t at u ^ (t % 8); two stages
+    // on their way.  Byte offsets from the tile's first token (launch_tile checks that they fit).
+    const uint8_t *xbase = reinterpret_cast<const uint8_t *>(a.x + (size_t)m0 * a.xs);
+    uint32_t xo[XL];
+    uint4 xr[AHEAD][XL];
+#pragma unroll
+    for (int i = 0; i < XL; i++) {
+        const int k = i * THREADS + tid, u = (k & 7) ^ ((k >> 3) & 7);
+        xo[i] = (uint32_t)(2 * (min(k >> 3, a.T - 1 - m0) * a.xs + unit_column<QT>(0, u)));
+    }
+    // stage `at` counted over the group's superblocks; past the end the last superblock again, not used
+    auto fetch_x = [&](int at, uint4(&v)[XL]) __attribute__((always_inline)) {
+        const int sb = min((at >> 2) * KW + kg, nsb - 1);
+        const uint8_t *p = xbase + 512 * (size_t)sb + 2 * unit_column<QT>(at & 3, 0);
+        if (!UNIT && a.cols - 256 * sb < 256) {  // the row ends in this superblock: zeros from there
+#pragma unroll
+            for (int i = 0; i < XL; i++) {
+                const int k = i * THREADS + tid, u = (k & 7) ^ ((k >> 3) & 7);
+                v[i] = unit_column<QT>(at & 3, u) < a.cols - 256 * sb ? ld_b128(p + xo[i]) : make_uint4(0u, 0u, 0u, 0u);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < XL; i++) v[i] = ld_b128(p + xo[i]);
+    };
+    auto keep_x = [&](int at, const uint4(&v)[XL]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < XL; i++) {
+            const int k = i * THREADS + tid, t = k >> 3;
+            xs[at & 1][k] = v[i];
+            if constexpr (QT == BREAD_QTYPE_Q4_K) {
+                // the sub-block's four units lie in four lanes; two of them store the parts
+                float x = sum_h8(v[i], 0.f);
+                x += dpp_f<0xB1>(x);  // quad_perm [1,0,3,2]
+                x += dpp_f<0x4E>(x);  // quad_perm [2,3,0,1]
+                x *= 1.0f / 32;
+                const float hi = (float)(_Float16)x;
+                if ((k & 3) < 2)
+                    xm[(at >> 2) & 1][t][((k ^ t) >> 2) & 1][4 * (k & 1) + (at & 3)] = f2h((k & 1) ? (x - hi) * 2048.f : hi);
+            }
+        }
+    };
+    // weights: the thread's pieces i THREADS + tid, adjacent lanes adjacent pieces of a row (a lane a row would
+    // cost the address unit a cycle a lane); rows past the last are the last one again, not stored
+    uint32_t wo[WL];
+    uint4 wr[WL];
+    const uint8_t *wbase = a.w + (size_t)n0 * a.rb;
+#pragma unroll
+    for (int i = 0; i < WL; i++) {
+        const int k = min(i * THREADS + tid, WP - 1), r = k / W::PIECES, piece = k % W::PIECES;
+        wo[i] = (uint32_t)(min(r, a.rows - 1 - n0) * a.rb);
+        if constexpr (DENSE) wo[i] += 2 * unit_column<QT>(0, piece ^ (r & 7));
+        else wo[i] += W::source(piece);
+    }
+    auto fetch_w = [&](int round, int st) __attribute__((always_inline)) {
+        const int sb = min(round * KW + kg, nsb - 1), left = a.cols - 256 * sb;
+        const uint8_t *p = wbase + (size_t)sb * W::BYTES + (DENSE ? 2 * unit_column<QT>(st, 0) : 0);
+        if (!UNIT && left < 256) {  // the row ends in this superblock: nothing is read beyond, the rest is zero
+#pragma unroll
+            for (int i = 0; i < WL; i++) {
+                const int k = min(i * THREADS + tid, WP - 1), piece = k % W::PIECES;
+                if constexpr (DENSE) {
+                    wr[i] = unit_column<QT>(st, piece ^ ((k / W::PIECES) & 7)) < left ? ld_b128(p + wo[i])
+                                                                                      : make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    const int bytes = left / Q80_ELEMS * Q80_BYTES - 16 * piece;
+                    uint32_t v[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int h = 0; h < 8; h++)
+                        if (2 * h < bytes) v[h / 2] |= ldu2(p + wo[i] + 2 * h) << (16 * (h & 1));
+                    wr[i] = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < WL; i++) {
+            if constexpr (QT == BREAD_QTYPE_Q4_K || DENSE) wr[i] = ld_b128(p + wo[i]);
+            else wr[i] = ldu16(p + wo[i]);
+        }
+    };
+    auto keep_w = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < WL; i++) {
+            const int k = i * THREADS + tid;
+            if (WP % THREADS == 0 || k < WP) {
+                uint8_t *p = ws[buf] + (k / W::PIECES) * W::STRIDE + 16 * (k % W::PIECES);
+                if constexpr (W::STRIDE % 16 == 0) {
+                    *reinterpret_cast<uint4 *>(p) = wr[i];
+                } else {
+#pragma unroll
+                    for (int v = 0; v < 4; v++) reinterpret_cast<uint32_t *>(p)[v] = word(wr[i], v);
+                }
+            }
+        }
+    };
+    f32x16 acc[WM][WN];
+#pragma unroll
+    for (int i = 0; i < WM; i++)
+#pragma unroll
+        for (int j = 0; j < WN; j++) acc[i][j] = zero16();
+    float unit[WN];
+#pragma unroll
+    for (int j = 0; j < WN; j++) unit[j] = 1.0f;
+    fetch_w(0, 0);
+    fetch_x(0, xr[0]);
+    if constexpr (AHEAD > 1) fetch_x(1, xr[1]);
+    keep_w(0);
+    keep_x(0, xr[0]);
+    q4m_bar();
+    for (int round = 0; round < rounds; round++) {
+        const bool any = KW == 1 || round * KW + kg < nsb;  // a superblock for this group
+        W w[DENSE ? 1 : WN];
+        if constexpr (!DENSE) if (any) {
+#pragma unroll
+            for (int j = 0; j < WN; j++) {
+                const float d = w[j].take(ws[0] + (32 * (wn * WN + j) + c) * W::STRIDE, kh);
+                if constexpr (UNIT) {
+                    if (d == 0.f) w[j].clear();
+                    const float to = d == 0.f ? unit[j] : d, ratio = unit[j] / to;
+                    unit[j] = to;
+#pragma unroll
+                    for (int i = 0; i < WM; i++) scale16(acc[i][j], ratio);
+                }
+            }
+        }
+#pragma unroll
+        for (int st = 0; st < 4; st++) {
+            const int buf = st & 1;
+            // the activations of two stages on; the next superblock's weights, once for the four stages
+            fetch_x(4 * round + st + AHEAD, xr[st % AHEAD]);
+            if (DENSE) fetch_w(st < 3 ? round : round + 1, (st + 1) & 3);
+            else if (st == 0) fetch_w(round + 1, 0);
+            if (any) {
+            if constexpr (!DENSE) {
+#pragma unroll
+                for (int j = 0; j < WN; j++) {
+                    if constexpr (QT != BREAD_QTYPE_Q6_K) {
+                        if (st == 2) w[j].half(ws[0] + (32 * (wn * WN + j) + c) * W::STRIDE, kh, 1);
+                    }
+                    w[j].stage(st);
+                }
+            }
+            if constexpr (QT == BREAD_QTYPE_Q8_0) {
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    uint4 xa[WM][2];
+#pragma unroll
+                    for (int i = 0; i < WM; i++)
+#pragma unroll
+                        for (int s = 0; s < 2; s++)
+                            xa[i][s] = xs[buf][(32 * (wm * WM + i) + c) * 8 + (step_unit<QT>(kh, 2 * b + s) ^ (c & 7))];
+#pragma unroll
+                    for (int j = 0; j < WN; j++) {
+                        const h8 w0 = w[j].step(st, 2 * b), w1 = w[j].step(st, 2 * b + 1);
+                        const float d = w[j].d[2 * (st & 1) + b];
+#pragma unroll
+                        for (int i = 0; i < WM; i++) {
+                            const f32x16 p = mfma32(xa[i][1], w1, mfma32(xa[i][0], w0, zero16()));
+                            add16(acc[i][j], d, p);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);  // else all partial sums are in flight at once
+                    }
+                }
+            } else {
+                // a step's operands are read and unpacked beside the products of the step before it; the scheduler
+                // is kept to that, else it makes the whole stage's operands first and runs out of registers
+                uint4 xa[AHEAD][WM];
+                h8 wf[AHEAD][WN][EXACT ? 2 : 1];
+                auto operands = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < WM; i++)
+                        xa[s % AHEAD][i] = xs[buf][(32 * (wm * WM + i) + c) * 8 + (step_unit<QT>(kh, s) ^ (c & 7))];
+#pragma unroll
+                    for (int j = 0; j < WN; j++) {
+                        if constexpr (DENSE)
+                            wf[s % AHEAD][j][0] = __builtin_bit_cast(
+                                h8, reinterpret_cast<const uint4 *>(
+                                        ws[buf])[(32 * (wn * WN + j) + c) * 8 + (step_unit<QT>(kh, s) ^ (c & 7))]);
+                        else if constexpr (EXACT)
+                            w[j].step2(st, s, wf[s % AHEAD][j][0], wf[s % AHEAD][j][1]);
+                        else
+                            wf[s % AHEAD][j][0] = w[j].step(st, s);
+                    }
+                };
+                if constexpr (AHEAD > 1) operands(0);
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    if (AHEAD == 1) operands(s);
+                    else if (s < 3) operands(s + 1);
+#pragma unroll
+                    for (int j = 0; j < WN; j++)
+#pragma unroll
+                        for (int i = 0; i < WM; i++) {
+                            acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][0], acc[i][j]);
+                            if constexpr (EXACT) acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][1], acc[i][j]);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            }
+            // every wave has taken its share of the weights before stage 2's barrier
+            if (DENSE) keep_w(buf ^ 1);
+            else if (st == 3) keep_w(0);
+            keep_x(4 * round + st + 1, xr[(st + 1) % AHEAD]);
+            q4m_bar();
+        }
+        if constexpr (QT == BREAD_QTYPE_Q4_K) if (any) {
+#pragma unroll
+            for (int j = 0; j < WN; j++) {
+                const h8 m = w[j].mins();
+                const float f = -32.f * (w[j].dmin() / unit[j]);
+#pragma unroll
+                for (int i = 0; i < WM; i++) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(xm[round & 1][32 * (wm * WM + i) + c][kh]);
+                    add16(acc[i][j], f, mfma32(x, m, zero16()));
+                }
+            }
+        }
+    }
+    // 32 by 32 results at a time through the wave's own part of the activations' buffers, which every wave has
+    // read: lanes then hold four consecutive rows of a token, and the groups' sums are joined, each group taking
+    // its part of the tokens
+    static_assert(2 * WM >= NW && 4 % KW == 0, "4 KB a wave");
+    float *all_out = reinterpret_cast<float *>(&xs_all[0][0][0]), *out = all_out + 1024 * wave_id();
+#pragma unroll
+    for (int j = 0; j < WN; j++)
+#pragma unroll
+        for (int i = 0; i < WM; i++) {
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                out[32 * (8 * (k >> 2) + 4 * kh + (k & 3)) + c] = UNIT ? acc[i][j][k] * unit[j] : acc[i][j][k];
+            if (KW > 1) __syncthreads();
+            else __builtin_amdgcn_wave_barrier();
+            const int r = n0 + 32 * (wn * WN + j) + 4 * (l & 7);
+#pragma unroll 1
+            for (int k = kg * (4 / KW); k < (kg + 1) * (4 / KW); k++) {
+                const int tt = 8 * k + (l >> 3), t = m0 + 32 * (wm * WM + i) + tt;
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < KW; g++) {
+                    const float4 f = *reinterpret_cast<const float4 *>(all_out + 1024 * (g * MW * NW + wv) + 32 * tt + 4 * (l & 7));
+                    v[0] += f.x;
+                    v[1] += f.y;
+                    v[2] += f.z;
+                    v[3] += f.w;
+                }
+                if (t < a.T && r < a.rows) put4(a, t, r, v);
+            }
+            if (KW > 1) __syncthreads();
+            else __builtin_amdgcn_wave_barrier();
+        }
+}
+
+template <int QT, int WM, int WN, int MW, int NW, int KW, bool EXACT>
+int launch_tile(const MmArgs &a, hipStream_t st)
+{
+    const int64_t mt = (a.T + 32 * WM * MW - 1) / (32 * WM * MW), nt = ((int64_t)a.rows + 32 * WN * NW - 1) / (32 * WN * NW);
+    BREAD_REQUIRE(mt * nt < (1ll << 28), BREAD_ERR_SHAPE, "too many tiles");
+    bread_clear_stale_error();
+    hipLaunchKernelGGL((k_mm_tile<QT, WM, WN, MW, NW, KW, EXACT>), dim3((unsigned)((mt * nt + 7) / 8 * 8)),
+                       dim3(WAVE * MW * NW * KW), 0, st, a, (int)mt, (int)nt);
+    BREAD_HIP(hipGetLastError());
+    return BREAD_OK;
+}
+
 template <int QT, bool EXACT>
 int launch_rows(const MmArgs &a, hipStream_t st)
 {
@@ -369,6 +910,44 @@ int launch_rows(const MmArgs &a, hipStream_t st)
     }
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
+}
+
+// The kernel and its tile.  Up to ROWS_T tokens: rows, which read a weight once and have no barrier between
+// its arrival and its products.  Beyond, tiles: the largest that leave something for most of the 256 CUs, since a
+// superblock takes a workgroup about as long for a small tile as for a large one; the smaller ones split the
+// superblocks over groups of waves.  us on MI355X, fp16 results, tokens by
+// 32 x 64, 64 x 64, 128 x 128, 128 x 256 and 256 x 256 tiles:
+//   Q4_K   24 tokens, 2048 x 2048   rows 7.1   9.6   12.5   27.5    39.5    69.1
+//          48         8192 x 2048       32.8  11.4   13.5   30.5    41.9    73.3
+//         256         4096 x 2048       78.6  15.8   14.1   30.8    44.9    81.1
+//        1024         4096 x 2048        274  56.9   55.5   39.4    50.1    84.3
+//        2048         8192 x 2048       1011   220    226    141     109     102
+//   Q6_K  509         2048 x 4096       77.5  37.3   27.5   53.8    80.6     183
+//        1024         8192 x 2048        314   166    113   70.5    57.3     112
+//   Q8_0 1024         4096 x 2048        219  84.0   58.7   38.2    59.9     176
+//        2048         8192 x 2048        866   331    247    145     127     225
+//   fp16 2048         8192 x 2048       1068   338    253    112     112    90.1
+// (256 x 256 of Q6_K and Q8_0 do not fit their registers and are not built.)
+constexpr int ROWS_T = 32;
+constexpr int64_t FILL = 200;  // workgroups
+
+template <int QT, bool EXACT>
+int launch_matmul(const MmArgs &a, hipStream_t st)
+{
+    auto tiles = [&](int64_t m, int64_t n) { return (a.T + m - 1) / m * ((a.rows + n - 1) / n); };
+    // a tile's rows and tokens are addressed by 32-bit offsets
+    if (a.T <= ROWS_T || a.rb >= (1u << 23) || a.xs >= (1 << 22)) return launch_rows<QT, EXACT>(a, st);
+    if constexpr (QT == BREAD_QTYPE_Q4_K || QT == BREAD_QTYPE_F16) {
+        if (tiles(256, 256) >= FILL) return launch_tile<QT, 4, 2, 2, 4, 1, EXACT>(a, st);
+    }
+    if (tiles(128, 256) >= FILL) return launch_tile<QT, 4, 1, 1, 8, 1, EXACT>(a, st);
+    if (tiles(128, 128) >= FILL) return launch_tile<QT, 2, 1, 2, 4, 1, EXACT>(a, st);
+    if (tiles(64, 64) >= FILL) {
+        // (Q6_K unpacks with twice the instructions: a wave's weights against twice the tokens)
+        if constexpr (QT == BREAD_QTYPE_Q6_K) return launch_tile<QT, 2, 1, 1, 2, 4, EXACT>(a, st);
+        else return launch_tile<QT, 1, 1, 2, 2, 4, EXACT>(a, st);
+    }
+    return launch_tile<QT, 1, 1, 1, 2, 4, EXACT>(a, st);
 }
 
 }  // namespace
@@ -419,10 +998,10 @@ extern "C" int bread_matmul(const void *w, const uint16_t *x, void *y, int rows,
     a.y32 = o.y_type == BREAD_QTYPE_F32;
     const hipStream_t st = to_hip(stream);
     switch (qtype) {
-    case BREAD_QTYPE_Q4_K: return launch_rows<BREAD_QTYPE_Q4_K, false>(a, st);
+    case BREAD_QTYPE_Q4_K: return launch_matmul<BREAD_QTYPE_Q4_K, false>(a, st);
     case BREAD_QTYPE_Q6_K:
-        return a.y32 ? launch_rows<BREAD_QTYPE_Q6_K, true>(a, st) : launch_rows<BREAD_QTYPE_Q6_K, false>(a, st);
-    case BREAD_QTYPE_Q8_0: return launch_rows<BREAD_QTYPE_Q8_0, false>(a, st);
-    default: return launch_rows<BREAD_QTYPE_F16, false>(a, st);
+        return a.y32 ? launch_matmul<BREAD_QTYPE_Q6_K, true>(a, st) : launch_matmul<BREAD_QTYPE_Q6_K, false>(a, st);
+    case BREAD_QTYPE_Q8_0: return launch_matmul<BREAD_QTYPE_Q8_0, false>(a, st);
+    default: return launch_matmul<BREAD_QTYPE_F16, false>(a, st);
     }
 }
