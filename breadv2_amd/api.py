@@ -267,8 +267,9 @@ def route_select(logits: torch.Tensor, top_k: int, rule: RouteRule, stream=None)
     rule.check(E)
     ls = _rows_of(logits, "logits", E)
     st = _on(stream, (logits, rule.bias))
-    idx = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
-    w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    dev = logits.device
+    idx = torch.empty(T, top_k, dtype=torch.int32, device=dev)
+    w = torch.empty(T, top_k, dtype=torch.float32, device=dev)
     rc = lib.bread_route_select(rule.ref, logits.data_ptr(), ls, E, top_k, T, idx.data_ptr(), w.data_ptr(), st)
     if rc:
         check(rc, "bread_route_select")
