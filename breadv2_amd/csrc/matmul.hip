@@ -354,7 +354,9 @@ constexpr int MR_MAXTT = 4;  // 16-token tiles a workgroup
 
 // Workgroup b takes row tiles b / ny, b / ny + stride, ... against token tiles
 // [yb NTT, yb NTT + NTT), yb = b % ny.  Wave v owns the chunks v, v + 8, ... of every row.
-template <int QT, int NTT, bool EXACT>
+// HOLD: a row has no more chunks than waves, so that a wave keeps its activations in registers for all its row
+// tiles and loads the next tile's weights while it works on one.
+template <int QT, int NTT, bool EXACT, bool HOLD>
 __global__ __launch_bounds__(MR_THREADS) void k_mm_rows(const MmArgs a, int ny, int stride)
 {
     __shared__ float part[2][MR_WAVES][NTT * 16][17];
@@ -368,20 +370,38 @@ __global__ __launch_bounds__(MR_THREADS) void k_mm_rows(const MmArgs a, int ny, 
         const int t = t0 + 16 * tt + c;  // beyond the last token: the last one again, not stored
         xt[tt] = a.x + (size_t)(t < a.T ? t : a.T - 1) * a.xs;
     }
-    int buf = 0;
-    for (int ti = (int)blockIdx.x / ny; ti < ntile; ti += stride, buf ^= 1) {
+    uint4 xf[NTT][8];
+    Raw<QT> raw;
+    int ti = (int)blockIdx.x / ny, buf = 0;
+    if (HOLD && wv < nw) {
         const int r = 16 * ti + c;
-        const uint8_t *row = a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb;
+        raw.load(a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb, wv, g, a.cols);
+#pragma unroll
+        for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[tt], xt[tt], wv, g, a.cols);
+    }
+    for (; ti < ntile; ti += stride, buf ^= 1) {
         f32x4 out[NTT];
 #pragma unroll
         for (int tt = 0; tt < NTT; tt++) out[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int ch = wv; ch < nch; ch += MR_WAVES) {
-            Raw<QT> raw;
-            raw.load(row, ch, g, a.cols);
-            uint4 xf[NTT][8];
+        if constexpr (HOLD) {
+            if (wv < nw) {
+                Raw<QT> next = raw;
+                if (ti + stride < ntile) {
+                    const int r = 16 * (ti + stride) + c;
+                    next.load(a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb, wv, g, a.cols);
+                }
+                chunk_mma<QT, NTT, EXACT>(raw, xf, out, g);
+                raw = next;
+            }
+        } else {
+            const int r = 16 * ti + c;
+            const uint8_t *row = a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb;
+            for (int ch = wv; ch < nch; ch += MR_WAVES) {
+                raw.load(row, ch, g, a.cols);
 #pragma unroll
-            for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[tt], xt[tt], ch, g, a.cols);
-            chunk_mma<QT, NTT, EXACT>(raw, xf, out, g);
+                for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[tt], xt[tt], ch, g, a.cols);
+                chunk_mma<QT, NTT, EXACT>(raw, xf, out, g);
+            }
         }
         if (wv < nw) {
 #pragma unroll
@@ -849,7 +869,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
     // 32 by 32 results at a time through the wave's own part of the activations' buffers, which every wave has
     // read: lanes then hold four consecutive rows of a token, and the groups' sums are joined, each group taking
     // its part of the tokens
-    static_assert(2 * WM >= NW && 4 % KW == 0, "4 KB a wave");
+    static_assert(2 * WM >= NW, "4 KB a wave");
     float *all_out = reinterpret_cast<float *>(&xs_all[0][0][0]), *out = all_out + 1024 * wave_id();
 #pragma unroll
     for (int j = 0; j < WN; j++)
@@ -862,7 +882,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
             else __builtin_amdgcn_wave_barrier();
             const int r = n0 + 32 * (wn * WN + j) + 4 * (l & 7);
 #pragma unroll 1
-            for (int k = kg * (4 / KW); k < (kg + 1) * (4 / KW); k++) {
+            for (int k = kg * 4 / KW; k < (kg + 1) * 4 / KW; k++) {
                 const int tt = 8 * k + (l >> 3), t = m0 + 32 * (wm * WM + i) + tt;
                 float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -902,11 +922,13 @@ int launch_rows(const MmArgs &a, hipStream_t st)
     if (stride > ntile) stride = ntile;
     const dim3 grid((unsigned)(stride * ny)), block(MR_THREADS);
     bread_clear_stale_error();
+    const bool hold = a.cols <= 256 * MR_WAVES;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, ny, (int)stride); };
     switch (ntt) {
-    case 1: hipLaunchKernelGGL((k_mm_rows<QT, 1, EXACT>), grid, block, 0, st, a, ny, (int)stride); break;
-    case 2: hipLaunchKernelGGL((k_mm_rows<QT, 2, EXACT>), grid, block, 0, st, a, ny, (int)stride); break;
-    case 3: hipLaunchKernelGGL((k_mm_rows<QT, 3, EXACT>), grid, block, 0, st, a, ny, (int)stride); break;
-    default: hipLaunchKernelGGL((k_mm_rows<QT, 4, EXACT>), grid, block, 0, st, a, ny, (int)stride); break;
+    case 1: hold ? go(k_mm_rows<QT, 1, EXACT, true>) : go(k_mm_rows<QT, 1, EXACT, false>); break;
+    case 2: hold ? go(k_mm_rows<QT, 2, EXACT, true>) : go(k_mm_rows<QT, 2, EXACT, false>); break;
+    case 3: go(k_mm_rows<QT, 3, EXACT, false>); break;
+    default: go(k_mm_rows<QT, 4, EXACT, false>); break;
     }
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
@@ -928,6 +950,12 @@ int launch_rows(const MmArgs &a, hipStream_t st)
 //        2048         8192 x 2048        866   331    247    145     127     225
 //   fp16 2048         8192 x 2048       1068   338    253    112     112    90.1
 // (256 x 256 of Q6_K and Q8_0 do not fit their registers and are not built.)
+// Where 32 x 32 tiles are no more than the CUs, a workgroup has one, with its superblocks over eight groups and not
+// four: a round fewer to wait for.  us with 32 x 64 and four groups, and with 32 x 32 and eight:
+//   Q8_0   67 tokens, 2048 x 4096   19.0  13.9     Q4_K   64 tokens, 2048 x 2048   9.7   8.5
+//   Q6_K   64         2048 x 4096   21.6  14.7     fp16  128         2048 x 4096  18.4  16.0
+//   448 tiles, Q8_0, 200 tokens, 2048 x 4096       19.4  25.0
+//   four groups for two superblocks, Q4_K, 64 tokens, 2048 x 512                   6.3   7.6
 constexpr int ROWS_T = 32;
 constexpr int64_t FILL = 200;  // workgroups
 
@@ -947,6 +975,7 @@ int launch_matmul(const MmArgs &a, hipStream_t st)
         if constexpr (QT == BREAD_QTYPE_Q6_K) return launch_tile<QT, 2, 1, 1, 2, 4, EXACT>(a, st);
         else return launch_tile<QT, 1, 1, 2, 2, 4, EXACT>(a, st);
     }
+    if (tiles(32, 32) <= 256 && a.cols > 4 * 256) return launch_tile<QT, 1, 1, 1, 1, 8, EXACT>(a, st);
     return launch_tile<QT, 1, 1, 1, 2, 4, EXACT>(a, st);
 }
 

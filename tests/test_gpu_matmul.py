@@ -143,6 +143,17 @@ def test_large(qtype):
     case(qtype, 1030, 2048, 768, seed=8, half=False)
 
 
+@pytest.mark.parametrize("half", [True, False], ids=["y16", "y32"])
+@pytest.mark.parametrize("qtype", [Q4, Q6, Q8, F16], ids=lambda q: NAMES[q])
+@pytest.mark.parametrize("T", [33, 70, 97])
+def test_long_rows_for_a_few_dozen_tokens(qtype, T, half):
+    """Superblocks over eight groups of waves: fewer than groups, some more, the last one cut short."""
+    short = {Q4: 0, Q6: 0, Q8: 32, F16: 8}[qtype]
+    for i, cols in enumerate((1280, 2048, 2304 + short, 4352 - short)):
+        for rows in (31, 96):
+            case(qtype, T, rows, cols, seed=T + 10 * i + rows, bias=i % 2 == 0, act=None, res=i % 2 == 1, half=half)
+
+
 @pytest.mark.parametrize("act", [a for a in ACTS if a])
 @pytest.mark.parametrize("T", [3, 150])
 def test_activations(act, T):
