@@ -24,7 +24,8 @@ constexpr int SV_WAVES = SV_THREADS / WAVE;
 // Logits a thread (PER): 32 once there is work for the whole GPU, 8 below that, where the time is one
 // workgroup's chain of loads and exponentials.  A workgroup's chunk of a row is SV_THREADS times as many.
 constexpr int SV_MANY = 32, SV_FEW = 8;
-constexpr int SV_CHAINS = 4;  // exponentials side by side
+constexpr int SV_JUDGES = 8;  // waves of k_sv_judge: rows judged side by side
+constexpr int SV_CHAINS = 2;  // exponentials side by side
 constexpr int SV_MAX_CHUNKS = 2048;  // of a row: 2^24 logits in chunks of 8192
 
 // One chunk of a row: the largest logit and the sum of exp((l - max) / T).
@@ -83,7 +84,7 @@ __device__ __forceinline__ float logit(LT v)
 // 2^y for y <= 0 by 2^n p(f), n the nearest whole number to y, f = y - n and p the polynomial of degree 9 that is 1
 // at 0 and has the least largest relative error on [-1/2, 1/2], 8e-14 (by Remez exchange).  The coefficients stay
 // in scalar registers: left to itself the compiler moves each to vector registers for every use, two moves for a
-// multiply-add (with the quieting of max's arguments 31 instructions a logit in k_sv_stats, 18 in its loop now).
+// multiply-add.
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct Exp2 {
@@ -110,30 +111,66 @@ struct Exp2 {
         const double n = __builtin_rint(y);
         return __builtin_amdgcn_ldexp(part(y - n), (int)n);
     }
-    // The sum of N of them, each y in [-1000, 1]: n comes out of the low bits of y + 1.5 2^52 and goes to the
-    // exponent.  N chains at a time, so that no instruction waits for the one before it.
-    template <int N>
-    __device__ __forceinline__ double sum_mid(const double (&y)[N]) const
+};
+
+// 2^(j / 32), rounded
+__constant__ double SV_TWO[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+
+// Many of them, each y in [-1000, 1]: 2^(k / 32) p(f) with k the nearest whole number to 32 y, f = y - k / 32 and p of
+// degree 4 (to 8e-14 on [-1/64, 1/64]).  2^(j / 32), j = k % 32, comes from 32 doubles in LDS, a bank each, that
+// hold j subtracted from the exponent's place, so that k is added there whole.  Bound by its 64-bit instructions,
+// ten a logit; with the polynomial of degree 9 and no table they are sixteen, and k_sv_stats' 101 us below 119.
+struct Exp2Table {
+    double c[4];
+    const double *two;
+    // lanes 0 to 31 of the wave fill its table
+    __device__ __forceinline__ explicit Exp2Table(double *mem)
+        : c{0x1.62e42fef6d0cdp-1, 0x1.ebfbdff87b60bp-3, 0x1.c6b167d804924p-5, 0x1.3b2a9efd4ad16p-7}, two(mem)
     {
-        double t[N], f[N], p[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) t[i] = y[i] + 0x1.8p52;
+        for (int k = 0; k < 3; k++) asm("" : "+s"(c[k]));
+        asm("" : "+v"(c[3]));
+        const int j = lane_id();
+        if (j < 32) {
+            u32x2 q = __builtin_bit_cast(u32x2, SV_TWO[j]);
+            q.y -= (uint32_t)j << 15;
+            mem[j] = __builtin_bit_cast(double, q);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // s[i] += 2^y[i], N chains so that no instruction waits for the one before it
+    template <int N>
+    __device__ __forceinline__ void add(const double (&y)[N], double (&s)[N]) const
+    {
+        double t[N], f[N], p[N], w[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) f[i] = y[i] - (t[i] - 0x1.8p52);
-#pragma unroll
-        for (int i = 0; i < N; i++) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p[i]) : "v"(c[8]), "v"(f[i]), "s"(c[7]));
-#pragma unroll
-        for (int k = 6; k >= 0; k--)
-#pragma unroll
-            for (int i = 0; i < N; i++) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p[i]) : "v"(p[i]), "v"(f[i]), "s"(c[k]));
-        double s = 0.0;
+        for (int i = 0; i < N; i++) t[i] = y[i] + 0x1.8p47;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            u32x2 q = __builtin_bit_cast(u32x2, fma(p[i], f[i], 1.0));
-            q.y += __builtin_bit_cast(u32x2, t[i]).x << 20;
-            s += __builtin_bit_cast(double, q);
+            const uint32_t k = __builtin_bit_cast(u32x2, t[i]).x;
+            u32x2 q = __builtin_bit_cast(u32x2, two[k & 31]);
+            q.y += k << 15;
+            w[i] = __builtin_bit_cast(double, q);
         }
-        return s;
+#pragma unroll
+        for (int i = 0; i < N; i++) f[i] = y[i] - (t[i] - 0x1.8p47);
+#pragma unroll
+        for (int i = 0; i < N; i++) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p[i]) : "v"(c[3]), "v"(f[i]), "s"(c[2]));
+#pragma unroll
+        for (int k = 1; k >= 0; k--)
+#pragma unroll
+            for (int i = 0; i < N; i++) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p[i]) : "v"(p[i]), "v"(f[i]), "s"(c[k]));
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = fma(w[i], fma(p[i], f[i], 1.0), s[i]);
     }
 };
 
@@ -248,41 +285,54 @@ __device__ __forceinline__ Eight<uint16_t> raise8(const Eight<uint16_t> &v, floa
 
 // A chunk a wave (chunk i % nchunk of row i / nchunk), 32 logits a lane at a time and the next ones on their way:
 // the largest so far, and in each lane its own sum relative to it; a larger one scales the sum down.
-// Bound by the 64-bit exponentials: 64 requests with 8 drafts over 248,320 tokens, 143M logits, 119 us on MI355X
-// (2.4 TB/s).  With a chunk a workgroup, 32 logits a thread, a third of the instructions went into its two
-// reductions: 149 us.
+// Bound by the 64-bit instructions: 64 requests with 8 drafts over 248,320 tokens, 143M fp16 logits, 101 us on MI355X
+// (2.8 TB/s; nine tenths of the issue slots are taken).  A chunk a workgroup, 32 logits a thread, spent a third of its
+// instructions on two reductions (149 us before the table); several chunks a wave, one round of waves for the GPU, end
+// unevenly (130 us).  Two chains leave room for four waves a SIMD, three for fp32 logits: 4 us less than four chains.
 template <typename LT, int PER>
-__global__ __launch_bounds__(SV_THREADS) void k_sv_stats(const SvArgs a)
+__global__ __launch_bounds__(SV_THREADS, sizeof(LT) == 2 ? 4 : 3) void k_sv_stats(const SvArgs a)
 {
     constexpr int STEPS = PER * SV_WAVES / 32, STEP = 32 * WAVE;
+    __shared__ double s_two[SV_WAVES][32];
     const Exp2 e2;
     const int lane = lane_id(), at = (int)blockIdx.x * SV_WAVES + wave_id();
     if (at >= a.R * a.nchunk) return;
-    const int row = at / a.nchunk, i0 = (at - row * a.nchunk) * (STEPS * STEP) + lane * 8;
+    const int row = at / a.nchunk, base = (at - row * a.nchunk) * (STEPS * STEP), i0 = base + lane * 8;
     const LT *z = static_cast<const LT *>(a.logits) + (size_t)row * a.stride;
     Eight<LT> v[4], nx[4];
-    auto load = [&](Eight<LT>(&d)[4], int i) {
+    auto load = [&](int step) __attribute__((always_inline)) {
+        const int i = i0 + step * STEP;
+        if (base + (step + 1) * STEP <= a.V) {  // (the whole wave)
 #pragma unroll
-        for (int j = 0; j < 4; j++) load8<LT>(z, i + j * (8 * WAVE), a.V, Eight<LT>::NONE, d[j]);
+            for (int j = 0; j < 4; j++) __builtin_memcpy(&nx[j], z + i + j * (8 * WAVE), sizeof(nx[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) load8<LT>(z, i + j * (8 * WAVE), a.V, Eight<LT>::NONE, nx[j]);
+        }
     };
-    load(nx, i0);
+    load(0);
+    const Exp2Table many(s_two[wave_id()]);
     const int b = request_of(a.off, a.B, row);
     const double c2 = scale2(a.temp, b);
     const bool gr = greedy(a.temp, b);
     float m = -__builtin_inff(), least = 0.f;
-    double s = 0.0, mc = 0.0;
+    double s[SV_CHAINS] = {}, mc = 0.0;
     bool plain = false;
     int arg = 0x7FFFFFFF;
     for (int step = 0; step < STEPS; step++) {
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = nx[j];
-        if (step + 1 < STEPS) load(nx, i0 + (step + 1) * STEP);
+        if (step + 1 < STEPS) load(step + 1);
         float ms = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < 4; j++) ms = max8(v[j], ms);
         ms = wave_max(ms);
         if (ms > m) {
-            s *= weight(e2, m, ms, c2);
+            if (m > -__builtin_inff()) {
+                const double down = weight(e2, m, ms, c2);
+#pragma unroll
+                for (int i = 0; i < SV_CHAINS; i++) s[i] *= down;
+            }
             m = ms;
             arg = 0x7FFFFFFF;
             // Logits whose 2^y would have y < -1000 or so, masked ones and NaN too, are raised to `least` and count
@@ -303,14 +353,14 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_stats(const SvArgs a)
                     double y[SV_CHAINS];
 #pragma unroll
                     for (int i = 0; i < SV_CHAINS; i++) y[i] = fma((double)r.value(k + i), c2, mc);
-                    s += e2.sum_mid(y);
+                    many.add(y, s);
                 }
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int k = 0; k < 8; k++) s += weight(e2, num(v[j].value(k)), m, c2);
+                for (int k = 0; k < 8; k++) s[k % SV_CHAINS] += weight(e2, num(v[j].value(k)), m, c2);
         }
         if (gr && arg == 0x7FFFFFFF) {  // (of the lane; the first step that has the largest has the lane's lowest)
 #pragma unroll
@@ -322,10 +372,13 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_stats(const SvArgs a)
                 }
         }
     }
-    s = sum_f64(s);
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < SV_CHAINS; i++) sum += s[i];
+    sum = sum_f64(sum);
     if (gr)
         for (int o = WAVE / 2; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o));
-    if (lane == 0) a.part[at] = SvPart{s, m, arg};
+    if (lane == 0) a.part[at] = SvPart{sum, m, arg};
 }
 
 // A row's statistics from its chunks, by one wave
@@ -337,14 +390,26 @@ struct SvRow {
 
 __device__ __forceinline__ SvRow row_stats(const SvArgs &a, const Exp2 &e2, int row, double c2)
 {
+    // the first chunks (all of 262144 logits in chunks of 2048) stay in registers: one trip to memory
+    constexpr int KEEP = 2;
     const SvPart *p = a.part + (size_t)row * a.nchunk;
+    const int lane = lane_id();
     SvRow r{0.0, -__builtin_inff(), 0x7FFFFFFF};
-    for (int c = lane_id(); c < a.nchunk; c += WAVE) r.max = fmaxf(r.max, p[c].max);
+    SvPart k[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        k[i] = i * WAVE + lane < a.nchunk ? p[i * WAVE + lane] : SvPart{0.0, -__builtin_inff(), 0x7FFFFFFF};
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) r.max = fmaxf(r.max, k[i].max);
+    for (int c = KEEP * WAVE + lane; c < a.nchunk; c += WAVE) r.max = fmaxf(r.max, p[c].max);
     r.max = wave_max(r.max);
-    for (int c = lane_id(); c < a.nchunk; c += WAVE) {
-        r.sum += p[c].sum * weight(e2, p[c].max, r.max, c2);
-        if (p[c].max == r.max) r.arg = min(r.arg, p[c].arg);
-    }
+    auto add = [&](const SvPart &q) __attribute__((always_inline)) {
+        r.sum += q.sum * weight(e2, q.max, r.max, c2);
+        if (q.max == r.max) r.arg = min(r.arg, q.arg);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) add(k[i]);
+    for (int c = KEEP * WAVE + lane; c < a.nchunk; c += WAVE) add(p[c]);
     r.sum = sum_f64(r.sum);
     for (int o = WAVE / 2; o > 0; o >>= 1) r.arg = min(r.arg, __shfl_xor(r.arg, o));
     return r;
@@ -420,7 +485,8 @@ __device__ __forceinline__ double whole_sum(const double *tot, int nchunk)
     return sum_f64(t);
 }
 
-// Sum over the workgroup, in every thread (s_d: one double a wave)
+// Sum over the workgroup of W waves, in every thread (s_d: one double a wave)
+template <int W>
 __device__ __forceinline__ double block_sum(double v, double *s_d)
 {
     v = sum_f64(v);
@@ -429,14 +495,16 @@ __device__ __forceinline__ double block_sum(double v, double *s_d)
     __syncthreads();
     v = s_d[0];
 #pragma unroll
-    for (int k = 1; k < SV_WAVES; k++) v += s_d[k];
+    for (int k = 1; k < W; k++) v += s_d[k];
     return v;
 }
 
+// What is left of a chunk, its parts in the first SV_THREADS threads of the workgroup
 template <typename LT, int PER>
 __device__ __forceinline__ double chunk_left(const Exp2 &e2, const SvLeft &left, const LT *z, int ch, int V, float max, double c2)
 {
     double s = 0.0;
+    if ((int)threadIdx.x >= SV_THREADS) return s;
 #pragma unroll
     for (int j = 0; j < PER / 8; j++) {
         double d[8];
@@ -457,17 +525,19 @@ __device__ __forceinline__ int draw(const Exp2 &e2, const SvLeft &left, const LT
     int hit;
     double before;
     find_chunk(tot, nchunk, border, hit, before);
-    // thread t owns PER consecutive tokens of the chunk
+    // thread t of the first SV_THREADS owns PER consecutive tokens of the chunk
     const int i0 = hit * (SV_THREADS * PER) + tid * PER;
-    double x[PER], own = 0.0;
+    double x[PER] = {}, own = 0.0;
+    if (tid < SV_THREADS) {
 #pragma unroll
-    for (int j = 0; j < PER / 8; j++) {
-        double d[8];
-        left.template eight<LT>(e2, z, i0 + 8 * j, V, max, c2, d);
+        for (int j = 0; j < PER / 8; j++) {
+            double d[8];
+            left.template eight<LT>(e2, z, i0 + 8 * j, V, max, c2, d);
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            x[8 * j + k] = d[k];
-            own += d[k];
+            for (int k = 0; k < 8; k++) {
+                x[8 * j + k] = d[k];
+                own += d[k];
+            }
         }
     }
     const double inc = wave_scan_incl_f64(own);
@@ -508,16 +578,17 @@ __device__ __forceinline__ void answer(const SvArgs &a, int b, int row, const LT
         a.logp[a.off[b + 1] - 1] = log_p(token >= 0 && token < a.V ? logit(z[token]) : -__builtin_inff(), rs, c2);
 }
 
-// Workgroup b: judges request b's drafts, and draws its token unless a draft
-// fell against a draft model's probabilities (k_sv_left then draws it).  Its
-// time is a chain of loads: offsets, then tokens and chunk statistics, then
-// the drafts' logits, then the chunk that holds the token.
+// Workgroup b: judges request b's drafts, a row a wave, and draws its token
+// unless a draft fell against a draft model's probabilities (k_sv_left then
+// draws it).  Its time is a chain of loads: offsets, then tokens and chunk
+// statistics, then the drafts' logits, then the chunk that holds the token:
+// 10.8 us on MI355X for one request with four drafts, 16 us for 64 requests.
 template <typename LT, int PER>
-__global__ __launch_bounds__(SV_THREADS) void k_sv_judge(const SvArgs a)
+__global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
 {
-    __shared__ int s_stop[SV_WAVES], s_pass[SV_WAVES];
-    __shared__ SvRow s_row[SV_WAVES];
-    __shared__ double s_d[SV_WAVES], s_tot[SV_MAX_CHUNKS];
+    __shared__ int s_stop[SV_JUDGES], s_pass[SV_JUDGES], s_token[SV_JUDGES];
+    __shared__ SvRow s_row[SV_JUDGES];
+    __shared__ double s_d[SV_JUDGES], s_tot[SV_MAX_CHUNKS];
     __shared__ int s_win;
     const Exp2 e2;
     const int b = (int)blockIdx.x, tid = (int)threadIdx.x, wv = wave_id(), lane = lane_id();
@@ -535,10 +606,11 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_judge(const SvArgs a)
         }
         return;
     }
-    // wave w judges the rows r0 + w, r0 + w + 4, ...; its first that stops
-    int stop = 0x7FFFFFFF, pass = 0;
+    const float u_last = a.u[r1 - 1];
+    // wave w judges the rows r0 + w, r0 + w + 8, ...; its first that stops
+    int stop = 0x7FFFFFFF, pass = 0, token = -1;
     SvRow mine{0.0, 0.f, 0};
-    for (int r = r0 + wv; r < r1; r += SV_WAVES) {
+    for (int r = r0 + wv; r < r1; r += SV_JUDGES) {
         if (stop != 0x7FFFFFFF && !a.logp) break;
         bool in = false;
         int d = -1;
@@ -564,25 +636,28 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_judge(const SvArgs a)
         if (stop == 0x7FFFFFFF && (!ok || ends)) {
             stop = r;
             pass = ok;
+            token = d;
             mine = s;
         }
     }
     if (lane == 0) {
         s_stop[wv] = stop;
         s_pass[wv] = pass;
+        s_token[wv] = token;
         s_row[wv] = mine;
     }
     __syncthreads();
     int at = 0;
 #pragma unroll
-    for (int k = 1; k < SV_WAVES; k++)
+    for (int k = 1; k < SV_JUDGES; k++)
         if (s_stop[k] < s_stop[at]) at = k;
     const int row = s_stop[at];
     const SvRow rs = s_row[at];
     const LT *z = z0 + (size_t)row * a.stride;
+    const int draft = s_token[at];  // (none in the last row)
     const bool ended = s_pass[at];  // the end token stood
     if (ended || gr || !(rs.sum > 0.0)) {
-        if (tid == 0) answer(a, b, row, z, rs, c2, ended ? a.tokens[row + 1] : rs.sum > 0.0 ? rs.arg : 0);
+        if (tid == 0) answer(a, b, row, z, rs, c2, ended ? draft : rs.sum > 0.0 ? rs.arg : 0);
         return;
     }
     const bool fell = row + 1 < r1;
@@ -591,17 +666,20 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_judge(const SvArgs a)
         return;
     }
     // the row's own weights, without the draft that was looked up
-    const SvLeft left{nullptr, fell ? a.tokens[row + 1] : -1, rs.sum};
-    for (int c = tid; c < a.nchunk; c += SV_THREADS) {
+    const SvLeft left{nullptr, fell ? draft : -1, rs.sum};
+    const bool one = left.one >= 0 && left.one < a.V;
+    // (summed again rather than subtracted: the draft may be nearly all there was; its chunk is on its way while the
+    // others' sums are)
+    const int its = one ? left.one / (SV_THREADS * PER) : -1;
+    const double part = one ? chunk_left<LT, PER>(e2, left, z, its, a.V, rs.max, c2) : 0.0;
+    for (int c = tid; c < a.nchunk; c += SV_JUDGES * WAVE) {
         const SvPart &p = a.part[(size_t)row * a.nchunk + c];
-        s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
+        if (c != its) s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
     }
     double total = rs.sum;
-    if (left.one >= 0 && left.one < a.V) {
-        // summed again rather than subtracted: the draft may be nearly all there was
-        const int c = left.one / (SV_THREADS * PER);
-        const double x = block_sum(chunk_left<LT, PER>(e2, left, z, c, a.V, rs.max, c2), s_d);
-        if (tid == 0) s_tot[c] = x;
+    if (one) {
+        const double x = block_sum<SV_JUDGES>(part, s_d);
+        if (tid == 0) s_tot[its] = x;
         __syncthreads();
         total = whole_sum(s_tot, a.nchunk);
     } else {
@@ -611,15 +689,15 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_judge(const SvArgs a)
     if (!(total > 0.0)) {  // the draft was all there was
         from.one = -1;
         __syncthreads();
-        for (int c = tid; c < a.nchunk; c += SV_THREADS) {
+        for (int c = tid; c < a.nchunk; c += SV_JUDGES * WAVE) {
             const SvPart &p = a.part[(size_t)row * a.nchunk + c];
             s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
         }
         __syncthreads();
         total = whole_sum(s_tot, a.nchunk);
     }
-    const int token = draw<LT, PER>(e2, from, z, s_tot, a.nchunk, (double)a.u[r1 - 1] * total, a.V, rs.max, c2, s_d, &s_win);
-    if (tid == 0) answer(a, b, row, z, rs, c2, token);
+    const int next = draw<LT, PER>(e2, from, z, s_tot, a.nchunk, (double)u_last * total, a.V, rs.max, c2, s_d, &s_win);
+    if (tid == 0) answer(a, b, row, z, rs, c2, next);
 }
 
 // Workgroup i: what is left of chunk i % nchunk at the row where a draft of
@@ -637,7 +715,7 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_left(const SvArgs a)
     const double c2 = scale2(a.temp, b);
     const LT *z = static_cast<const LT *>(a.logits) + (size_t)st.row * a.stride;
     SvLeft left{a.q + (size_t)(st.row - b) * a.qstride, -1, st.sum};
-    const double s = block_sum(chunk_left<LT, PER>(e2, left, z, ch, a.V, st.max, c2), s_d);
+    const double s = block_sum<SV_WAVES>(chunk_left<LT, PER>(e2, left, z, ch, a.V, st.max, c2), s_d);
     if (tid == 0) {
         __hip_atomic_store(&a.tot[(size_t)b * a.nchunk + ch], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // the store has reached where every workgroup sees it before the counter moves; the last workgroup of the
@@ -675,7 +753,7 @@ int launch(const SvArgs &a, hipStream_t st)
     const int all = a.R * a.nchunk;
     hipLaunchKernelGGL((k_sv_stats<LT, PER>), dim3((unsigned)((all + SV_WAVES - 1) / SV_WAVES)), dim3(SV_THREADS), 0, st, a);
     BREAD_HIP(hipGetLastError());
-    hipLaunchKernelGGL((k_sv_judge<LT, PER>), dim3((unsigned)a.B), dim3(SV_THREADS), 0, st, a);
+    hipLaunchKernelGGL((k_sv_judge<LT, PER>), dim3((unsigned)a.B), dim3(SV_JUDGES * WAVE), 0, st, a);
     BREAD_HIP(hipGetLastError());
     if (!a.q) return BREAD_OK;
     hipLaunchKernelGGL((k_sv_left<LT, PER>), dim3((unsigned)(a.B * a.nchunk)), dim3(SV_THREADS), 0, st, a);

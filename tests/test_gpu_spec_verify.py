@@ -161,6 +161,25 @@ def test_long_drafts():
     assert ra[0] == 100
 
 
+@pytest.mark.parametrize("half", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("probs", [True, False], ids=["model", "lookup"])
+def test_enough_rows_for_the_large_chunks(probs, half):
+    counts = [4, 0, 7, 1, 12] * 7
+    z, tokens, off, u, q = round_of(counts, 3 * CHUNK + 77, 61, half, probs)
+    assert len(tokens) * (3 * CHUNK + 77) > 2048 * 2048
+    temp = np.array([0.0, 0.7, 1.3, -1.0, 2.0, 0.01, 60.0] * 5)
+    z[3, :CHUNK] = -np.inf
+    z[9, 5:] = -np.inf
+    check(z, tokens, off, u, q)
+    check(z, tokens, off, u, q, temp=temp, eos=int(tokens[-1]))
+
+
+@pytest.mark.parametrize("V,counts", [(300_001, [0, 2]), (1_100_000, [4])])
+def test_more_chunks_than_two_a_lane(V, counts):
+    z, tokens, off, u, _ = round_of(counts, V, 62, probs=False)
+    check(z, tokens, off, u, temp=[0.9, 1.1][: len(counts)])
+
+
 @pytest.mark.parametrize("V", [50, 2 * CHUNK + 5])
 def test_greedy_is_spec_accept(V):
     """Temperature 0 gives bread_spec_accept's count and token on the rows' greedy predictions."""
