@@ -621,6 +621,13 @@ template <> struct Share<BREAD_QTYPE_F16> {
     static constexpr int BYTES = 512, PIECES = 8, STRIDE = 128;
 };
 
+// What a wave wrote to LDS comes before what it reads after this (the hardware keeps a wave's LDS accesses in order)
+__device__ __forceinline__ void wave_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <int QT, int WM, int WN, int MW, int NW, int KW, bool EXACT>
 __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a, int mt, int nt)
 {
@@ -630,7 +637,9 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
     constexpr bool DENSE = QT == BREAD_QTYPE_F16;
     constexpr int AHEAD = WM * WN > 4 ? 1 : 2;  // stages of activations on their way, and of operands made: registers
     constexpr bool UNIT = QT == BREAD_QTYPE_Q4_K || QT == BREAD_QTYPE_Q6_K;
-    __shared__ uint4 xs_all[KW][2][TM * 8];
+    // a group of one wave needs neither a second buffer nor barriers: its LDS accesses are in order
+    constexpr bool ALONE = MW * NW == 1;
+    __shared__ uint4 xs_all[KW][ALONE ? 1 : 2][TM * 8];
     // Q4_K: X_j / 32 of every token by superblock parity and half, four high parts, then four low ones
     __shared__ __attribute__((aligned(16))) uint16_t xm_all[KW][2][QT == BREAD_QTYPE_Q4_K ? TM : 1][2][8];
     __shared__ __attribute__((aligned(16))) uint8_t ws_all[KW][DENSE ? 2 : 1][TN * W::STRIDE];
@@ -675,7 +684,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
 #pragma unroll
         for (int i = 0; i < XL; i++) {
             const int k = i * THREADS + tid, t = k >> 3;
-            xs[at & 1][k] = v[i];
+            xs[ALONE ? 0 : at & 1][k] = v[i];
             if constexpr (QT == BREAD_QTYPE_Q4_K) {
                 // the sub-block's four units lie in four lanes; two of them store the parts
                 float x = sum_h8(v[i], 0.f);
@@ -753,9 +762,13 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
     fetch_w(0, 0);
     fetch_x(0, xr[0]);
     if constexpr (AHEAD > 1) fetch_x(1, xr[1]);
+    auto group_sync = [&]() __attribute__((always_inline)) {
+        if constexpr (ALONE) wave_order();
+        else q4m_bar();
+    };
     keep_w(0);
     keep_x(0, xr[0]);
-    q4m_bar();
+    group_sync();
     for (int round = 0; round < rounds; round++) {
         const bool any = KW == 1 || round * KW + kg < nsb;  // a superblock for this group
         W w[DENSE ? 1 : WN];
@@ -797,7 +810,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
                     for (int i = 0; i < WM; i++)
 #pragma unroll
                         for (int s = 0; s < 2; s++)
-                            xa[i][s] = xs[buf][(32 * (wm * WM + i) + c) * 8 + (step_unit<QT>(kh, 2 * b + s) ^ (c & 7))];
+                            xa[i][s] = xs[ALONE ? 0 : buf][(32 * (wm * WM + i) + c) * 8 + (step_unit<QT>(kh, 2 * b + s) ^ (c & 7))];
 #pragma unroll
                     for (int j = 0; j < WN; j++) {
                         const h8 w0 = w[j].step(st, 2 * b), w1 = w[j].step(st, 2 * b + 1);
@@ -818,7 +831,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
                 auto operands = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i < WM; i++)
-                        xa[s % AHEAD][i] = xs[buf][(32 * (wm * WM + i) + c) * 8 + (step_unit<QT>(kh, s) ^ (c & 7))];
+                        xa[s % AHEAD][i] = xs[ALONE ? 0 : buf][(32 * (wm * WM + i) + c) * 8 + (step_unit<QT>(kh, s) ^ (c & 7))];
 #pragma unroll
                     for (int j = 0; j < WN; j++) {
                         if constexpr (DENSE)
@@ -843,15 +856,16 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
                             acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][0], acc[i][j]);
                             if constexpr (EXACT) acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][1], acc[i][j]);
                         }
-                    __builtin_amdgcn_sched_barrier(0);
+                    if (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
                 }
             }
             }
             // every wave has taken its share of the weights before stage 2's barrier
             if (DENSE) keep_w(buf ^ 1);
             else if (st == 3) keep_w(0);
+            if (ALONE) wave_order();
             keep_x(4 * round + st + 1, xr[(st + 1) % AHEAD]);
-            q4m_bar();
+            group_sync();
         }
         if constexpr (QT == BREAD_QTYPE_Q4_K) if (any) {
 #pragma unroll
@@ -870,6 +884,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
     // read: lanes then hold four consecutive rows of a token, and the groups' sums are joined, each group taking
     // its part of the tokens
     static_assert(2 * WM >= NW, "4 KB a wave");
+    if (ALONE) __syncthreads();
     float *all_out = reinterpret_cast<float *>(&xs_all[0][0][0]), *out = all_out + 1024 * wave_id();
 #pragma unroll
     for (int j = 0; j < WN; j++)
@@ -952,10 +967,11 @@ int launch_rows(const MmArgs &a, hipStream_t st)
 // (256 x 256 of Q6_K and Q8_0 do not fit their registers and are not built.)
 // Where 32 x 32 tiles are no more than the CUs, a workgroup has one, with its superblocks over eight groups and not
 // four: a round fewer to wait for.  us with 32 x 64 and four groups, and with 32 x 32 and eight:
-//   Q8_0   67 tokens, 2048 x 4096   19.0  13.9     Q4_K   64 tokens, 2048 x 2048   9.7   8.5
-//   Q6_K   64         2048 x 4096   21.6  14.7     fp16  128         2048 x 4096  18.4  16.0
-//   448 tiles, Q8_0, 200 tokens, 2048 x 4096       19.4  25.0
+//   Q8_0   67 tokens, 2048 x 4096   19.0  12.3     Q4_K   64 tokens, 2048 x 2048   9.7   8.0
+//   Q6_K   64         2048 x 4096   21.6  13.1     fp16  128         2048 x 4096  18.4  13.8
+//   448 tiles, Q8_0, 200 tokens, 2048 x 4096       19.1  21.5
 //   four groups for two superblocks, Q4_K, 64 tokens, 2048 x 512                   6.3   7.6
+// (A group is then one wave and needs no barriers: 1.5 us of the 12.3.)
 constexpr int ROWS_T = 32;
 constexpr int64_t FILL = 200;  // workgroups
 
