@@ -919,7 +919,7 @@ template <int QT, int WM, int WN, int MW, int NW, int KW, bool EXACT>
 int launch_tile(const MmArgs &a, hipStream_t st)
 {
     const int64_t mt = (a.T + 32 * WM * MW - 1) / (32 * WM * MW), nt = ((int64_t)a.rows + 32 * WN * NW - 1) / (32 * WN * NW);
-    BREAD_REQUIRE(mt * nt < (1ll << 28), BREAD_ERR_SHAPE, "too many tiles");
+    BREAD_REQUIRE((mt * nt + 7) * (WAVE * MW * NW * KW) < (1ll << 32), BREAD_ERR_SHAPE, "too many tiles for a launch");
     bread_clear_stale_error();
     hipLaunchKernelGGL((k_mm_tile<QT, WM, WN, MW, NW, KW, EXACT>), dim3((unsigned)((mt * nt + 7) / 8 * 8)),
                        dim3(WAVE * MW * NW * KW), 0, st, a, (int)mt, (int)nt);
@@ -1004,6 +1004,8 @@ extern "C" int bread_matmul(const void *w, const uint16_t *x, void *y, int rows,
     const bread_matmul_opts_t &o = opts ? *opts : plain;
     BREAD_REQUIRE(rows >= 0 && cols > 0 && n_tokens >= 0, BREAD_ERR_ARG,
                   "rows and n_tokens must be >= 0 and cols > 0");
+    BREAD_REQUIRE(rows <= 1 << 30 && cols <= 1 << 30 && n_tokens <= 1 << 28, BREAD_ERR_SHAPE,
+                  "rows or cols above 2^30, or n_tokens above 2^28");
     BREAD_REQUIRE(qtype == BREAD_QTYPE_Q4_K || qtype == BREAD_QTYPE_Q6_K || qtype == BREAD_QTYPE_Q8_0 ||
                       qtype == BREAD_QTYPE_F16,
                   BREAD_ERR_QTYPE, "qtype must be 12 (Q4_K), 14 (Q6_K), 8 (Q8_0) or 1 (F16)");

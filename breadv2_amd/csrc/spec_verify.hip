@@ -807,7 +807,7 @@ extern "C" int bread_spec_verify(bread_moe_ctx_t *c, const bread_verify_t *v, br
         return (size_t)chunks(per) * ((size_t)a.R * sizeof(SvPart) + (size_t)a.B * sizeof(double)) +
                (size_t)a.B * sizeof(SvStop);
     };
-    BREAD_REQUIRE(bytes(SV_MANY) <= have && (int64_t)a.R * chunks(SV_MANY) < (1ll << 31), BREAD_ERR_CAPACITY,
+    BREAD_REQUIRE(bytes(SV_MANY) <= have && (int64_t)a.R * chunks(SV_MANY) < (1ll << 24), BREAD_ERR_CAPACITY,
                   "the context's scratch is too small for this vocabulary: create it for more tokens");
     const bool few = (int64_t)a.R * chunks(SV_FEW) <= 2048 && chunks(SV_FEW) <= SV_MAX_CHUNKS && bytes(SV_FEW) <= have;
     a.nchunk = chunks(few ? SV_FEW : SV_MANY);

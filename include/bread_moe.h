@@ -128,7 +128,8 @@ typedef struct {
  * 16-byte aligned (Q6_K and Q8_0: 4-byte), x 16-byte aligned with a stride
  * that is a multiple of 8.  y must not overlap x, w or bias, and residual is y
  * or does not overlap it.  Elements of y between one row's end and the next
- * row's start are left as they were.  n_tokens or rows 0: nothing is done.  No
+ * row's start are left as they were.  n_tokens or rows 0: nothing is done; rows
+ * and cols up to 2^30, n_tokens up to 2^28 (BREAD_ERR_SHAPE beyond).  No
  * workspace: calls on different streams may overlap. */
 int bread_matmul(const void *w, const uint16_t *x, void *y, int rows, int cols, int qtype, int n_tokens,
                  const bread_matmul_opts_t *opts, bread_stream_t stream);
@@ -297,7 +298,8 @@ typedef struct {
 
 /* Experts and weights of n_tokens tokens from their router logits by a rule.
  * d_logits fp32, n_experts (up to 1024) of a token every `stride` floats (0:
- * n_experts); d_idx int32 and d_w fp32 [n_tokens][top_k], top_k up to 32.  No
+ * n_experts); d_idx int32 and d_w fp32 [n_tokens][top_k], top_k up to 32,
+ * n_tokens up to 2^26.  A bias has no infinities of both signs in one group.  No
  * workspace: calls on different streams may overlap. */
 int bread_route_select(const bread_route_rule_t *rule, const float *d_logits, int64_t stride, int n_experts,
                        int top_k, int n_tokens, int32_t *d_idx, float *d_w, bread_stream_t stream);

@@ -226,6 +226,38 @@ def test_layer_by_rule(layer, T):
         assert_moe_close(h.cpu().numpy(), want, base=hidden)
 
 
+@pytest.mark.parametrize("dims,types", [
+    ((512, 256, 256, 12, 4), (12, 12, 12, 12, 12, 12)),
+    ((512, 256, 256, 12, 4), (12, 12, 14, 12, 12, 14)),
+    ((1024, 512, 256, 60, 6), (14, 12, 14, 14, 12, 12)),
+    ((256, 768, 512, 10, 3), (12, 12, 14, 12, 12, 14)),
+])
+def test_other_layers_by_rule(dims, types):
+    """Shapes and weight types of the per-token and the grouped paths, one token to a chunk."""
+    s = api.shape(*dims)
+    t = api.synth_layer_tensors(s, seed=5, layer=0, types=types)
+    torch.cuda.synchronize()
+    hl = host_layer(t)
+    E, K = s.n_experts, s.top_k
+    kw = dict(score="sigmoid", n_groups=2, top_groups=1, group_top=2, renorm=False, scale=0.5)
+    rng = np.random.default_rng(E)
+    bias = (0.2 * rng.standard_normal(E)).astype(np.float32)
+    rule = B.RouteRule(bias=dev(bias), **kw)
+    ctx = B.MoeContext(s, max_tokens=150)
+    for T in (1, 5, 40, 150):
+        x = rng.standard_normal((T, s.hidden)).astype(np.float32)
+        hidden = rng.standard_normal((T, s.hidden)).astype(np.float32)
+        logits = O.route_batch(hl, x, want_logits=True)[-1]
+        ri, rw = plain(np.asarray(logits), K, bias=bias, **kw)
+        h = dev(hidden)
+        idx, w, g = ctx.forward_by_rule(t.desc(), rule, dev(x), h, T, want_routing=True)
+        torch.cuda.synchronize()
+        assert ctx.check_device() == 0
+        assert np.array_equal(idx.cpu().numpy(), ri)
+        assert np.all(np.abs(w.cpu().numpy() - rw) <= (2.0 ** -24 + 1e-12) * rw)
+        assert_moe_close(h.cpu().numpy(), block(hl, x, hidden, ri, rw.astype(np.float32), g.cpu().numpy()), base=hidden)
+
+
 def test_route_layers_own_rule_is_the_default(layer):
     """RouteRule() chooses route_layer's experts in its order, with its weights to fp32 roundings."""
     s, t, hl = layer

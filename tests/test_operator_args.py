@@ -35,6 +35,13 @@ def test_matmul_refuses(kw, want):
     assert "bread_matmul" in lib.bread_last_error().decode()
 
 
+@pytest.mark.parametrize("kw", [dict(rows=(1 << 30) + 1), dict(cols=(1 << 30) + 256), dict(T=(1 << 28) + 1),
+                                dict(rows=1 << 30, cols=32, qtype=8, T=1 << 20)])
+def test_matmul_refuses_sizes_that_no_launch_has(kw):
+    assert matmul(**kw) == _lib.ERR_SHAPE
+    assert select(T=(1 << 26) + 1) == _lib.ERR_SHAPE
+
+
 def test_matmul_of_nothing():
     assert matmul(rows=0) == _lib.OK and matmul(T=0) == _lib.OK
     assert matmul(rows=0, w=None, x=None, y=None) == _lib.OK
