@@ -194,10 +194,11 @@ template <> struct Raw<BREAD_QTYPE_Q4_K> {
     }
 };
 
+// The eight scales of a lane's half and d in one load: even lanes of a row load the scales, odd ones the eight bytes
+// that end with d, and each takes the other's.
 template <> struct Raw<BREAD_QTYPE_Q6_K> {
     uint4 l0, l1, qh;
-    uint2 sc;
-    uint32_t d;
+    uint2 s;
     __device__ __forceinline__ void load(const uint8_t *row, int ch, int g, int)
     {
         const uint8_t *b = row + (size_t)ch * Q6K_BYTES;
@@ -205,8 +206,7 @@ template <> struct Raw<BREAD_QTYPE_Q6_K> {
         l0 = ldu16(b + 64 * h + o);
         l1 = ldu16(b + 64 * h + 32 + o);
         qh = ldu16(b + 128 + 32 * h + o);
-        sc = ldu8(b + 192 + 8 * h);
-        d = ldu2(b + 208);
+        s = ldu8(b + ((g & 1) ? 202 : 192 + 8 * h));
     }
 };
 
@@ -345,7 +345,9 @@ __device__ __forceinline__ void chunk_mma(const Raw<QT> &r, const uint4 (&xf)[NT
             for (int i = 0; i < 4; i++) out[tt][i] += d * acc[i] - dmin * accm[i];
         }
     } else if constexpr (QT == BREAD_QTYPE_Q6_K) {
-        const float d = h2f(r.d);
+        const lane_pair top = swap16(r.s.y);
+        const uint2 sc = make_uint2(swap16(r.s.x).a, top.a);
+        const float d = h2f(top.b >> 16);
         f32x4 acc[NTT];
 #pragma unroll
         for (int tt = 0; tt < NTT; tt++) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -354,7 +356,7 @@ __device__ __forceinline__ void chunk_mma(const Raw<QT> &r, const uint4 (&xf)[NT
         for (int i = 0; i < 8; i++) {
             const int qd = i >> 1, k = 2 * (i & 1);
             const uint4 &lw = (qd & 1) ? r.l1 : r.l0;
-            const uint32_t sb = (qd < 2 ? r.sc.x : r.sc.y) >> (16 * (qd & 1) + 8 * (g & 1));
+            const uint32_t sb = (qd < 2 ? sc.x : sc.y) >> (16 * (qd & 1) + 8 * (g & 1));
             const h2 S = both((float)(int8_t)(sb & 0xFFu));
             uint32_t v0 = (word(lw, k) >> (4 * (qd >> 1))) & 0x0F0F0F0Fu, v1 = (word(lw, k + 1) >> (4 * (qd >> 1))) & 0x0F0F0F0Fu;
             v0 |= ((word(r.qh, k) >> (2 * qd)) & 0x03030303u) << 4;
