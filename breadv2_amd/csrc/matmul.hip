@@ -421,7 +421,7 @@ constexpr int MR_MAXTT = 4;  // 16-token tiles a workgroup
 // HOLD: a row has no more chunks than waves, so that a wave keeps its activations in registers for all its row
 // tiles and loads the next tile's weights while it works on one.
 template <int QT, int NTT, bool EXACT, bool HOLD>
-__global__ __launch_bounds__(MR_THREADS) void k_mm_rows(const MmArgs a, int ny, int stride)
+__global__ __launch_bounds__(MR_THREADS, HOLD && QT != BREAD_QTYPE_F16 ? 4 : 2) void k_mm_rows(const MmArgs a, int ny, int stride)
 {
     __shared__ float part[2][MR_WAVES][NTT * 16][17];
     const int wv = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
