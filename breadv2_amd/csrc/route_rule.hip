@@ -21,8 +21,27 @@ constexpr int RR_THREADS = 256;
 // Order-preserving key of a choice: 0 taken or not allowed, 1 NaN, -inf and up above.
 __device__ __forceinline__ uint64_t choice_key(double c)
 {
+    // (by words, without branches)
     const uint64_t u = __builtin_bit_cast(uint64_t, c);
-    return c != c ? 1u : (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+    const uint32_t hi = (uint32_t)(u >> 32), all = (uint32_t)((int32_t)hi >> 31);
+    const bool nan = c != c;
+    const uint32_t kh = nan ? 0u : hi ^ (all | 0x80000000u), kl = nan ? 1u : (uint32_t)u ^ all;
+    return ((uint64_t)kh << 32) | kl;
+}
+
+// The larger of two, a number against NaN
+__device__ __forceinline__ double max_num(double a, double b)
+{
+    double d;
+    asm("v_max_f64 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+    return d;
+}
+
+__device__ __forceinline__ double min_num(double a, double b)
+{
+    double d;
+    asm("v_min_f64 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+    return d;
 }
 
 // Reductions over the L lanes (32 or 64, aligned) of a token; the result is in each of them.
@@ -142,17 +161,17 @@ __device__ __forceinline__ void wave_sync()
 // The two largest of two pairs of (largest, second)
 __device__ __forceinline__ void merge2(double &a1, double &a2, double b1, double b2)
 {
-    a2 = fmax(fmin(a1, b1), fmax(a2, b2));
-    a1 = fmax(a1, b1);
+    a2 = max_num(min_num(a1, b1), max_num(a2, b2));
+    a1 = max_num(a1, b1);
 }
 
 // L lanes a token, MAXV consecutive experts a lane.  A lane ranks its experts (all pairs compared once) and lays
 // their keys out in LDS in that order; of the lanes' best ones, the largest is then taken top_k times, by its high
 // word on DPP (its low word too where two are equal), and its lane goes on to its next.  Groups whose experts fill
 // a power of two of lanes are scored on DPP, others from LDS.
-// Bound by the instructions.  MI355X, 256 experts, sigmoid, four of eight groups, top 8: 16384 tokens 17.0 us (the
+// Bound by the instructions.  MI355X, 256 experts, sigmoid, four of eight groups, top 8: 16384 tokens 15.4 us (the
 // logits alone are 3.3 us at a copy's rate); a wave a token, with the library's exp and 64-bit maxima, took 31.
-// 100 tokens 5.8 us against 9.6; one token of softmax 4.1 us.  Two tokens a wave up to 256 experts because the
+// 100 tokens 5.6 us against 9.6; one token of softmax 4.0 us.  Two tokens a wave up to 256 experts because the
 // top_k rounds cost a wave the same for one.
 template <int MAXV, int L>
 __global__ __launch_bounds__(RR_THREADS) void k_route_rule(const float *__restrict__ logits, int64_t stride, int E,
@@ -204,7 +223,11 @@ __global__ __launch_bounds__(RR_THREADS) void k_route_rule(const float *__restri
     }
     uint64_t key[MAXV];
 #pragma unroll
-    for (int v = 0; v < MAXV; v++) key[v] = e0 + v < E ? choice_key(c[v]) : 0u;
+    for (int v = 0; v < MAXV; v++) key[v] = choice_key(c[v]);
+    if (e0 + MAXV > E) {
+#pragma unroll
+        for (int v = 0; v < MAXV; v++) key[v] = e0 + v < E ? key[v] : 0u;
+    }
     if (rule.top_groups < rule.n_groups) {
         // a group's score: NaN choices count as -inf
         const int G = rule.n_groups;
@@ -212,9 +235,9 @@ __global__ __launch_bounds__(RR_THREADS) void k_route_rule(const float *__restri
             double a1 = -__builtin_inf(), a2 = -__builtin_inf();
 #pragma unroll
             for (int v = 0; v < MAXV; v++) {
-                const double x = e0 + v < E && c[v] == c[v] ? c[v] : -__builtin_inf();
-                a2 = fmax(a2, fmin(a1, x));
-                a1 = fmax(a1, x);
+                const double x = max_num(c[v], -__builtin_inf());  // (a lane's experts are all there or none)
+                a2 = max_num(a2, min_num(a1, x));
+                a1 = max_num(a1, x);
             }
             if (rule.lanes >= 2) merge2(a1, a2, dpp_f64<0xB1>(a1), dpp_f64<0xB1>(a2));
             if (rule.lanes >= 4) merge2(a1, a2, dpp_f64<0x4E>(a1), dpp_f64<0x4E>(a2));
