@@ -235,31 +235,26 @@ template <> struct Raw<BREAD_QTYPE_Q8_0> {
         for (int i = 0; i < 16; i++) v[i] = word(p[i / 4], i & 3);
         v[16] = t;
     }
-    // q[i]: block i's eight values 8 g ..; d[i]: its scale
-    __device__ __forceinline__ void spread(uint2 (&q)[8], float (&d)[8]) const
+    // q[i]: the eight values 8 g .. of block 2 i + odd
+    __device__ __forceinline__ void spread(int odd, uint2 (&q)[4]) const
     {
         uint32_t lo[4], hi[4];
 #pragma unroll
-        for (int odd = 0; odd < 2; odd++) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                lo[j] = odd ? v[9 + 2 * j] : __builtin_amdgcn_alignbyte(v[2 * j + 1], v[2 * j], 2);
-                hi[j] = odd ? v[10 + 2 * j] : __builtin_amdgcn_alignbyte(v[2 * j + 2], v[2 * j + 1], 2);
-            }
-            transpose4(lo);
-            transpose4(hi);
-#pragma unroll
-            for (int i = 0; i < 4; i++) q[2 * i + odd] = make_uint2(lo[i], hi[i]);
+        for (int j = 0; j < 4; j++) {
+            lo[j] = odd ? v[9 + 2 * j] : __builtin_amdgcn_alignbyte(v[2 * j + 1], v[2 * j], 2);
+            hi[j] = odd ? v[10 + 2 * j] : __builtin_amdgcn_alignbyte(v[2 * j + 2], v[2 * j + 1], 2);
         }
-        const uint32_t dd = (v[0] & 0xFFFFu) | (v[8] & 0xFFFF0000u);
-#pragma unroll
-        for (int j = 0; j < 4; j++) lo[j] = dd;
         transpose4(lo);
+        transpose4(hi);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            d[2 * i] = h2f(lo[i] & 0xFFFFu);
-            d[2 * i + 1] = h2f(lo[i] >> 16);
-        }
+        for (int i = 0; i < 4; i++) q[i] = make_uint2(lo[i], hi[i]);
+    }
+    // d[i]: the scales of blocks 2 i and 2 i + 1 in its halves
+    __device__ __forceinline__ void scales(uint32_t (&d)[4]) const
+    {
+#pragma unroll
+        for (int j = 0; j < 4; j++) d[j] = (v[0] & 0xFFFFu) | (v[8] & 0xFFFF0000u);
+        transpose4(d);
     }
 };
 
@@ -310,6 +305,13 @@ __device__ __forceinline__ float sum_h8(const uint4 &v, float s)
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v.w), one, s, false);
 }
 
+// A dot product's result needs three wait states before a matrix instruction reads it; the compiler leaves none
+// between the two (it does before other vector instructions), and the last product is then missing.
+__device__ __forceinline__ void dot_to_mfma(float &x)
+{
+    asm volatile("s_nop 3" : "+v"(x));
+}
+
 // out[tt] += the chunk's products, tokens 16 tt + 4 g + i of weight row l % 16 in out[tt][i].
 // EXACT (Q6_K): the integers sc q above 2048 that fp16 would round, by at most 2^-12 of themselves and only
 // for the largest scales, are kept exact as sc (q with its low bit cleared) + sc (low bit), at twice the
@@ -325,24 +327,48 @@ __device__ __forceinline__ void chunk_mma(const Raw<QT> &r, const uint4 (&xf)[NT
         scale_min_k4(2 * g + 1, b.head.y, b.head.z, b.head.w, sc1, m1);
         const h2 S0 = both((float)sc0), N0 = both(-1024.f * (float)sc0);
         const h2 S1 = both((float)sc1), N1 = both(-1024.f * (float)sc1);
-        const h8 bq[8] = {q4m_b8(b.q0.x, b.q0.y, 0, S0, N0), q4m_b8(b.q0.z, b.q0.w, 0, S0, N0),
-                          q4m_b8(b.q1.x, b.q1.y, 0, S0, N0), q4m_b8(b.q1.z, b.q1.w, 0, S0, N0),
-                          q4m_b8(b.q0.x, b.q0.y, 1, S1, N1), q4m_b8(b.q0.z, b.q0.w, 1, S1, N1),
-                          q4m_b8(b.q1.x, b.q1.y, 1, S1, N1), q4m_b8(b.q1.z, b.q1.w, 1, S1, N1)};
+        auto operands = [&](int j, h8(&q)[4]) __attribute__((always_inline)) {
+            const h2 S = j ? S1 : S0, N = j ? N1 : N0;
+            q[0] = q4m_b8(b.q0.x, b.q0.y, j, S, N);
+            q[1] = q4m_b8(b.q0.z, b.q0.w, j, S, N);
+            q[2] = q4m_b8(b.q1.x, b.q1.y, j, S, N);
+            q[3] = q4m_b8(b.q1.z, b.q1.w, j, S, N);
+        };
+        auto products = [&](int tt, int j, const h8(&q)[4], f32x4 &acc, f32x4 &accm) __attribute__((always_inline)) {
+            float x = 0.f;
 #pragma unroll
-        for (int tt = 0; tt < NTT; tt++) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f}, accm = {0.f, 0.f, 0.f, 0.f};
-            float x0 = 0.f, x1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                acc = mfma(xf[tt][i], bq[i], acc);
-                if (i < 4) x0 = sum_h8(xf[tt][i], x0);
-                else x1 = sum_h8(xf[tt][i], x1);
+            for (int i = 0; i < 4; i++) {
+                acc = mfma(xf[tt][4 * j + i], q[i], acc);
+                x = sum_h8(xf[tt][4 * j + i], x);
             }
-            accm = __builtin_amdgcn_mfma_f32_16x16x4f32(x0, (float)m0, accm, 0, 0, 0);
-            accm = __builtin_amdgcn_mfma_f32_16x16x4f32(x1, (float)m1, accm, 0, 0, 0);
+            dot_to_mfma(x);
+            accm = __builtin_amdgcn_mfma_f32_16x16x4f32(x, (float)(j ? m1 : m0), accm, 0, 0, 0);
+        };
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (NTT == 1) {
+            // a sub-block's operands at a time: 16 registers less, for the second chunk that is held
+            f32x4 acc = zero, accm = zero;
 #pragma unroll
-            for (int i = 0; i < 4; i++) out[tt][i] += d * acc[i] - dmin * accm[i];
+            for (int j = 0; j < 2; j++) {
+                h8 q[4];
+                operands(j, q);
+                products(0, j, q, acc, accm);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[0][i] += d * acc[i] - dmin * accm[i];
+        } else {
+            h8 q0[4], q1[4];
+            operands(0, q0);
+            operands(1, q1);
+#pragma unroll
+            for (int tt = 0; tt < NTT; tt++) {
+                f32x4 acc = zero, accm = zero;
+                products(tt, 0, q0, acc, accm);
+                products(tt, 1, q1, acc, accm);
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[tt][i] += d * acc[i] - dmin * accm[i];
+            }
         }
     } else if constexpr (QT == BREAD_QTYPE_Q6_K) {
         const lane_pair top = swap16(r.s.y);
@@ -386,20 +412,25 @@ __device__ __forceinline__ void chunk_mma(const Raw<QT> &r, const uint4 (&xf)[NT
             for (int i = 0; i < 4; i++) out[tt][i] += d * acc[tt][i];
     } else if constexpr (QT == BREAD_QTYPE_Q8_0) {
         const h2 off = both(-1152.f);  // 1024 + (q + 128) - 1152
-        uint2 q[8];
-        float ds[8];
-        r.spread(q, ds);
+        uint32_t dd[4];
+        r.scales(dd);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t v0 = q[i].x ^ 0x80808080u, v1 = q[i].y ^ 0x80808080u;
-            const h8 w = join(magic_lo(v0) + off, magic_hi(v0) + off, magic_lo(v1) + off, magic_hi(v1) + off);
-            const float d = ds[i];
+        for (int odd = 0; odd < 2; odd++) {
+            uint2 q[4];
+            r.spread(odd, q);
 #pragma unroll
-            for (int tt = 0; tt < NTT; tt++) {
-                const f32x4 p = mfma(xf[tt][i], w, f32x4{0.f, 0.f, 0.f, 0.f});
+            for (int i = 0; i < 4; i++) {
+                const uint32_t v0 = q[i].x ^ 0x80808080u, v1 = q[i].y ^ 0x80808080u;
+                const h8 w = join(magic_lo(v0) + off, magic_hi(v0) + off, magic_lo(v1) + off, magic_hi(v1) + off);
+                const float d = h2f(odd ? dd[i] >> 16 : dd[i] & 0xFFFFu);
 #pragma unroll
-                for (int j = 0; j < 4; j++) out[tt][j] += d * p[j];
+                for (int tt = 0; tt < NTT; tt++) {
+                    const f32x4 p = mfma(xf[tt][2 * i + odd], w, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                    for (int j = 0; j < 4; j++) out[tt][j] += d * p[j];
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     } else {
 #pragma unroll
@@ -418,16 +449,16 @@ constexpr int MR_MAXTT = 4;  // 16-token tiles a workgroup
 
 // Workgroup b takes row tiles b / ny, b / ny + stride, ... against token tiles
 // [yb NTT, yb NTT + NTT), yb = b % ny.  Wave v owns the chunks v, v + 8, ... of every row.
-// HOLD: a row has no more chunks than waves, so that a wave keeps its activations in registers for all its row
-// tiles (reading them again for every tile took the vocabulary's logits from 111 to 167 us) and loads the next
-// tile's weights while it works on one.  Two workgroups a CU, so at most 128 registers (20 tokens, Q4_K: 105 us with
+// HOLD: a row has no more chunks than waves (1) or twice as many (2), and a wave keeps its activations in registers
+// for all its row tiles (reading them again for every tile took the vocabulary's logits from 111 to 167 us) and loads
+// the next weights while it works on one chunk.  Two workgroups a CU, so at most 128 registers (20 tokens, Q4_K: 105 us with
 // one, 89 with two); fp16 rows for 17 to 32 tokens would not fit them (117 us, spilled 285).
 // MI355X, 9 tokens: 248320 x 2048 Q6_K 111 us (3.8 TB/s), Q4_K 66 to 76 us (4 TB/s), 8192 x 2048 Q4_K 7.3 us.  Bound by
 // the loads: a lane's load from a row of its own costs the address unit a cycle, four loads and 64 lanes a chunk of
 // Q6_K.  Rows brought through LDS in the order they lie in took as long (110 us; 91 without the products), and so did
 // registers in turn for the weights on their way.
-template <int QT, int NTT, bool EXACT, bool HOLD>
-__global__ __launch_bounds__(MR_THREADS, HOLD && QT != BREAD_QTYPE_F16 ? 4 : 2) void k_mm_rows(const MmArgs a, int ny, int stride)
+template <int QT, int NTT, bool EXACT, int HOLD>
+__global__ __launch_bounds__(MR_THREADS, HOLD == 0 || QT == BREAD_QTYPE_F16 || (HOLD > 1 && QT == BREAD_QTYPE_Q8_0) ? 2 : 4) void k_mm_rows(const MmArgs a, int ny, int stride)
 {
     __shared__ float part[2][MR_WAVES][NTT * 16][17];
     const int wv = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
@@ -440,37 +471,52 @@ __global__ __launch_bounds__(MR_THREADS, HOLD && QT != BREAD_QTYPE_F16 ? 4 : 2) 
         const int t = t0 + 16 * tt + c;  // beyond the last token: the last one again, not stored
         xt[tt] = a.x + (size_t)(t < a.T ? t : a.T - 1) * a.xs;
     }
-    uint4 xf[NTT][8];
+    constexpr int SETS = HOLD > 1 ? HOLD : 1;
+    uint4 xf[SETS][NTT][8];
     Raw<QT> raw;
     int ti = (int)blockIdx.x / ny, buf = 0;
-    if (HOLD && wv < nw) {
-        const int r = 16 * ti + c;
-        raw.load(a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb, wv, g, a.cols);
+    auto row_of = [&](int tile) __attribute__((always_inline)) {  // (past the last row: the last one again, not stored)
+        const int r = 16 * tile + c;
+        return a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb;
+    };
+    const bool two = HOLD > 1 && wv + MR_WAVES < nch;  // a second chunk for this wave
+    if (HOLD > 0 && wv < nw) {
+        raw.load(row_of(ti), wv, g, a.cols);
 #pragma unroll
-        for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[tt], xt[tt], wv, g, a.cols);
+        for (int k = 0; k < SETS; k++)
+#pragma unroll
+            for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[k][tt], xt[tt], wv + MR_WAVES * k, g, a.cols);
     }
     for (; ti < ntile; ti += stride, buf ^= 1) {
         f32x4 out[NTT];
 #pragma unroll
         for (int tt = 0; tt < NTT; tt++) out[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (HOLD) {
+        if constexpr (HOLD > 1) {
+            Raw<QT> second;
+            // (the two chunks are kept apart: together they run out of registers)
+            if (two) second.load(row_of(ti), wv + MR_WAVES, g, a.cols);
+            __builtin_amdgcn_sched_barrier(0);
+            if (wv < nw) {
+                chunk_mma<QT, NTT, EXACT>(raw, xf[0], out, g);
+                __builtin_amdgcn_sched_barrier(0);
+                if (ti + stride < ntile) raw.load(row_of(ti + stride), wv, g, a.cols);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (two) chunk_mma<QT, NTT, EXACT>(second, xf[1], out, g);
+        } else if constexpr (HOLD == 1) {
             if (wv < nw) {
                 Raw<QT> next = raw;
-                if (ti + stride < ntile) {
-                    const int r = 16 * (ti + stride) + c;
-                    next.load(a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb, wv, g, a.cols);
-                }
-                chunk_mma<QT, NTT, EXACT>(raw, xf, out, g);
+                if (ti + stride < ntile) next.load(row_of(ti + stride), wv, g, a.cols);
+                chunk_mma<QT, NTT, EXACT>(raw, xf[0], out, g);
                 raw = next;
             }
         } else {
-            const int r = 16 * ti + c;
-            const uint8_t *row = a.w + (size_t)(r < a.rows ? r : a.rows - 1) * a.rb;
+            const uint8_t *row = row_of(ti);
             for (int ch = wv; ch < nch; ch += MR_WAVES) {
                 raw.load(row, ch, g, a.cols);
 #pragma unroll
-                for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[tt], xt[tt], ch, g, a.cols);
-                chunk_mma<QT, NTT, EXACT>(raw, xf, out, g);
+                for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[0][tt], xt[tt], ch, g, a.cols);
+                chunk_mma<QT, NTT, EXACT>(raw, xf[0], out, g);
             }
         }
         if (wv < nw) {
@@ -1007,14 +1053,18 @@ int launch_rows(const MmArgs &a, hipStream_t st)
     if (stride > ntile) stride = ntile;
     const dim3 grid((unsigned)(stride * ny)), block(MR_THREADS);
     bread_clear_stale_error();
-    const bool hold = a.cols <= 256 * MR_WAVES;
+    const int sets = (a.cols + 256 * MR_WAVES - 1) / (256 * MR_WAVES);  // chunks of a wave
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, ny, (int)stride); };
-    switch (ntt) {
-    case 1: hold ? go(k_mm_rows<QT, 1, EXACT, true>) : go(k_mm_rows<QT, 1, EXACT, false>); break;
-    case 2: hold ? go(k_mm_rows<QT, 2, EXACT, true>) : go(k_mm_rows<QT, 2, EXACT, false>); break;
-    case 3: go(k_mm_rows<QT, 3, EXACT, false>); break;
-    default: go(k_mm_rows<QT, 4, EXACT, false>); break;
-    }
+    // Two chunks are held for row tiles enough to make up for a workgroup less on a CU or registers at their limit.
+    // 9 tokens by 40000 x 4096, not held and held: Q4_K 50 and 37 us, Q6_K 56 and 42, Q8_0 62 and 54; by 8192 x 2304
+    // Q4_K, one tile a workgroup, 7.5 and 9.3.  Two fp16 chunks beside their activations would not fit the registers.
+    if (ntt == 1 && sets == 1) go(k_mm_rows<QT, 1, EXACT, 1>);
+    else if (ntt == 1 && sets == 2 && QT != BREAD_QTYPE_F16 && ntile >= 2 * stride) go(k_mm_rows<QT, 1, EXACT, QT == BREAD_QTYPE_F16 ? 0 : 2>);
+    else if (ntt == 1) go(k_mm_rows<QT, 1, EXACT, 0>);
+    else if (ntt == 2 && sets == 1) go(k_mm_rows<QT, 2, EXACT, 1>);
+    else if (ntt == 2) go(k_mm_rows<QT, 2, EXACT, 0>);
+    else if (ntt == 3) go(k_mm_rows<QT, 3, EXACT, 0>);
+    else go(k_mm_rows<QT, 4, EXACT, 0>);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
 }

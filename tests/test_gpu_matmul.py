@@ -154,6 +154,16 @@ def test_long_rows_for_a_few_dozen_tokens(qtype, T, half):
             case(qtype, T, rows, cols, seed=T + 10 * i + rows, bias=i % 2 == 0, act=None, res=i % 2 == 1, half=half)
 
 
+@pytest.mark.parametrize("half", [True, False], ids=["y16", "y32"])
+@pytest.mark.parametrize("qtype", [Q4, Q6, Q8, F16], ids=lambda q: NAMES[q])
+def test_many_rows_of_two_chunks_a_wave(qtype, half):
+    """Rows enough for every workgroup to take several tiles, with 9 to 16 superblocks, the last one cut short."""
+    short = {Q4: 0, Q6: 0, Q8: 32, F16: 8}[qtype]
+    case(qtype, 7, 16403, 2304, seed=21, bias=True, act=None, res=False, half=half)
+    case(qtype, 16, 24601, 2304 + short, seed=22, bias=False, act=None, res=True, half=half)
+    case(qtype, 1, 20000, 4096 - short, seed=23, half=half)
+
+
 @pytest.mark.parametrize("act", [a for a in ACTS if a])
 @pytest.mark.parametrize("T", [3, 150])
 def test_activations(act, T):
