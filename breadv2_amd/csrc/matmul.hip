@@ -453,7 +453,7 @@ constexpr int MR_MAXTT = 4;  // 16-token tiles a workgroup
 // for all its row tiles (reading them again for every tile took the vocabulary's logits from 111 to 167 us) and loads
 // the next weights while it works on one chunk.  Two workgroups a CU, so at most 128 registers (20 tokens, Q4_K: 105 us with
 // one, 89 with two); fp16 rows for 17 to 32 tokens would not fit them (117 us, spilled 285).
-// MI355X, 9 tokens: 248320 x 2048 Q6_K 111 us (3.8 TB/s), Q4_K 66 to 76 us (4 TB/s), 8192 x 2048 Q4_K 7.3 us.  Bound by
+// MI355X, 9 tokens: 248320 x 2048 Q6_K 101 to 111 us (4 TB/s), Q4_K 66 to 76 us (4 TB/s), 8192 x 2048 Q4_K 7.1 us.  Bound by
 // the loads: a lane's load from a row of its own costs the address unit a cycle, four loads and 64 lanes a chunk of
 // Q6_K.  Rows brought through LDS in the order they lie in took as long (110 us; 91 without the products), and so did
 // registers in turn for the weights on their way.
