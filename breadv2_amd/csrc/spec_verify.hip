@@ -21,10 +21,14 @@ namespace {
 
 constexpr int SV_THREADS = 256;
 constexpr int SV_WAVES = SV_THREADS / WAVE;
-// Logits a thread (PER): 32 once there is work for the whole GPU, 8 below that, where the time is one
-// workgroup's chain of loads and exponentials.  A workgroup's chunk of a row is SV_THREADS times as many.
+// Logits a thread (PER): 32 once there is plenty of work, 8 below that, where the time is a workgroup's chain of
+// loads and exponentials.  A workgroup's chunk of a row is SV_THREADS times as many.  us on MI355X with 32 and with 8,
+// drafts looked up, rows of 248,320 tokens: 4 rows 27.7 and 15.6, 64 rows 36.0 and 27.7, 128 rows 46.7 and 38.5, 400
+// rows 88 and 86, 1024 rows 185 and 200; of 32,000 tokens: 8 rows 27.4 and 15.4, 1024 rows 45.9 and 40.8.
+// 64 requests with 8 drafts and their probabilities, 248,320 tokens: 144 and 172.
 constexpr int SV_MANY = 32, SV_FEW = 8;
-constexpr int SV_JUDGES = 8;  // waves of k_sv_judge: rows judged side by side
+constexpr int SV_FEW_CHUNKS = 16384;  // in all, at 8 a thread
+constexpr int SV_ROWS = 8;  // waves of k_sv_accept: rows looked at side by side
 constexpr int SV_CHAINS = 2;  // exponentials side by side
 constexpr int SV_MAX_CHUNKS = 2048;  // of a row: 2^24 logits in chunks of 8192
 
@@ -578,17 +582,17 @@ __device__ __forceinline__ void answer(const SvArgs &a, int b, int row, const LT
         a.logp[a.off[b + 1] - 1] = log_p(token >= 0 && token < a.V ? logit(z[token]) : -__builtin_inff(), rs, c2);
 }
 
-// Workgroup b: judges request b's drafts, a row a wave, and draws its token
+// Workgroup b: tries request b's drafts, a row a wave, and draws its token
 // unless a draft fell against a draft model's probabilities (k_sv_left then
 // draws it).  Its time is a chain of loads: offsets, then tokens and chunk
 // statistics, then the drafts' logits, then the chunk that holds the token:
 // 10.8 us on MI355X for one request with four drafts, 16 us for 64 requests.
 template <typename LT, int PER>
-__global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
+__global__ __launch_bounds__(SV_ROWS *WAVE) void k_sv_accept(const SvArgs a)
 {
-    __shared__ int s_stop[SV_JUDGES], s_pass[SV_JUDGES], s_token[SV_JUDGES];
-    __shared__ SvRow s_row[SV_JUDGES];
-    __shared__ double s_d[SV_JUDGES], s_tot[SV_MAX_CHUNKS];
+    __shared__ int s_stop[SV_ROWS], s_pass[SV_ROWS], s_token[SV_ROWS];
+    __shared__ SvRow s_row[SV_ROWS];
+    __shared__ double s_d[SV_ROWS], s_tot[SV_MAX_CHUNKS];
     __shared__ int s_win;
     const Exp2 e2;
     const int b = (int)blockIdx.x, tid = (int)threadIdx.x, wv = wave_id(), lane = lane_id();
@@ -597,7 +601,7 @@ __global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
     const double c2 = scale2(a.temp, b);
     const LT *z0 = static_cast<const LT *>(a.logits);
     if (tid == 0) a.stop[b].row = -1;
-    // rows of no request's, or draft rows past the probabilities': nothing is judged
+    // rows of no request's, or draft rows past the probabilities': nothing is done
     if (r0 < b || r1 <= r0 || r1 > a.R || r1 - 2 - b >= a.R - a.B) {
         if (tid == 0) {
             __hip_atomic_fetch_or(a.err, BREAD_DEV_ERR_OFFSET, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -607,10 +611,10 @@ __global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
         return;
     }
     const float u_last = a.u[r1 - 1];
-    // wave w judges the rows r0 + w, r0 + w + 8, ...; its first that stops
+    // wave w takes the rows r0 + w, r0 + w + 8, ...; its first that stops
     int stop = 0x7FFFFFFF, pass = 0, token = -1;
     SvRow mine{0.0, 0.f, 0};
-    for (int r = r0 + wv; r < r1; r += SV_JUDGES) {
+    for (int r = r0 + wv; r < r1; r += SV_ROWS) {
         if (stop != 0x7FFFFFFF && !a.logp) break;
         bool in = false;
         int d = -1;
@@ -649,7 +653,7 @@ __global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
     __syncthreads();
     int at = 0;
 #pragma unroll
-    for (int k = 1; k < SV_JUDGES; k++)
+    for (int k = 1; k < SV_ROWS; k++)
         if (s_stop[k] < s_stop[at]) at = k;
     const int row = s_stop[at];
     const SvRow rs = s_row[at];
@@ -672,13 +676,13 @@ __global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
     // others' sums are)
     const int its = one ? left.one / (SV_THREADS * PER) : -1;
     const double part = one ? chunk_left<LT, PER>(e2, left, z, its, a.V, rs.max, c2) : 0.0;
-    for (int c = tid; c < a.nchunk; c += SV_JUDGES * WAVE) {
+    for (int c = tid; c < a.nchunk; c += SV_ROWS * WAVE) {
         const SvPart &p = a.part[(size_t)row * a.nchunk + c];
         if (c != its) s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
     }
     double total = rs.sum;
     if (one) {
-        const double x = block_sum<SV_JUDGES>(part, s_d);
+        const double x = block_sum<SV_ROWS>(part, s_d);
         if (tid == 0) s_tot[its] = x;
         __syncthreads();
         total = whole_sum(s_tot, a.nchunk);
@@ -689,7 +693,7 @@ __global__ __launch_bounds__(SV_JUDGES *WAVE) void k_sv_judge(const SvArgs a)
     if (!(total > 0.0)) {  // the draft was all there was
         from.one = -1;
         __syncthreads();
-        for (int c = tid; c < a.nchunk; c += SV_JUDGES * WAVE) {
+        for (int c = tid; c < a.nchunk; c += SV_ROWS * WAVE) {
             const SvPart &p = a.part[(size_t)row * a.nchunk + c];
             s_tot[c] = p.sum * weight(e2, p.max, rs.max, c2);
         }
@@ -753,7 +757,7 @@ int launch(const SvArgs &a, hipStream_t st)
     const int all = a.R * a.nchunk;
     hipLaunchKernelGGL((k_sv_stats<LT, PER>), dim3((unsigned)((all + SV_WAVES - 1) / SV_WAVES)), dim3(SV_THREADS), 0, st, a);
     BREAD_HIP(hipGetLastError());
-    hipLaunchKernelGGL((k_sv_judge<LT, PER>), dim3((unsigned)a.B), dim3(SV_JUDGES * WAVE), 0, st, a);
+    hipLaunchKernelGGL((k_sv_accept<LT, PER>), dim3((unsigned)a.B), dim3(SV_ROWS * WAVE), 0, st, a);
     BREAD_HIP(hipGetLastError());
     if (!a.q) return BREAD_OK;
     hipLaunchKernelGGL((k_sv_left<LT, PER>), dim3((unsigned)(a.B * a.nchunk)), dim3(SV_THREADS), 0, st, a);
@@ -809,7 +813,7 @@ extern "C" int bread_spec_verify(bread_moe_ctx_t *c, const bread_verify_t *v, br
     };
     BREAD_REQUIRE(bytes(SV_MANY) <= have && (int64_t)a.R * chunks(SV_MANY) < (1ll << 24), BREAD_ERR_CAPACITY,
                   "the context's scratch is too small for this vocabulary: create it for more tokens");
-    const bool few = (int64_t)a.R * chunks(SV_FEW) <= 2048 && chunks(SV_FEW) <= SV_MAX_CHUNKS && bytes(SV_FEW) <= have;
+    const bool few = (int64_t)a.R * chunks(SV_FEW) <= SV_FEW_CHUNKS && chunks(SV_FEW) <= SV_MAX_CHUNKS && bytes(SV_FEW) <= have;
     a.nchunk = chunks(few ? SV_FEW : SV_MANY);
     a.part = reinterpret_cast<SvPart *>(c->h);
     a.stop = reinterpret_cast<SvStop *>(a.part + (size_t)a.R * a.nchunk);

@@ -444,7 +444,7 @@ int bread_spec_accept(const int32_t *pred, const int32_t *draft, int n_draft, in
  * the target's logits after it.  With p_r = softmax(logits[r] /
  * temperature[b]) and q_r the probabilities that the draft tokens[r + 1] was
  * drawn from, draft tokens[r + 1] stands when u[r] * q_r(draft) < p_r(draft).
- * Drafts are judged in order; the request stops at row r
+ * Drafts are taken in order; the request stops at row r
  *   - where a draft falls: next is drawn from max(p_r - q_r, 0) (from p_r if
  *     that is zero everywhere);
  *   - where the draft that stands is eos: next is eos, which n_accept does not

@@ -174,6 +174,18 @@ def test_enough_rows_for_the_large_chunks(probs, half):
     check(z, tokens, off, u, q, temp=temp, eos=int(tokens[-1]))
 
 
+@pytest.mark.parametrize("probs,half", [(True, False), (False, True)], ids=["model-f32", "lookup-f16"])
+def test_many_rows_of_several_large_chunks(probs, half):
+    counts = [4, 0, 7, 1, 12] * 46
+    V = 3 * CHUNK + 77
+    z, tokens, off, u, q = round_of(counts, V, 63, half, probs)
+    assert len(tokens) * -(-V // 2048) > 16384
+    temp = np.array([0.0, 0.7, 1.3, -1.0, 2.0, 0.01, 60.0] * 33)[: len(counts)]
+    z[3, :CHUNK] = -np.inf
+    z[9, 5:] = -np.inf
+    check(z, tokens, off, u, q, temp=temp, eos=int(tokens[-1]))
+
+
 @pytest.mark.parametrize("V,counts", [(300_001, [0, 2]), (1_100_000, [4])])
 def test_more_chunks_than_two_a_lane(V, counts):
     z, tokens, off, u, _ = round_of(counts, V, 62, probs=False)
