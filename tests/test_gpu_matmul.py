@@ -164,6 +164,21 @@ def test_many_rows_of_two_chunks_a_wave(qtype, half):
     case(qtype, 1, 20000, 4096 - short, seed=23, half=half)
 
 
+@pytest.mark.parametrize("qtype", [Q4, Q6, Q8, F16], ids=lambda q: NAMES[q])
+def test_tokens_far_apart(qtype):
+    """Tokens 2^22 elements from each other: beyond the tiles' 32-bit offsets."""
+    rows, cols = 50, 512
+    wide = torch.zeros(70, 1 << 22, dtype=torch.float16, device=DEV)
+    w = weights(qtype, rows, cols, 8)
+    for T in (33, 64, 70):
+        x = np.random.default_rng(T).standard_normal((T, cols)).astype(np.float16)
+        wide[:T, 64:64 + cols] = dev(x)
+        y = torch.empty(T, rows, device=DEV)
+        B.bread_matmul(dev(w), wide[:T, 64:64 + cols], y, rows, cols, qtype)
+        want, tol = expected(w, qtype, rows, cols, x, None, None, None, False)
+        assert np.all(np.abs(y.cpu().numpy() - want) <= tol), (NAMES[qtype], T)
+
+
 @pytest.mark.parametrize("act", [a for a in ACTS if a])
 @pytest.mark.parametrize("T", [3, 150])
 def test_activations(act, T):
