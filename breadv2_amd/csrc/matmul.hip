@@ -313,10 +313,12 @@ __device__ __forceinline__ void dot_to_mfma(float &x)
 }
 
 // out[tt] += the chunk's products, tokens 16 tt + 4 g + i of weight row l % 16 in out[tt][i].
-// EXACT (Q6_K): the integers sc q above 2048 that fp16 would round, by at most 2^-12 of themselves and only
-// for the largest scales, are kept exact as sc (q with its low bit cleared) + sc (low bit), at twice the
-// MFMAs: for fp32 results.  An fp16 result has itself half a step of 2^-11.
-template <int QT, int NTT, bool EXACT>
+// Q6_K: the integers sc q, up to 4096, do not fit fp16's 11 bits, and the scales of trained weights reach -128 in
+// every superblock; they are multiplied as sc (q with its low bit cleared) + sc (low bit), both exact, at twice
+// the MFMAs.  us on MI355X with the integers rounded to 11 bits and with both parts, tokens by weights, fp16 results:
+// 9 by 248320 x 2048 102 and 113, 64 by 2048 x 4096 12.2 and 13.1, 509 by 2048 x 4096 25.7 and 30.2, 2048 by
+// 8192 x 2048 104 and 139.
+template <int QT, int NTT>
 __device__ __forceinline__ void chunk_mma(const Raw<QT> &r, const uint4 (&xf)[NTT][8], f32x4 (&out)[NTT], int g)
 {
     if constexpr (QT == BREAD_QTYPE_Q4_K) {
@@ -387,23 +389,16 @@ __device__ __forceinline__ void chunk_mma(const Raw<QT> &r, const uint4 (&xf)[NT
             uint32_t v0 = (word(lw, k) >> (4 * (qd >> 1))) & 0x0F0F0F0Fu, v1 = (word(lw, k + 1) >> (4 * (qd >> 1))) & 0x0F0F0F0Fu;
             v0 |= ((word(r.qh, k) >> (2 * qd)) & 0x03030303u) << 4;
             v1 |= ((word(r.qh, k + 1) >> (2 * qd)) & 0x03030303u) << 4;
-            if constexpr (EXACT) {
-                const uint32_t a0 = v0 & 0x3E3E3E3Eu, a1 = v1 & 0x3E3E3E3Eu;
-                const uint32_t b0 = v0 & 0x01010101u, b1 = v1 & 0x01010101u;
-                const h8 hi = join((magic_lo(a0) + off) * S, (magic_hi(a0) + off) * S, (magic_lo(a1) + off) * S,
-                                   (magic_hi(a1) + off) * S);
-                const h8 lo = join((magic_lo(b0) + one) * S, (magic_hi(b0) + one) * S, (magic_lo(b1) + one) * S,
-                                   (magic_hi(b1) + one) * S);
+            const uint32_t a0 = v0 & 0x3E3E3E3Eu, a1 = v1 & 0x3E3E3E3Eu;
+            const uint32_t b0 = v0 & 0x01010101u, b1 = v1 & 0x01010101u;
+            const h8 hi = join((magic_lo(a0) + off) * S, (magic_hi(a0) + off) * S, (magic_lo(a1) + off) * S,
+                               (magic_hi(a1) + off) * S);
+            const h8 lo = join((magic_lo(b0) + one) * S, (magic_hi(b0) + one) * S, (magic_lo(b1) + one) * S,
+                               (magic_hi(b1) + one) * S);
 #pragma unroll
-                for (int tt = 0; tt < NTT; tt++) {
-                    acc[tt] = mfma(xf[tt][i], hi, acc[tt]);
-                    acc[tt] = mfma(xf[tt][i], lo, acc[tt]);
-                }
-            } else {
-                const h8 w = join((magic_lo(v0) + off) * S, (magic_hi(v0) + off) * S, (magic_lo(v1) + off) * S,
-                                  (magic_hi(v1) + off) * S);
-#pragma unroll
-                for (int tt = 0; tt < NTT; tt++) acc[tt] = mfma(xf[tt][i], w, acc[tt]);
+            for (int tt = 0; tt < NTT; tt++) {
+                acc[tt] = mfma(xf[tt][i], hi, acc[tt]);
+                acc[tt] = mfma(xf[tt][i], lo, acc[tt]);
             }
         }
 #pragma unroll
@@ -453,11 +448,11 @@ constexpr int MR_MAXTT = 4;  // 16-token tiles a workgroup
 // for all its row tiles (reading them again for every tile took the vocabulary's logits from 111 to 167 us) and loads
 // the next weights while it works on one chunk.  Two workgroups a CU, so at most 128 registers (20 tokens, Q4_K: 105 us with
 // one, 89 with two); fp16 rows for 17 to 32 tokens would not fit them (117 us, spilled 285).
-// MI355X, 9 tokens: 248320 x 2048 Q6_K 101 to 111 us (4 TB/s), Q4_K 66 to 76 us (4 TB/s), 8192 x 2048 Q4_K 7.1 us.  Bound by
+// MI355X, 9 tokens: 248320 x 2048 Q6_K 112 to 115 us (3.7 TB/s), Q4_K 66 to 76 us (4 TB/s), 8192 x 2048 Q4_K 7.1 us.  Bound by
 // the loads: a lane's load from a row of its own costs the address unit a cycle, four loads and 64 lanes a chunk of
 // Q6_K.  Rows brought through LDS in the order they lie in took as long (110 us; 91 without the products), and so did
 // registers in turn for the weights on their way.
-template <int QT, int NTT, bool EXACT, int HOLD>
+template <int QT, int NTT, int HOLD>
 __global__ __launch_bounds__(MR_THREADS, HOLD == 0 || QT == BREAD_QTYPE_F16 || (HOLD > 1 && QT == BREAD_QTYPE_Q8_0) ? 2 : 4) void k_mm_rows(const MmArgs a, int ny, int stride)
 {
     __shared__ float part[2][MR_WAVES][NTT * 16][17];
@@ -497,17 +492,17 @@ __global__ __launch_bounds__(MR_THREADS, HOLD == 0 || QT == BREAD_QTYPE_F16 || (
             if (two) second.load(row_of(ti), wv + MR_WAVES, g, a.cols);
             __builtin_amdgcn_sched_barrier(0);
             if (wv < nw) {
-                chunk_mma<QT, NTT, EXACT>(raw, xf[0], out, g);
+                chunk_mma<QT, NTT>(raw, xf[0], out, g);
                 __builtin_amdgcn_sched_barrier(0);
                 if (ti + stride < ntile) raw.load(row_of(ti + stride), wv, g, a.cols);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (two) chunk_mma<QT, NTT, EXACT>(second, xf[1], out, g);
+            if (two) chunk_mma<QT, NTT>(second, xf[1], out, g);
         } else if constexpr (HOLD == 1) {
             if (wv < nw) {
                 Raw<QT> next = raw;
                 if (ti + stride < ntile) next.load(row_of(ti + stride), wv, g, a.cols);
-                chunk_mma<QT, NTT, EXACT>(raw, xf[0], out, g);
+                chunk_mma<QT, NTT>(raw, xf[0], out, g);
                 raw = next;
             }
         } else {
@@ -516,7 +511,7 @@ __global__ __launch_bounds__(MR_THREADS, HOLD == 0 || QT == BREAD_QTYPE_F16 || (
                 raw.load(row, ch, g, a.cols);
 #pragma unroll
                 for (int tt = 0; tt < NTT; tt++) load_x<QT>(xf[0][tt], xt[tt], ch, g, a.cols);
-                chunk_mma<QT, NTT, EXACT>(raw, xf[0], out, g);
+                chunk_mma<QT, NTT>(raw, xf[0], out, g);
             }
         }
         if (wv < nw) {
@@ -678,12 +673,6 @@ template <> struct Share<BREAD_QTYPE_Q6_K> {
         return join((magic_lo(v0) + off) * f, (magic_hi(v0) + off) * f, (magic_lo(v1) + off) * f,
                     (magic_hi(v1) + off) * f);
     }
-    __device__ __forceinline__ h8 step(int st, int s) const
-    {
-        uint32_t v0, v1;
-        codes(st, s, v0, v1);
-        return scaled(v0, v1, both(-1056.f), s);
-    }
     // the codes without their low bits, and the low bits alone
     __device__ __forceinline__ void step2(int st, int s, h8 &hi, h8 &lo) const
     {
@@ -744,7 +733,7 @@ __device__ __forceinline__ void wave_order()
     __builtin_amdgcn_wave_barrier();
 }
 
-template <int QT, int WM, int WN, int MW, int NW, int KW, bool EXACT>
+template <int QT, int WM, int WN, int MW, int NW, int KW>
 __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a, int mt, int nt)
 {
     using W = Share<QT>;
@@ -753,6 +742,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
     constexpr bool DENSE = QT == BREAD_QTYPE_F16;
     constexpr int AHEAD = WM * WN > 4 ? 1 : 2;  // stages of activations on their way, and of operands made: registers
     constexpr bool UNIT = QT == BREAD_QTYPE_Q4_K || QT == BREAD_QTYPE_Q6_K;
+    constexpr bool TWO = QT == BREAD_QTYPE_Q6_K;  // a weight is two operands
     // a group of one wave needs neither a second buffer nor barriers: its LDS accesses are in order
     constexpr bool ALONE = MW * NW == 1;
     __shared__ uint4 xs_all[KW][ALONE ? 1 : 2][TM * 8];
@@ -943,7 +933,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
                 // a step's operands are read and unpacked beside the products of the step before it; the scheduler
                 // is kept to that, else it makes the whole stage's operands first and runs out of registers
                 uint4 xa[AHEAD][WM];
-                h8 wf[AHEAD][WN][EXACT ? 2 : 1];
+                h8 wf[AHEAD][WN][TWO ? 2 : 1];
                 auto operands = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i < WM; i++)
@@ -954,7 +944,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
                             wf[s % AHEAD][j][0] = __builtin_bit_cast(
                                 h8, reinterpret_cast<const uint4 *>(
                                         ws[buf])[(32 * (wn * WN + j) + c) * 8 + (step_unit<QT>(kh, s) ^ (c & 7))]);
-                        else if constexpr (EXACT)
+                        else if constexpr (TWO)
                             w[j].step2(st, s, wf[s % AHEAD][j][0], wf[s % AHEAD][j][1]);
                         else
                             wf[s % AHEAD][j][0] = w[j].step(st, s);
@@ -970,7 +960,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
 #pragma unroll
                         for (int i = 0; i < WM; i++) {
                             acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][0], acc[i][j]);
-                            if constexpr (EXACT) acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][1], acc[i][j]);
+                            if constexpr (TWO) acc[i][j] = mfma32(xa[s % AHEAD][i], wf[s % AHEAD][j][1], acc[i][j]);
                         }
                     if (AHEAD > 1) __builtin_amdgcn_sched_barrier(0);
                 }
@@ -1031,19 +1021,19 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
         }
 }
 
-template <int QT, int WM, int WN, int MW, int NW, int KW, bool EXACT>
+template <int QT, int WM, int WN, int MW, int NW, int KW>
 int launch_tile(const MmArgs &a, hipStream_t st)
 {
     const int64_t mt = (a.T + 32 * WM * MW - 1) / (32 * WM * MW), nt = ((int64_t)a.rows + 32 * WN * NW - 1) / (32 * WN * NW);
     BREAD_REQUIRE((mt * nt + 7) * (WAVE * MW * NW * KW) < (1ll << 32), BREAD_ERR_SHAPE, "too many tiles for a launch");
     bread_clear_stale_error();
-    hipLaunchKernelGGL((k_mm_tile<QT, WM, WN, MW, NW, KW, EXACT>), dim3((unsigned)((mt * nt + 7) / 8 * 8)),
+    hipLaunchKernelGGL((k_mm_tile<QT, WM, WN, MW, NW, KW>), dim3((unsigned)((mt * nt + 7) / 8 * 8)),
                        dim3(WAVE * MW * NW * KW), 0, st, a, (int)mt, (int)nt);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
 }
 
-template <int QT, bool EXACT>
+template <int QT>
 int launch_rows(const MmArgs &a, hipStream_t st)
 {
     const int tt = (a.T + 15) / 16, ny = (tt + MR_MAXTT - 1) / MR_MAXTT, ntt = (tt + ny - 1) / ny;
@@ -1058,13 +1048,13 @@ int launch_rows(const MmArgs &a, hipStream_t st)
     // Two chunks are held for row tiles enough to make up for a workgroup less on a CU or registers at their limit.
     // 9 tokens by 40000 x 4096, not held and held: Q4_K 50 and 37 us, Q6_K 56 and 42, Q8_0 62 and 54; by 8192 x 2304
     // Q4_K, one tile a workgroup, 7.5 and 9.3.  Two fp16 chunks beside their activations would not fit the registers.
-    if (ntt == 1 && sets == 1) go(k_mm_rows<QT, 1, EXACT, 1>);
-    else if (ntt == 1 && sets == 2 && QT != BREAD_QTYPE_F16 && ntile >= 2 * stride) go(k_mm_rows<QT, 1, EXACT, QT == BREAD_QTYPE_F16 ? 0 : 2>);
-    else if (ntt == 1) go(k_mm_rows<QT, 1, EXACT, 0>);
-    else if (ntt == 2 && sets == 1) go(k_mm_rows<QT, 2, EXACT, 1>);
-    else if (ntt == 2) go(k_mm_rows<QT, 2, EXACT, 0>);
-    else if (ntt == 3) go(k_mm_rows<QT, 3, EXACT, 0>);
-    else go(k_mm_rows<QT, 4, EXACT, 0>);
+    if (ntt == 1 && sets == 1) go(k_mm_rows<QT, 1, 1>);
+    else if (ntt == 1 && sets == 2 && QT != BREAD_QTYPE_F16 && ntile >= 2 * stride) go(k_mm_rows<QT, 1, QT == BREAD_QTYPE_F16 ? 0 : 2>);
+    else if (ntt == 1) go(k_mm_rows<QT, 1, 0>);
+    else if (ntt == 2 && sets == 1) go(k_mm_rows<QT, 2, 1>);
+    else if (ntt == 2) go(k_mm_rows<QT, 2, 0>);
+    else if (ntt == 3) go(k_mm_rows<QT, 3, 0>);
+    else go(k_mm_rows<QT, 4, 0>);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
 }
@@ -1095,24 +1085,24 @@ int launch_rows(const MmArgs &a, hipStream_t st)
 constexpr int ROWS_T = 32;
 constexpr int64_t FILL = 200;  // workgroups
 
-template <int QT, bool EXACT>
+template <int QT>
 int launch_matmul(const MmArgs &a, hipStream_t st)
 {
     auto tiles = [&](int64_t m, int64_t n) { return (a.T + m - 1) / m * ((a.rows + n - 1) / n); };
     // a tile's rows and tokens are addressed by 32-bit offsets
-    if (a.T <= ROWS_T || a.rb >= (1u << 23) || a.xs >= (1 << 22)) return launch_rows<QT, EXACT>(a, st);
+    if (a.T <= ROWS_T || a.rb >= (1u << 23) || a.xs >= (1 << 22)) return launch_rows<QT>(a, st);
     if constexpr (QT == BREAD_QTYPE_Q4_K || QT == BREAD_QTYPE_F16) {
-        if (tiles(256, 256) >= FILL) return launch_tile<QT, 4, 2, 2, 4, 1, EXACT>(a, st);
+        if (tiles(256, 256) >= FILL) return launch_tile<QT, 4, 2, 2, 4, 1>(a, st);
     }
-    if (tiles(128, 256) >= FILL) return launch_tile<QT, 4, 1, 1, 8, 1, EXACT>(a, st);
-    if (tiles(128, 128) >= FILL) return launch_tile<QT, 2, 1, 2, 4, 1, EXACT>(a, st);
+    if (tiles(128, 256) >= FILL) return launch_tile<QT, 4, 1, 1, 8, 1>(a, st);
+    if (tiles(128, 128) >= FILL) return launch_tile<QT, 2, 1, 2, 4, 1>(a, st);
     if (tiles(64, 64) >= FILL) {
         // (Q6_K unpacks with twice the instructions: a wave's weights against twice the tokens)
-        if constexpr (QT == BREAD_QTYPE_Q6_K) return launch_tile<QT, 2, 1, 1, 2, 4, EXACT>(a, st);
-        else return launch_tile<QT, 1, 1, 2, 2, 4, EXACT>(a, st);
+        if constexpr (QT == BREAD_QTYPE_Q6_K) return launch_tile<QT, 2, 1, 1, 2, 4>(a, st);
+        else return launch_tile<QT, 1, 1, 2, 2, 4>(a, st);
     }
-    if (tiles(32, 32) <= 256 && a.cols > 4 * 256) return launch_tile<QT, 1, 1, 1, 1, 8, EXACT>(a, st);
-    return launch_tile<QT, 1, 1, 1, 2, 4, EXACT>(a, st);
+    if (tiles(32, 32) <= 256 && a.cols > 4 * 256) return launch_tile<QT, 1, 1, 1, 1, 8>(a, st);
+    return launch_tile<QT, 1, 1, 1, 2, 4>(a, st);
 }
 
 }  // namespace
@@ -1165,10 +1155,9 @@ extern "C" int bread_matmul(const void *w, const uint16_t *x, void *y, int rows,
     a.y32 = o.y_type == BREAD_QTYPE_F32;
     const hipStream_t st = to_hip(stream);
     switch (qtype) {
-    case BREAD_QTYPE_Q4_K: return launch_matmul<BREAD_QTYPE_Q4_K, false>(a, st);
-    case BREAD_QTYPE_Q6_K:
-        return a.y32 ? launch_matmul<BREAD_QTYPE_Q6_K, true>(a, st) : launch_matmul<BREAD_QTYPE_Q6_K, false>(a, st);
-    case BREAD_QTYPE_Q8_0: return launch_matmul<BREAD_QTYPE_Q8_0, false>(a, st);
-    default: return launch_matmul<BREAD_QTYPE_F16, false>(a, st);
+    case BREAD_QTYPE_Q4_K: return launch_matmul<BREAD_QTYPE_Q4_K>(a, st);
+    case BREAD_QTYPE_Q6_K: return launch_matmul<BREAD_QTYPE_Q6_K>(a, st);
+    case BREAD_QTYPE_Q8_0: return launch_matmul<BREAD_QTYPE_Q8_0>(a, st);
+    default: return launch_matmul<BREAD_QTYPE_F16>(a, st);
     }
 }

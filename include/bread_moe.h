@@ -122,15 +122,14 @@ typedef struct {
  * few tokens, and its tiles are shared by many.  qtype is 12 (Q4_K), 14 (Q6_K),
  * 8 (Q8_0) or 1 (F16); cols must be a multiple of 256 (K-quants), 32 (Q8_0) or
  * 8 (F16).  x is fp16, bias fp32, y and residual are fp16 or fp32 (y_type).
- * Products are exact and sums fp32 (fp16 results from Q6_K: weights whose
- * integer part, scale times code, exceeds 2048 are rounded to 11 bits), and y
- * is rounded once.  opts NULL: fp16 y, packed rows, no epilogue.  w must be
- * 16-byte aligned (Q6_K and Q8_0: 4-byte), x 16-byte aligned with a stride
- * that is a multiple of 8.  y must not overlap x, w or bias, and residual is y
- * or does not overlap it.  Elements of y between one row's end and the next
- * row's start are left as they were.  n_tokens or rows 0: nothing is done; rows
- * and cols up to 2^30, n_tokens up to 2^28 (BREAD_ERR_SHAPE beyond).  No
- * workspace: calls on different streams may overlap. */
+ * Products are exact and sums fp32, and y is rounded once.  opts NULL: fp16 y,
+ * packed rows, no epilogue.  w must be 16-byte aligned (Q6_K and Q8_0: 4-byte),
+ * x 16-byte aligned with a stride that is a multiple of 8.  y must not overlap
+ * x, w or bias, and residual is y or does not overlap it.  Elements of y
+ * between one row's end and the next row's start are left as they were.
+ * n_tokens or rows 0: nothing is done; rows and cols up to 2^30, n_tokens up to
+ * 2^28 (BREAD_ERR_SHAPE beyond).  No workspace: calls on different streams may
+ * overlap. */
 int bread_matmul(const void *w, const uint16_t *x, void *y, int rows, int cols, int qtype, int n_tokens,
                  const bread_matmul_opts_t *opts, bread_stream_t stream);
 
