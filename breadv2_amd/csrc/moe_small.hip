@@ -149,15 +149,27 @@ __device__ void sb_number_slots(const int *sidx, int E, int K, int T, int32_t *_
     for (int t = tid; t < T; t += RT_THREADS) slot_pair[t] = t * (K + 1);  // slot t / SB_CH, place t % SB_CH
 }
 
-// The slots of experts that are already chosen.  One workgroup.
+// The slots of experts that are already chosen, by workgroup 0.  With xq (H = 2048 only) workgroup 1 + t writes
+// token t's activations in the decode shape's fixed-point form.
 __global__ __launch_bounds__(RT_THREADS) void k_sb_slots(const int32_t *__restrict__ idx, int E, int K, int T,
                                                          int32_t *__restrict__ slot_expert,
                                                          int32_t *__restrict__ slot_cnt,
                                                          int32_t *__restrict__ slot_pair,
-                                                         int32_t *__restrict__ n_slots)
+                                                         int32_t *__restrict__ n_slots, const float *__restrict__ x,
+                                                         uint8_t *__restrict__ xq)
 {
     __shared__ int sidx[SB_MAX_T * MAX_K];
-    for (int i = threadIdx.x; i < T * K; i += RT_THREADS) sidx[i] = idx[i];
+    const int tid = (int)threadIdx.x;
+    if (blockIdx.x > 0) {
+        if (tid >= XQ_H / 8) return;
+        const int t = (int)blockIdx.x - 1;
+        const float4 *p = reinterpret_cast<const float4 *>(x + (size_t)t * XQ_H + 8 * tid);
+        const float4 a = p[0], b = p[1];
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        xq16_store(v, tid, xq + (size_t)t * XQ_TOKEN_BYTES);
+        return;
+    }
+    for (int i = tid; i < T * K; i += RT_THREADS) sidx[i] = idx[i];
     __syncthreads();
     sb_number_slots(sidx, E, K, T, slot_expert, slot_cnt, slot_pair, n_slots);
 }
@@ -1138,17 +1150,15 @@ int bread_launch_moe_small(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const
     const bool mv4 = E <= 4 * WAVE;
     // the decode shape: every workgroup owns a slice of every slot
     // (k_sw_gateup / k_sw_down), on the activations in fixed point that
-    // k_route_fast writes
+    // k_route_fast (by a rule k_sb_slots) writes
     const bool cert = bread_route_certified_ok(c, T);
     const bool sw = cert && H == SW_H && I == SW_I && Ish == SW_I && K <= SW_K && T <= SW_MAX_T;
     if (rule) {
-        // the rule's experts from the reference-order logits; at the decode
-        // shape k_route_fast then writes the activations in fixed point
-        int rc = bread_launch_route_by_rule(c, L, rule, x, T, c->idx, c->w, c->gsh, st);
-        if (rc == BREAD_OK && sw) rc = bread_launch_route_fast(c, L, x, T, c->gsh, c->h, g.xq, st);
+        // the rule's experts and the shared gate from the reference-order sums
+        const int rc = bread_launch_route_by_rule(c, L, rule, x, T, c->idx, c->w, c->gsh, st);
         if (rc) return rc;
-        hipLaunchKernelGGL(k_sb_slots, dim3(1), dim3(RT_THREADS), 0, st, c->idx, E, K, T, g.slot_expert, g.slot_cnt,
-                           g.slot_pair, g.n_slots);
+        hipLaunchKernelGGL(k_sb_slots, dim3(sw ? 1 + T : 1), dim3(RT_THREADS), 0, st, c->idx, E, K, T, g.slot_expert,
+                           g.slot_cnt, g.slot_pair, g.n_slots, x, sw ? g.xq : nullptr);
     } else if (cert) {
         float *radii = c->h;
         const int rc = bread_launch_route_fast(c, L, x, T, c->gsh, radii, sw ? g.xq : nullptr, st);
