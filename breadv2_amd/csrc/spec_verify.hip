@@ -64,12 +64,20 @@ struct SvArgs {
 };
 
 // The larger of two, a number against NaN (fmaxf's rule, without the compiler's two extra instructions to quiet
-// its arguments first)
+// its arguments first; of a signalling NaN after nan_is_nan())
 __device__ __forceinline__ float max2(float a, float b)
 {
     float d;
     asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
     return d;
+}
+
+// At a kernel's start: from here on the wave's maxima take a signalling NaN as any other.  With the mode register's
+// IEEE bit (9), which kernels start with, v_max of one and a number is NaN; quieting the logits first would be an
+// instruction for each (for each two, in fp16).
+__device__ __forceinline__ void nan_is_nan()
+{
+    __builtin_amdgcn_s_setreg(1 | (9 << 6) | (0 << 11), 0u);  // hwreg(HW_REG_MODE, 9, 1)
 }
 
 // A logit as a number: NaN counts as -inf
@@ -298,6 +306,7 @@ __global__ __launch_bounds__(SV_THREADS, sizeof(LT) == 2 ? 4 : 3) void k_sv_stat
 {
     constexpr int STEPS = PER * SV_WAVES / 32, STEP = 32 * WAVE;
     __shared__ double s_two[SV_WAVES][32];
+    nan_is_nan();
     const Exp2 e2;
     const int lane = lane_id(), at = (int)blockIdx.x * SV_WAVES + wave_id();
     if (at >= a.R * a.nchunk) return;
@@ -594,6 +603,7 @@ __global__ __launch_bounds__(SV_ROWS *WAVE) void k_sv_accept(const SvArgs a)
     __shared__ SvRow s_row[SV_ROWS];
     __shared__ double s_d[SV_ROWS], s_tot[SV_MAX_CHUNKS];
     __shared__ int s_win;
+    nan_is_nan();
     const Exp2 e2;
     const int b = (int)blockIdx.x, tid = (int)threadIdx.x, wv = wave_id(), lane = lane_id();
     const int r0 = a.off[b], r1 = a.off[b + 1];
@@ -711,6 +721,7 @@ __global__ __launch_bounds__(SV_THREADS) void k_sv_left(const SvArgs a)
 {
     __shared__ double s_d[SV_WAVES], s_tot[SV_MAX_CHUNKS];
     __shared__ int s_win, s_last;
+    nan_is_nan();
     const Exp2 e2;
     const int b = (int)blockIdx.x / a.nchunk, ch = (int)blockIdx.x % a.nchunk;
     const int tid = (int)threadIdx.x;
