@@ -1000,7 +1000,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
             for (int k = 0; k < 16; k++)
                 out[32 * (8 * (k >> 2) + 4 * kh + (k & 3)) + c] = UNIT ? acc[i][j][k] * unit[j] : acc[i][j][k];
             if (KW > 1) __syncthreads();
-            else __builtin_amdgcn_wave_barrier();
+            else wave_order();
             const int r = n0 + 32 * (wn * WN + j) + 4 * (l & 7);
 #pragma unroll 1
             for (int k = kg * 4 / KW; k < (kg + 1) * 4 / KW; k++) {
@@ -1017,7 +1017,7 @@ __global__ __launch_bounds__(WAVE *MW *NW *KW, 2) void k_mm_tile(const MmArgs a,
                 if (t < a.T && r < a.rows) put4(a, t, r, v);
             }
             if (KW > 1) __syncthreads();
-            else __builtin_amdgcn_wave_barrier();
+            else wave_order();
         }
 }
 
