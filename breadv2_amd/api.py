@@ -131,6 +131,8 @@ def bread_matmul(w, x, y, rows: int, cols: int, qtype: int, bias=None, act=None,
     block = _WEIGHT_BLOCKS.get(qtype)
     if block and rows > 0 and cols > 0 and w.numel() * w.element_size() < rows * -(-cols // block[0]) * block[1]:
         raise ValueError("w holds fewer than rows x cols weights")
+    if not w.is_contiguous():
+        raise ValueError("w must be dense")
     bp = rp = None
     if bias is not None:
         if bias.dtype != torch.float32 or not bias.is_contiguous() or bias.numel() != rows:
