@@ -5,6 +5,11 @@ Names mirror the reference's interface for this path (kernels.cu:289
 bread_matvec, one_layer.cu:937 route_layer, the MoE block of
 one_layer_forward one_layer.cu:1800-1986), with the reference's exit(1)
 replaced by a raised BreadError carrying the status code.
+
+A call goes to torch's current stream, or to `stream`.  Tensors that it
+returns are of that stream's memory, as if it had been the current one:
+another stream that uses them waits for it and records itself on them
+(Tensor.record_stream).
 """
 from __future__ import annotations
 
@@ -49,7 +54,21 @@ def _on(stream, tensors) -> int:
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
-    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(dev)
+    if stream.device_index != dev:
+        raise ValueError(f"the stream is on cuda:{stream.device_index}, the current device is cuda:{dev}")
+    return stream.cuda_stream
+
+
+def _empty(stream, size, dtype, device) -> torch.Tensor:
+    """An output of a call on `stream`, from that stream's memory: a block of the
+    current stream's may still be waiting for work queued there before it was
+    freed, and would be handed on there before the call is done with it."""
+    if stream is None:
+        return torch.empty(size, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(size, dtype=dtype, device=device)
 
 
 _HIP = None
@@ -151,7 +170,7 @@ def bread_matmul(w, x, y, rows: int, cols: int, qtype: int, bias=None, act=None,
 
 def bread_dequant_rows(w, qtype: int, rows: int, cols: int, out=None, stream=None) -> torch.Tensor:
     if out is None:
-        out = torch.empty(rows * cols, dtype=torch.float32, device=w.device)
+        out = _empty(stream, rows * cols, torch.float32, w.device)
     check(lib.bread_dequant_rows(_p(w), qtype, rows, cols, _p(out), _s(stream)), "bread_dequant_rows")
     return out
 
@@ -229,9 +248,9 @@ def route_noalloc(s: MoeShape, layer: MoeLayer, x: torch.Tensor, n_tokens: int, 
     """bread_route_noalloc: routing without a context (the library's static
     device workspace holds the logits; n_tokens * n_experts <= 1048576)."""
     K = s.top_k
-    idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
-    w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
-    gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+    idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
+    w = _empty(stream, (n_tokens, K), torch.float32, x.device)
+    gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
     check(lib.bread_route_noalloc(ctypes.byref(s), ctypes.byref(layer), _p(x), n_tokens, _p(idx), _p(w), _p(gsh),
                                   _s(stream)), "bread_route_noalloc")
     return idx, w, gsh
@@ -270,8 +289,8 @@ def route_select(logits: torch.Tensor, top_k: int, rule: RouteRule, stream=None)
     ls = _rows_of(logits, "logits", E)
     st = _on(stream, (logits, rule.bias))
     dev = logits.device
-    idx = torch.empty(T, top_k, dtype=torch.int32, device=dev)
-    w = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    idx = _empty(stream, (T, top_k), torch.int32, dev)
+    w = _empty(stream, (T, top_k), torch.float32, dev)
     rc = lib.bread_route_select(rule.ref, logits.data_ptr(), ls, E, top_k, T, idx.data_ptr(), w.data_ptr(), st)
     if rc:
         check(rc, "bread_route_select")
@@ -350,7 +369,7 @@ def synth_layer_tensors(s: MoeShape, seed: int, layer: int = 0, router_std: floa
 def argmax_f16(logits: torch.Tensor, stream=None) -> torch.Tensor:
     """bread_argmax_f16 over the rows of a 2-d fp16 device tensor."""
     assert logits.dtype == torch.float16 and logits.dim() == 2 and logits.is_contiguous()
-    out = torch.empty((logits.shape[0],), dtype=torch.int32, device=logits.device)
+    out = _empty(stream, (logits.shape[0],), torch.int32, logits.device)
     check(lib.bread_argmax_f16(_p(logits), logits.shape[1], logits.shape[0], _p(out), _s(stream)),
           "bread_argmax_f16")
     return out
@@ -531,9 +550,9 @@ class MoeContext:
 
     def route(self, layer: MoeLayer, x: torch.Tensor, n_tokens: int, stream=None):
         K = self.shape.top_k
-        idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
-        w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
-        gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+        idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
+        w = _empty(stream, (n_tokens, K), torch.float32, x.device)
+        gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
         check(lib.bread_route(self._h, ctypes.byref(layer), _p(x), n_tokens, _p(idx), _p(w), _p(gsh), _s(stream)),
               "bread_route")
         return idx, w, gsh
@@ -566,9 +585,9 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
-            w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
-            gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+            idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
+            w = _empty(stream, (n_tokens, K), torch.float32, x.device)
+            gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
         check(lib.bread_moe_forward(self._h, ctypes.byref(layer), _p(x), _p(hidden), n_tokens, _p(idx), _p(w),
                                     _p(gsh), _s(stream)), "bread_moe_forward")
         return idx, w, gsh
@@ -578,9 +597,9 @@ class MoeContext:
         K = self.shape.top_k
         rule.check(self.shape.n_experts)
         st = _on(stream, (x, rule.bias))
-        idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
-        w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
-        gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+        idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
+        w = _empty(stream, (n_tokens, K), torch.float32, x.device)
+        gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
         check(lib.bread_route_by_rule(self._h, ctypes.byref(layer), rule.ref, _p(x), n_tokens, _p(idx),
                                       _p(w), _p(gsh), st), "bread_route_by_rule")
         return idx, w, gsh
@@ -593,9 +612,9 @@ class MoeContext:
         st = _on(stream, (x, hidden, rule.bias))
         idx = w = gsh = None
         if want_routing:
-            idx = torch.empty((n_tokens, K), dtype=torch.int32, device=x.device)
-            w = torch.empty((n_tokens, K), dtype=torch.float32, device=x.device)
-            gsh = torch.empty((n_tokens,), dtype=torch.float32, device=x.device)
+            idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
+            w = _empty(stream, (n_tokens, K), torch.float32, x.device)
+            gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
         check(lib.bread_moe_forward_by_rule(self._h, ctypes.byref(layer), rule.ref, _p(x), _p(hidden),
                                             n_tokens, _p(idx), _p(w), _p(gsh), st), "bread_moe_forward_by_rule")
         return idx, w, gsh
@@ -630,11 +649,11 @@ class MoeContext:
                 raise ValueError("temperature must be dense float32 [n_requests]")
             tp = temperature.data_ptr()
         st = _on(stream, (logits, tokens, offsets, u, draft_probs, temperature))
-        accepted = torch.empty((B,), dtype=torch.int32, device=logits.device)
-        following = torch.empty((B,), dtype=torch.int32, device=logits.device)
+        accepted = _empty(stream, (B,), torch.int32, logits.device)
+        following = _empty(stream, (B,), torch.int32, logits.device)
         logp = None
         if want_logprob:
-            logp = torch.empty((R,), dtype=torch.float32, device=logits.device)
+            logp = _empty(stream, (R,), torch.float32, logits.device)
             lp = logp.data_ptr()
         a = _lib.VerifyArgs(logits.data_ptr(), _rows_of(logits, "logits", V), z_type, V, R, B, tokens.data_ptr(),
                             offsets.data_ptr(), u.data_ptr(), qp, qs, tp, eos, accepted.data_ptr(),
@@ -662,9 +681,9 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = torch.empty((n_tokens, K), dtype=torch.int32, device=hidden.device)
-            w = torch.empty((n_tokens, K), dtype=torch.float32, device=hidden.device)
-            gsh = torch.empty((n_tokens,), dtype=torch.float32, device=hidden.device)
+            idx = _empty(stream, (n_tokens, K), torch.int32, hidden.device)
+            w = _empty(stream, (n_tokens, K), torch.float32, hidden.device)
+            gsh = _empty(stream, (n_tokens,), torch.float32, hidden.device)
         nw = norm_w if isinstance(norm_w, int) or norm_w is None else norm_w.data_ptr()
         check(lib.bread_moe_forward_f16(self._h, ctypes.byref(layer), nw, _p(hidden), _p(normed), n_tokens, _p(idx),
                                         _p(w), _p(gsh), _s(stream)), "bread_moe_forward_f16")
@@ -678,9 +697,9 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = torch.empty((n, K), dtype=torch.int32, device=hidden.device)
-            w = torch.empty((n, K), dtype=torch.float32, device=hidden.device)
-            gsh = torch.empty((n,), dtype=torch.float32, device=hidden.device)
+            idx = _empty(stream, (n, K), torch.int32, hidden.device)
+            w = _empty(stream, (n, K), torch.float32, hidden.device)
+            gsh = _empty(stream, (n,), torch.float32, hidden.device)
         check(lib.bread_moe_decode_layers(self._h, arr, n, _p(hidden), _p(idx), _p(w), _p(gsh), _s(stream)),
               "bread_moe_decode_layers")
         return idx, w, gsh
@@ -711,9 +730,9 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = torch.empty((n, n_tokens, K), dtype=torch.int32, device=hidden.device)
-            w = torch.empty((n, n_tokens, K), dtype=torch.float32, device=hidden.device)
-            gsh = torch.empty((n, n_tokens), dtype=torch.float32, device=hidden.device)
+            idx = _empty(stream, (n, n_tokens, K), torch.int32, hidden.device)
+            w = _empty(stream, (n, n_tokens, K), torch.float32, hidden.device)
+            gsh = _empty(stream, (n, n_tokens), torch.float32, hidden.device)
         check(lib.bread_moe_stack_forward(self._h, arr, n, _p(hidden), n_tokens, _p(idx), _p(w), _p(gsh),
                                           _s(stream)), "bread_moe_stack_forward")
         return idx, w, gsh
@@ -722,8 +741,8 @@ class MoeContext:
                     vocab: int, n_tokens: int, stream=None):
         """bread_moe_greedy_head: (tokens int32 [n_tokens], fp16 logits
         [n_tokens][vocab]) of the output norm + lm_head + greedy argmax."""
-        logits = torch.empty((n_tokens, vocab), dtype=torch.float16, device=hidden.device)
-        tokens = torch.empty((n_tokens,), dtype=torch.int32, device=hidden.device)
+        logits = _empty(stream, (n_tokens, vocab), torch.float16, hidden.device)
+        tokens = _empty(stream, (n_tokens,), torch.int32, hidden.device)
         check(lib.bread_moe_greedy_head(self._h, _p(hidden), _p(norm_w), _p(w_out), qtype, vocab, n_tokens,
                                         _p(logits), _p(tokens), _s(stream)), "bread_moe_greedy_head")
         return tokens, logits
