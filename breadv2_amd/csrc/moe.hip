@@ -654,35 +654,37 @@ static bool grouped_takes_mix(const bread_moe_shape_t &s, const bread_moe_layer_
            ((uintptr_t)hidden & 15) == 0;
 }
 
-// bread_moe_forward, and with a rule bread_moe_forward_by_rule
-static int moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const bread_route_rule_t *rule, const float *x,
-                       float *hidden, int T, int32_t *idx, float *w, float *gsh, bread_stream_t stream)
+// bread_moe_forward, and with a rule bread_moe_forward_by_rule; who: the entry point, for its errors
+static int moe_forward(const char *who, bread_moe_ctx_t *c, const bread_moe_layer_t *L,
+                       const bread_route_rule_t *rule, const float *x, float *hidden, int T, int32_t *idx, float *w,
+                       float *gsh, bread_stream_t stream)
 {
     int rc = BREAD_OK;
     if (T == 0) return BREAD_OK;
     hipStream_t st = to_hip(stream);
     c->last_stream = st;
-    if (c->path == BREAD_PATH_DECODE || c->path == BREAD_PATH_GROUPED || c->path == BREAD_PATH_SMALL)
-        BREAD_REQUIRE(bread_standard_qtypes(L), BREAD_ERR_QTYPE,
-                      "pinned, the decode, small-batch and grouped paths take Q4_K gate/up and Q6_K down "
-                      "(BREAD_PATH_PER_TOKEN and BREAD_PATH_AUTO take any mix of Q4_K and Q6_K)");
+    if ((c->path == BREAD_PATH_DECODE || c->path == BREAD_PATH_GROUPED || c->path == BREAD_PATH_SMALL) &&
+        !bread_standard_qtypes(L))
+        return bread_fail(BREAD_ERR_QTYPE, who,
+                          "pinned, the decode, small-batch and grouped paths take Q4_K gate/up and Q6_K down "
+                          "(BREAD_PATH_PER_TOKEN and BREAD_PATH_AUTO take any mix of Q4_K and Q6_K)");
     switch (c->path) {
     case BREAD_PATH_DECODE:
-        BREAD_REQUIRE(T == 1, BREAD_ERR_SHAPE, "the decode path takes one token");
-        BREAD_REQUIRE(!rule, BREAD_ERR_SHAPE, "the decode path routes by softmax only");
+        if (T != 1) return bread_fail(BREAD_ERR_SHAPE, who, "the decode path takes one token");
+        if (rule) return bread_fail(BREAD_ERR_SHAPE, who, "the decode path routes by softmax only");
         rc = bread_launch_moe_decode(c, L, x, hidden, st);
-        if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, "bread_moe_forward", "shape not supported by the decode kernel");
+        if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, who, "shape not supported by the decode kernel");
         break;
     case BREAD_PATH_GROUPED:
         rc = bread_launch_moe_grouped(c, L, x, hidden, T, st, rule);
-        if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, "bread_moe_forward", "shape not supported by the grouped path");
+        if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, who, "shape not supported by the grouped path");
         break;
     case BREAD_PATH_PER_TOKEN:
         rc = bread_launch_moe_multi(c, L, x, hidden, T, st, rule);
         break;
     case BREAD_PATH_SMALL:
         rc = bread_launch_moe_small(c, L, x, hidden, T, st, rule);
-        if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, "bread_moe_forward", "shape not supported by the small-batch path");
+        if (rc == BREAD_ERR_SHAPE) return bread_fail(rc, who, "shape not supported by the small-batch path");
         break;
     default:
         rc = (T == 1 && !rule) ? bread_launch_moe_decode(c, L, x, hidden, st) : BREAD_ERR_SHAPE;
@@ -706,7 +708,7 @@ extern "C" int bread_moe_forward(bread_moe_ctx_t *c, const bread_moe_layer_t *L,
     const int rc = check_tokens(c, L, x, T);
     if (rc) return rc;
     BREAD_REQUIRE(hidden, BREAD_ERR_ARG, "NULL hidden");
-    return moe_forward(c, L, nullptr, x, hidden, T, idx, w, gsh, stream);
+    return moe_forward(__func__, c, L, nullptr, x, hidden, T, idx, w, gsh, stream);
 }
 
 extern "C" int bread_moe_forward_by_rule(bread_moe_ctx_t *c, const bread_moe_layer_t *L,
@@ -718,7 +720,7 @@ extern "C" int bread_moe_forward_by_rule(bread_moe_ctx_t *c, const bread_moe_lay
     BREAD_REQUIRE(hidden, BREAD_ERR_ARG, "NULL hidden");
     rc = bread_validate_rule(rule, c->shape.n_experts, c->shape.top_k);
     if (rc) return rc;
-    return moe_forward(c, L, rule, x, hidden, T, idx, w, gsh, stream);
+    return moe_forward(__func__, c, L, rule, x, hidden, T, idx, w, gsh, stream);
 }
 
 extern "C" int bread_route_by_rule(bread_moe_ctx_t *c, const bread_moe_layer_t *L, const bread_route_rule_t *rule,
