@@ -426,7 +426,8 @@ extern "C" int bread_route_select(const bread_route_rule_t *rule, const float *l
     const int rc = bread_validate_rule(rule, E, K);
     if (rc) return rc;
     BREAD_REQUIRE(T >= 0, BREAD_ERR_ARG, "n_tokens < 0");
-    BREAD_REQUIRE(T <= 1 << 26, BREAD_ERR_SHAPE, "n_tokens above 2^26");
+    // (four tokens a workgroup of 256 for many experts: 2^32 threads are one launch's limit)
+    BREAD_REQUIRE(T <= (1 << 26) - 4, BREAD_ERR_SHAPE, "n_tokens above 2^26 - 4");
     BREAD_REQUIRE(stride == 0 || stride >= E, BREAD_ERR_SHAPE, "stride smaller than n_experts");
     if (T == 0) return BREAD_OK;
     BREAD_REQUIRE(logits && idx && w, BREAD_ERR_ARG, "NULL input or output");

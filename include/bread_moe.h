@@ -298,8 +298,8 @@ typedef struct {
 /* Experts and weights of n_tokens tokens from their router logits by a rule.
  * d_logits fp32, n_experts (up to 1024) of a token every `stride` floats (0:
  * n_experts); d_idx int32 and d_w fp32 [n_tokens][top_k], top_k up to 32,
- * n_tokens up to 2^26.  A bias has no infinities of both signs in one group.  No
- * workspace: calls on different streams may overlap. */
+ * n_tokens up to 2^26 - 4.  A bias has no infinities of both signs in one
+ * group.  No workspace: calls on different streams may overlap. */
 int bread_route_select(const bread_route_rule_t *rule, const float *d_logits, int64_t stride, int n_experts,
                        int top_k, int n_tokens, int32_t *d_idx, float *d_w, bread_stream_t stream);
 
