@@ -281,8 +281,9 @@ int bread_route_noalloc(const bread_moe_shape_t *shape, const bread_moe_layer_t 
  * largest c among them are chosen, in that order, ties everywhere to the lower
  * index; the weight of rank k is its s (never c), divided by the chosen ones'
  * sum if renorm, times scale.  Scores and choices are compared in 64 bits.  A
- * logit of NaN or -inf has score 0; +inf logits share softmax evenly; where
- * the chosen scores sum to zero, renorm gives weights of zero.
+ * logit of NaN or -inf has score 0 (sigmoid: one below -700 too); +inf logits
+ * share softmax evenly; where the chosen scores sum to zero, renorm gives
+ * weights of zero.  A bias of NaN puts its expert last, in its group as -inf.
  * route_layer's own rule (one_layer.cu:983-985) is softmax, no bias, one
  * group, renorm, scale 1. */
 typedef struct {
@@ -298,8 +299,8 @@ typedef struct {
 /* Experts and weights of n_tokens tokens from their router logits by a rule.
  * d_logits fp32, n_experts (up to 1024) of a token every `stride` floats (0:
  * n_experts); d_idx int32 and d_w fp32 [n_tokens][top_k], top_k up to 32,
- * n_tokens up to 2^26 - 4.  A bias has no infinities of both signs in one
- * group.  No workspace: calls on different streams may overlap. */
+ * n_tokens up to 2^26 - 4.  No group has a bias of +inf next to one of -inf or
+ * NaN.  No workspace: calls on different streams may overlap. */
 int bread_route_select(const bread_route_rule_t *rule, const float *d_logits, int64_t stride, int n_experts,
                        int top_k, int n_tokens, int32_t *d_idx, float *d_w, bread_stream_t stream);
 
@@ -437,12 +438,14 @@ int bread_spec_accept(const int32_t *pred, const int32_t *draft, int n_draft, in
 /* Verification of drafted tokens by sampling, for many requests at once: the
  * acceptance of main_speculative.cu:477-497 for requests that sample, with
  * the random numbers given.  Request b has the rows offsets[b] to
- * offsets[b + 1] - 1 (at least one; offsets[0] = 0, offsets[n_requests] =
- * n_rows): tokens[r] is the token that was run at row r (the request's first:
- * its last confirmed token; the others: its drafts in order) and logits[r]
- * the target's logits after it.  With p_r = softmax(logits[r] /
- * temperature[b]) and q_r the probabilities that the draft tokens[r + 1] was
- * drawn from, draft tokens[r + 1] stands when u[r] * q_r(draft) < p_r(draft).
+ * offsets[b + 1] - 1, at least one (0 <= offsets[0], offsets[n_requests] <=
+ * n_rows; rows before and behind are no request's, whatever they hold, and
+ * their logprob is left as it was): tokens[r] is the token that was run at row
+ * r (the request's first: its last confirmed token; the others: its drafts in
+ * order) and logits[r] the target's logits after it.  With p_r =
+ * softmax(logits[r] / temperature[b]) and q_r the probabilities that the draft
+ * tokens[r + 1] was drawn from, draft tokens[r + 1] stands when
+ * u[r] * q_r(draft) < p_r(draft).
  * Drafts are taken in order; the request stops at row r
  *   - where a draft falls: next is drawn from max(p_r - q_r, 0) (from p_r if
  *     that is zero everywhere);
@@ -463,7 +466,8 @@ int bread_spec_accept(const int32_t *pred, const int32_t *draft, int n_draft, in
  * Every buffer is on the device.  n_rows <= the context's max_tokens; the
  * partial sums live in its scratch (BREAD_ERR_CAPACITY if a vocabulary is too
  * large for it: 16 bytes for every 8192 tokens of each row, and 16, and 8 for
- * every 8192 tokens, of each request).  Offsets that do not fit set bit 64 of the error word. */
+ * every 8192 tokens, of each request).  A request whose offsets do not fit sets
+ * bit 64 of the error word. */
 typedef struct {
     const void *logits;        /* [n_rows][vocab], fp16 or fp32 */
     int64_t logits_stride;     /* elements from one row to the next; 0: vocab */
