@@ -61,14 +61,19 @@ def _on(stream, tensors) -> int:
     return stream.cuda_stream
 
 
-def _empty(stream, size, dtype, device) -> torch.Tensor:
-    """An output of a call on `stream`, from that stream's memory: a block of the
-    current stream's may still be waiting for work queued there before it was
-    freed, and would be handed on there before the call is done with it."""
+def _empty(stream):
+    """torch.empty for the outputs of a call on `stream`, from that stream's memory:
+    a block of the current stream's may still be waiting for work queued there
+    before it was freed, and would be handed on there before the call is done
+    with it."""
     if stream is None:
-        return torch.empty(size, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(size, dtype=dtype, device=device)
+        return torch.empty
+
+    def empty(*size, dtype, device):
+        with torch.cuda.stream(stream):
+            return torch.empty(*size, dtype=dtype, device=device)
+
+    return empty
 
 
 _HIP = None
@@ -170,7 +175,8 @@ def bread_matmul(w, x, y, rows: int, cols: int, qtype: int, bias=None, act=None,
 
 def bread_dequant_rows(w, qtype: int, rows: int, cols: int, out=None, stream=None) -> torch.Tensor:
     if out is None:
-        out = _empty(stream, rows * cols, torch.float32, w.device)
+        empty = _empty(stream)
+        out = empty(rows * cols, dtype=torch.float32, device=w.device)
     check(lib.bread_dequant_rows(_p(w), qtype, rows, cols, _p(out), _s(stream)), "bread_dequant_rows")
     return out
 
@@ -248,9 +254,10 @@ def route_noalloc(s: MoeShape, layer: MoeLayer, x: torch.Tensor, n_tokens: int, 
     """bread_route_noalloc: routing without a context (the library's static
     device workspace holds the logits; n_tokens * n_experts <= 1048576)."""
     K = s.top_k
-    idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
-    w = _empty(stream, (n_tokens, K), torch.float32, x.device)
-    gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
+    empty = _empty(stream)
+    idx = empty((n_tokens, K), dtype=torch.int32, device=x.device)
+    w = empty((n_tokens, K), dtype=torch.float32, device=x.device)
+    gsh = empty((n_tokens,), dtype=torch.float32, device=x.device)
     check(lib.bread_route_noalloc(ctypes.byref(s), ctypes.byref(layer), _p(x), n_tokens, _p(idx), _p(w), _p(gsh),
                                   _s(stream)), "bread_route_noalloc")
     return idx, w, gsh
@@ -289,8 +296,9 @@ def route_select(logits: torch.Tensor, top_k: int, rule: RouteRule, stream=None)
     ls = _rows_of(logits, "logits", E)
     st = _on(stream, (logits, rule.bias))
     dev = logits.device
-    idx = _empty(stream, (T, top_k), torch.int32, dev)
-    w = _empty(stream, (T, top_k), torch.float32, dev)
+    empty = _empty(stream)
+    idx = empty(T, top_k, dtype=torch.int32, device=dev)
+    w = empty(T, top_k, dtype=torch.float32, device=dev)
     rc = lib.bread_route_select(rule.ref, logits.data_ptr(), ls, E, top_k, T, idx.data_ptr(), w.data_ptr(), st)
     if rc:
         check(rc, "bread_route_select")
@@ -369,7 +377,8 @@ def synth_layer_tensors(s: MoeShape, seed: int, layer: int = 0, router_std: floa
 def argmax_f16(logits: torch.Tensor, stream=None) -> torch.Tensor:
     """bread_argmax_f16 over the rows of a 2-d fp16 device tensor."""
     assert logits.dtype == torch.float16 and logits.dim() == 2 and logits.is_contiguous()
-    out = _empty(stream, (logits.shape[0],), torch.int32, logits.device)
+    empty = _empty(stream)
+    out = empty((logits.shape[0],), dtype=torch.int32, device=logits.device)
     check(lib.bread_argmax_f16(_p(logits), logits.shape[1], logits.shape[0], _p(out), _s(stream)),
           "bread_argmax_f16")
     return out
@@ -550,9 +559,10 @@ class MoeContext:
 
     def route(self, layer: MoeLayer, x: torch.Tensor, n_tokens: int, stream=None):
         K = self.shape.top_k
-        idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
-        w = _empty(stream, (n_tokens, K), torch.float32, x.device)
-        gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
+        empty = _empty(stream)
+        idx = empty((n_tokens, K), dtype=torch.int32, device=x.device)
+        w = empty((n_tokens, K), dtype=torch.float32, device=x.device)
+        gsh = empty((n_tokens,), dtype=torch.float32, device=x.device)
         check(lib.bread_route(self._h, ctypes.byref(layer), _p(x), n_tokens, _p(idx), _p(w), _p(gsh), _s(stream)),
               "bread_route")
         return idx, w, gsh
@@ -585,9 +595,10 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
-            w = _empty(stream, (n_tokens, K), torch.float32, x.device)
-            gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
+            empty = _empty(stream)
+            idx = empty((n_tokens, K), dtype=torch.int32, device=x.device)
+            w = empty((n_tokens, K), dtype=torch.float32, device=x.device)
+            gsh = empty((n_tokens,), dtype=torch.float32, device=x.device)
         check(lib.bread_moe_forward(self._h, ctypes.byref(layer), _p(x), _p(hidden), n_tokens, _p(idx), _p(w),
                                     _p(gsh), _s(stream)), "bread_moe_forward")
         return idx, w, gsh
@@ -597,9 +608,10 @@ class MoeContext:
         K = self.shape.top_k
         rule.check(self.shape.n_experts)
         st = _on(stream, (x, rule.bias))
-        idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
-        w = _empty(stream, (n_tokens, K), torch.float32, x.device)
-        gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
+        empty = _empty(stream)
+        idx = empty((n_tokens, K), dtype=torch.int32, device=x.device)
+        w = empty((n_tokens, K), dtype=torch.float32, device=x.device)
+        gsh = empty((n_tokens,), dtype=torch.float32, device=x.device)
         check(lib.bread_route_by_rule(self._h, ctypes.byref(layer), rule.ref, _p(x), n_tokens, _p(idx),
                                       _p(w), _p(gsh), st), "bread_route_by_rule")
         return idx, w, gsh
@@ -612,9 +624,10 @@ class MoeContext:
         st = _on(stream, (x, hidden, rule.bias))
         idx = w = gsh = None
         if want_routing:
-            idx = _empty(stream, (n_tokens, K), torch.int32, x.device)
-            w = _empty(stream, (n_tokens, K), torch.float32, x.device)
-            gsh = _empty(stream, (n_tokens,), torch.float32, x.device)
+            empty = _empty(stream)
+            idx = empty((n_tokens, K), dtype=torch.int32, device=x.device)
+            w = empty((n_tokens, K), dtype=torch.float32, device=x.device)
+            gsh = empty((n_tokens,), dtype=torch.float32, device=x.device)
         check(lib.bread_moe_forward_by_rule(self._h, ctypes.byref(layer), rule.ref, _p(x), _p(hidden),
                                             n_tokens, _p(idx), _p(w), _p(gsh), st), "bread_moe_forward_by_rule")
         return idx, w, gsh
@@ -649,11 +662,12 @@ class MoeContext:
                 raise ValueError("temperature must be dense float32 [n_requests]")
             tp = temperature.data_ptr()
         st = _on(stream, (logits, tokens, offsets, u, draft_probs, temperature))
-        accepted = _empty(stream, (B,), torch.int32, logits.device)
-        following = _empty(stream, (B,), torch.int32, logits.device)
+        empty = _empty(stream)
+        accepted = empty((B,), dtype=torch.int32, device=logits.device)
+        following = empty((B,), dtype=torch.int32, device=logits.device)
         logp = None
         if want_logprob:
-            logp = _empty(stream, (R,), torch.float32, logits.device)
+            logp = empty((R,), dtype=torch.float32, device=logits.device)
             lp = logp.data_ptr()
         a = _lib.VerifyArgs(logits.data_ptr(), _rows_of(logits, "logits", V), z_type, V, R, B, tokens.data_ptr(),
                             offsets.data_ptr(), u.data_ptr(), qp, qs, tp, eos, accepted.data_ptr(),
@@ -681,9 +695,10 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = _empty(stream, (n_tokens, K), torch.int32, hidden.device)
-            w = _empty(stream, (n_tokens, K), torch.float32, hidden.device)
-            gsh = _empty(stream, (n_tokens,), torch.float32, hidden.device)
+            empty = _empty(stream)
+            idx = empty((n_tokens, K), dtype=torch.int32, device=hidden.device)
+            w = empty((n_tokens, K), dtype=torch.float32, device=hidden.device)
+            gsh = empty((n_tokens,), dtype=torch.float32, device=hidden.device)
         nw = norm_w if isinstance(norm_w, int) or norm_w is None else norm_w.data_ptr()
         check(lib.bread_moe_forward_f16(self._h, ctypes.byref(layer), nw, _p(hidden), _p(normed), n_tokens, _p(idx),
                                         _p(w), _p(gsh), _s(stream)), "bread_moe_forward_f16")
@@ -697,9 +712,10 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = _empty(stream, (n, K), torch.int32, hidden.device)
-            w = _empty(stream, (n, K), torch.float32, hidden.device)
-            gsh = _empty(stream, (n,), torch.float32, hidden.device)
+            empty = _empty(stream)
+            idx = empty((n, K), dtype=torch.int32, device=hidden.device)
+            w = empty((n, K), dtype=torch.float32, device=hidden.device)
+            gsh = empty((n,), dtype=torch.float32, device=hidden.device)
         check(lib.bread_moe_decode_layers(self._h, arr, n, _p(hidden), _p(idx), _p(w), _p(gsh), _s(stream)),
               "bread_moe_decode_layers")
         return idx, w, gsh
@@ -730,9 +746,10 @@ class MoeContext:
         K = self.shape.top_k
         idx = w = gsh = None
         if want_routing:
-            idx = _empty(stream, (n, n_tokens, K), torch.int32, hidden.device)
-            w = _empty(stream, (n, n_tokens, K), torch.float32, hidden.device)
-            gsh = _empty(stream, (n, n_tokens), torch.float32, hidden.device)
+            empty = _empty(stream)
+            idx = empty((n, n_tokens, K), dtype=torch.int32, device=hidden.device)
+            w = empty((n, n_tokens, K), dtype=torch.float32, device=hidden.device)
+            gsh = empty((n, n_tokens), dtype=torch.float32, device=hidden.device)
         check(lib.bread_moe_stack_forward(self._h, arr, n, _p(hidden), n_tokens, _p(idx), _p(w), _p(gsh),
                                           _s(stream)), "bread_moe_stack_forward")
         return idx, w, gsh
@@ -741,8 +758,9 @@ class MoeContext:
                     vocab: int, n_tokens: int, stream=None):
         """bread_moe_greedy_head: (tokens int32 [n_tokens], fp16 logits
         [n_tokens][vocab]) of the output norm + lm_head + greedy argmax."""
-        logits = _empty(stream, (n_tokens, vocab), torch.float16, hidden.device)
-        tokens = _empty(stream, (n_tokens,), torch.int32, hidden.device)
+        empty = _empty(stream)
+        logits = empty((n_tokens, vocab), dtype=torch.float16, device=hidden.device)
+        tokens = empty((n_tokens,), dtype=torch.int32, device=hidden.device)
         check(lib.bread_moe_greedy_head(self._h, _p(hidden), _p(norm_w), _p(w_out), qtype, vocab, n_tokens,
                                         _p(logits), _p(tokens), _s(stream)), "bread_moe_greedy_head")
         return tokens, logits
