@@ -127,6 +127,8 @@ typedef struct {
  * x 16-byte aligned with a stride that is a multiple of 8.  y must not overlap
  * x, w or bias, and residual is y or does not overlap it.  Elements of y
  * between one row's end and the next row's start are left as they were.
+ * An infinity or NaN in a token's x stays in its results, where K-quants may
+ * give NaN for an infinite sum: their scaled codes and mins are summed apart.
  * n_tokens or rows 0: nothing is done; rows and cols up to 2^30, n_tokens up to
  * 2^28 (BREAD_ERR_SHAPE beyond).  No workspace: calls on different streams may
  * overlap. */
