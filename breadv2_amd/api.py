@@ -603,10 +603,15 @@ class MoeContext:
                                     _p(gsh), _s(stream)), "bread_moe_forward")
         return idx, w, gsh
 
+    def _check_rows(self, name: str, t: torch.Tensor, n_tokens: int) -> None:
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n_tokens * self.shape.hidden:
+            raise ValueError(f"{name} must be dense float32 with n_tokens rows of the context's hidden size")
+
     def route_by_rule(self, layer: MoeLayer, rule: RouteRule, x: torch.Tensor, n_tokens: int, stream=None):
         """bread_route_by_rule: route() with the experts and weights of a rule."""
         K = self.shape.top_k
         rule.check(self.shape.n_experts)
+        self._check_rows("x", x, n_tokens)
         st = _on(stream, (x, rule.bias))
         empty = _empty(stream)
         idx = empty((n_tokens, K), dtype=torch.int32, device=x.device)
@@ -621,6 +626,8 @@ class MoeContext:
         """bread_moe_forward_by_rule: forward() with the experts and weights of a rule."""
         K = self.shape.top_k
         rule.check(self.shape.n_experts)
+        self._check_rows("x", x, n_tokens)
+        self._check_rows("hidden", hidden, n_tokens)
         st = _on(stream, (x, hidden, rule.bias))
         idx = w = gsh = None
         if want_routing:
