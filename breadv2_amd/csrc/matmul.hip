@@ -447,7 +447,8 @@ constexpr int MR_MAXTT = 4;  // 16-token tiles a workgroup
 // HOLD: a row has no more chunks than waves (1) or twice as many (2), and a wave keeps its activations in registers
 // for all its row tiles (reading them again for every tile took the vocabulary's logits from 111 to 167 us) and loads
 // the next weights while it works on one chunk.  Two workgroups a CU, so at most 128 registers (20 tokens, Q4_K: 105 us with
-// one, 89 with two); fp16 rows for 17 to 32 tokens would not fit them (117 us, spilled 285).
+// one, 89 with two); fp16 rows for 17 to 32 tokens would not fit them (117 us, spilled 285).  Two chunks held spill 15
+// registers for Q4_K and 3 for Q6_K, 17 to 32 tokens of Q4_K 1.
 // MI355X, 9 tokens: 248320 x 2048 Q6_K 112 to 115 us (3.7 TB/s), Q4_K 66 to 76 us (4 TB/s), 8192 x 2048 Q4_K 7.1 us.  Bound by
 // the loads: a lane's load from a row of its own costs the address unit a cycle, four loads and 64 lanes a chunk of
 // Q6_K.  Rows brought through LDS in the order they lie in took as long (110 us; 91 without the products), and so did
@@ -1046,7 +1047,7 @@ int launch_rows(const MmArgs &a, hipStream_t st)
     const int sets = (a.cols + 256 * MR_WAVES - 1) / (256 * MR_WAVES);  // chunks of a wave
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, ny, (int)stride); };
     // Two chunks are held for row tiles enough to make up for a workgroup less on a CU or registers at their limit.
-    // 9 tokens by 40000 x 4096, not held and held: Q4_K 50 and 37 us, Q6_K 56 and 42, Q8_0 62 and 54; by 8192 x 2304
+    // 9 tokens by 40000 x 4096, not held and held: Q4_K 50 and 37 us, Q6_K 58 and 47, Q8_0 62 and 54; by 8192 x 2304
     // Q4_K, one tile a workgroup, 7.5 and 9.3.  Two fp16 chunks beside their activations would not fit the registers.
     if (ntt == 1 && sets == 1) go(k_mm_rows<QT, 1, 1>);
     else if (ntt == 1 && sets == 2 && QT != BREAD_QTYPE_F16 && ntile >= 2 * stride) go(k_mm_rows<QT, 1, QT == BREAD_QTYPE_F16 ? 0 : 2>);
@@ -1069,16 +1070,17 @@ int launch_rows(const MmArgs &a, hipStream_t st)
 //         256         4096 x 2048       78.6  15.8   14.1   30.8    44.9    81.1
 //        1024         4096 x 2048        274  56.9   55.5   39.4    50.1    84.3
 //        2048         8192 x 2048       1011   220    226    141     109     102
-//   Q6_K  509         2048 x 4096       77.5  37.3   27.5   53.8    80.6     183
-//        1024         8192 x 2048        314   166    113   70.5    57.3     112
+//   Q6_K  509         2048 x 4096       81.8  44.2   30.0   68.6     104
+//        1024         8192 x 2048          -   189    129   83.8    70.7
 //   Q8_0 1024         4096 x 2048        219  84.0   58.7   38.2    59.9     176
 //        2048         8192 x 2048        866   331    247    145     127     225
 //   fp16 2048         8192 x 2048       1068   338    253    112     112    90.1
-// (256 x 256 of Q6_K and Q8_0 do not fit their registers and are not built.)
+// (256 x 256 of Q6_K and Q8_0 do not fit their registers and are not built.  Q8_0's 128 x 256 and 64 x 64 are at their
+// limit and spill 13 and 11.)
 // Where 32 x 32 tiles are no more than the CUs, a workgroup has one, with its superblocks over eight groups and not
 // four: a round fewer to wait for.  us with 32 x 64 and four groups, and with 32 x 32 and eight:
 //   Q8_0   67 tokens, 2048 x 4096   19.0  12.3     Q4_K   64 tokens, 2048 x 2048   9.7   8.0
-//   Q6_K   64         2048 x 4096   21.6  13.1     fp16  128         2048 x 4096  18.4  13.8
+//   Q6_K   64         2048 x 4096   22.2  13.7     fp16  128         2048 x 4096  18.4  13.8
 //   448 tiles, Q8_0, 200 tokens, 2048 x 4096       19.1  21.5
 //   four groups for two superblocks, Q4_K, 64 tokens, 2048 x 512                   6.3   7.6
 // (A group is then one wave and needs no barriers: 1.5 us of the 12.3.)
