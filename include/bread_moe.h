@@ -358,9 +358,10 @@ int bread_moe_forward(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer,
                       const float *d_x_normed, float *d_hidden, int n_tokens,
                       int32_t *d_idx, float *d_w, float *d_gsh, bread_stream_t stream);
 
-/* bread_moe_forward with the experts and weights of bread_route_by_rule.  The
- * decode kernel has route_layer's rule built in, so a single token takes the
- * small-batch path here; BREAD_PATH_DECODE returns BREAD_ERR_SHAPE. */
+/* bread_moe_forward with the experts, weights and shared-gate scores of
+ * bread_route_by_rule, bit for bit on every path.  The decode kernel has
+ * route_layer's rule built in, so a single token takes the small-batch path
+ * here; BREAD_PATH_DECODE returns BREAD_ERR_SHAPE. */
 int bread_moe_forward_by_rule(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer,
                               const bread_route_rule_t *rule, const float *d_x_normed, float *d_hidden,
                               int n_tokens, int32_t *d_idx, float *d_w, float *d_gsh, bread_stream_t stream);
