@@ -77,3 +77,26 @@ def test_work_queued_on_freed_memory_does_not_reach_outputs(name, busy):
         side.synchronize()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", ["route_select", "route_by_rule", "spec_verify", "argmax_f16"])
+def test_a_side_stream_in_a_graph(name):
+    """A call on a stream that branches off a capture and joins it again."""
+    keep, fs = calls()
+    f = fs[name]
+    side = torch.cuda.Stream()
+    want = f(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        got = f(side)
+        main.wait_stream(side)
+    for _ in range(3):
+        for v in got:
+            v.fill_(9)
+        g.replay()
+        again = f(None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, want, again))
