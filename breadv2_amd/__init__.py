@@ -7,6 +7,7 @@ without the built library raises: there is no CPU fallback.
 from ._lib import BreadError, MoeLayer, MoeShape, lib, status_str  # noqa: F401
 from .api import (  # noqa: F401
     Arena,
+    Fp8Experts,
     Gguf,
     LayerTensors,
     MoeContext,
@@ -14,9 +15,12 @@ from .api import (  # noqa: F401
     argmax_f16,
     bread_dequant_rows,
     bread_matmul,
+    bread_matmul_fp8,
+    bread_matmul_fp8_grouped,
     bread_matvec,
     bread_matvec_f32,
     bread_rmsnorm_f32,
+    bread_rmsnorm_fp8,
     layer_seeds,
     route_select,
     row_bytes,

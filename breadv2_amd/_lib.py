@@ -28,6 +28,8 @@ QTYPE_F16 = 1
 QTYPE_Q8_0 = 8
 QTYPE_Q4_K = 12
 QTYPE_Q6_K = 14
+QTYPE_BF16 = 30
+QTYPE_E4M3 = 0x1000
 
 # bread_moe_path_t
 PATH_AUTO = 0
@@ -149,6 +151,75 @@ class VerifyArgs(ctypes.Structure):
     ]
 
 
+class RmsnormFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("residual", c_void_p),
+        ("hidden", c_void_p),
+        ("x_type", c_int),
+        ("x_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("hidden_stride", ctypes.c_int64),
+        ("weight", c_void_p),
+        ("eps", c_float),
+        ("n", c_int),
+        ("n_tokens", c_int),
+        ("codes", c_void_p),
+        ("codes_stride", ctypes.c_int64),
+        ("scales", c_void_p),
+        ("scales_stride", ctypes.c_int64),
+        ("normed", c_void_p),
+        ("normed_type", c_int),
+        ("normed_stride", ctypes.c_int64),
+    ]
+
+
+class MatmulFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("w", c_void_p),
+        ("w_scale", c_void_p),
+        ("up", c_void_p),
+        ("up_scale", c_void_p),
+        ("x", c_void_p),
+        ("x_scale", c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("x_scale_stride", ctypes.c_int64),
+        ("y", c_void_p),
+        ("y_scale", c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("y_scale_stride", ctypes.c_int64),
+        ("y_type", c_int),
+        ("bias", c_void_p),
+        ("residual", c_void_p),
+        ("act", c_int),
+        ("rows", c_int),
+        ("cols", c_int),
+        ("n_tokens", c_int),
+    ]
+
+
+class Fp8Groups(ctypes.Structure):
+    _fields_ = [
+        ("n_groups", c_int),
+        ("offsets", c_void_p),
+        ("x_rows", c_void_p),
+        ("n_x", c_int),
+        ("y_rows", c_void_p),
+        ("n_y", c_int),
+    ]
+
+
+class Fp8ExpertsDesc(ctypes.Structure):
+    _fields_ = [
+        ("gate", c_void_p),
+        ("up", c_void_p),
+        ("down", c_void_p),
+        ("gate_scale", c_void_p),
+        ("up_scale", c_void_p),
+        ("down_scale", c_void_p),
+    ]
+
+
 class GgufTensor(ctypes.Structure):
     _fields_ = [
         ("name", c_char_p),
@@ -171,6 +242,13 @@ SIGNATURES = {
     "bread_matvec_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "bread_matmul": (
         c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "bread_rmsnorm_fp8": (c_int, [c_void_p, c_void_p]),
+    "bread_matmul_fp8": (c_int, [c_void_p, c_void_p]),
+    "bread_matmul_fp8_grouped": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "bread_moe_expert_block_fp8": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p],
+    ),
     "bread_dequant_rows": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "bread_moe_shape_default": (None, [POINTER(MoeShape)]),
     "bread_moe_ctx_create": (c_int, [POINTER(MoeShape), c_int, POINTER(c_void_p)]),

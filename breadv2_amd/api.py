@@ -30,6 +30,8 @@ PATH_GROUPED = _lib.PATH_GROUPED
 PATH_PER_TOKEN = _lib.PATH_PER_TOKEN
 PATH_SMALL = _lib.PATH_SMALL
 QTYPE_F16 = _lib.QTYPE_F16
+QTYPE_BF16 = _lib.QTYPE_BF16
+QTYPE_E4M3 = _lib.QTYPE_E4M3
 
 
 def _p(t: torch.Tensor | None):
@@ -183,6 +185,187 @@ def bread_dequant_rows(w, qtype: int, rows: int, cols: int, out=None, stream=Non
 
 def bread_rmsnorm_f32(x, w, out, n: int, n_tokens: int, eps: float, stream=None) -> None:
     check(lib.bread_rmsnorm_f32(_p(x), _p(w), _p(out), n, n_tokens, eps, _s(stream)), "bread_rmsnorm_f32")
+
+
+# ---------------------------------------------------------------- 8-bit floating point
+
+_F8 = torch.float8_e4m3fn
+_WIDE_TYPES = {torch.float16: _lib.QTYPE_F16, torch.bfloat16: _lib.QTYPE_BF16, torch.float32: _lib.QTYPE_F32}
+
+
+def _codes_of(t: torch.Tensor, name: str, cols: int) -> int:
+    if t.dtype != _F8:
+        raise ValueError(f"{name} must be float8_e4m3fn")
+    return _rows_of(t, name, cols)
+
+
+def _scales_of(t: torch.Tensor, name: str, n: int, cols: int) -> int:
+    """Floats from one token's scales to the next: float32 [n][ceil(cols / 128)]."""
+    if t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] != n:
+        raise ValueError(f"{name} must be float32 with a row a token")
+    return _rows_of(t, name, -(-cols // 128))
+
+
+def _weights_of(w, scale, name: str, shape) -> None:
+    """Dense codes of a shape [..., rows, cols] and their dense scales."""
+    if w.dtype != _F8 or w.shape != shape or not w.is_contiguous():
+        raise ValueError(f"{name} must be dense float8_e4m3fn {list(shape)}")
+    want = (*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128))
+    if scale is None or scale.dtype != torch.float32 or scale.shape != want or not scale.is_contiguous():
+        raise ValueError(f"{name}'s scales must be dense float32 {list(want)}")
+
+
+def bread_rmsnorm_fp8(x, w, codes, scales, eps: float, residual=None, hidden=None, normed=None, stream=None) -> None:
+    """bread_rmsnorm_fp8: h = x + residual and v = h / sqrt(mean(h^2) + eps) * w for the
+    rows of x (float16, bfloat16 or float32 [n_tokens][n], n a multiple of 16);
+    codes float8_e4m3fn [n_tokens][n] and scales float32 [n_tokens][ceil(n / 128)]
+    receive v quantised, hidden (x's type; may be x or residual) h, normed
+    (float16, bfloat16 or float32) v.  w: float32 [n] or None.  Rows may be strided."""
+    kind = x.dtype
+    x_type = _WIDE_TYPES.get(kind)
+    if x_type is None or x.dim() != 2:
+        raise ValueError("x must be float16, bfloat16 or float32 [n_tokens][n]")
+    T, n = x.shape
+    xs, cs, ss = _rows_of(x, "x", n), _codes_of(codes, "codes", n), _scales_of(scales, "scales", T, n)
+    if codes.shape[0] != T:
+        raise ValueError("codes must have a row a token")
+    wp = rp = hp = op = None
+    rs = hs = os = out_type = 0
+    if w is not None:
+        if w.dtype != torch.float32 or w.shape != (n,) or not w.is_contiguous():
+            raise ValueError("w must be float32 [n]")
+        wp = w.data_ptr()
+    if residual is not None:
+        if residual.dtype != kind or residual.shape != x.shape:
+            raise ValueError("residual must have x's type and shape")
+        rs, rp = _rows_of(residual, "residual", n), residual.data_ptr()
+    if hidden is not None:
+        if hidden.dtype != kind or hidden.shape != x.shape:
+            raise ValueError("hidden must have x's type and shape")
+        hs, hp = _rows_of(hidden, "hidden", n), hidden.data_ptr()
+    if normed is not None:
+        out_type = _WIDE_TYPES.get(normed.dtype)
+        if out_type is None or normed.shape != x.shape:
+            raise ValueError("normed must be float16, bfloat16 or float32 of x's shape")
+        os, op = _rows_of(normed, "normed", n), normed.data_ptr()
+    st = _on(stream, (x, w, codes, scales, residual, hidden, normed))
+    rc = lib.bread_rmsnorm_fp8(ctypes.byref(_lib.RmsnormFp8Args(
+        x.data_ptr(), rp, hp, x_type, xs, rs, hs, wp, eps, n, T, codes.data_ptr(), cs, scales.data_ptr(), ss, op,
+        out_type, os)), st)
+    if rc:
+        check(rc, "bread_rmsnorm_fp8")
+
+
+def _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, rows, cols, T, n_y, bp, rp):
+    a = ACTS.get(act)
+    if a is None:
+        raise ValueError(f"unknown activation {act!r}")
+    xs, ss = _codes_of(x, "x", cols), _scales_of(x_scale, "x_scale", x.shape[0], cols)
+    kind = y.dtype
+    ysp, yss = None, 0
+    if kind == _F8:
+        y_type = _lib.QTYPE_E4M3
+        if y_scale is None:
+            raise ValueError("quantised results need y_scale")
+        yss, ysp = _scales_of(y_scale, "y_scale", n_y, rows), y_scale.data_ptr()
+    else:
+        y_type = _WIDE_TYPES.get(kind)
+        if y_type is None:
+            raise ValueError("y must be float16, bfloat16, float32 or float8_e4m3fn")
+        if y_scale is not None:
+            raise ValueError("y_scale is for quantised results")
+    ys = _rows_of(y, "y", rows)
+    if y.shape[0] != n_y:
+        raise ValueError("y has another number of rows than the call writes")
+    upp = usp = None
+    if up is not None:
+        _weights_of(up, up_scale, "up", w.shape)
+        upp, usp = up.data_ptr(), up_scale.data_ptr()
+    return _lib.MatmulFp8Args(w.data_ptr(), w_scale.data_ptr(), upp, usp, x.data_ptr(), x_scale.data_ptr(), xs, ss,
+                              y.data_ptr(), ysp, ys, yss, y_type, bp, rp, a, rows, cols, T)
+
+
+def bread_matmul_fp8(w, w_scale, x, x_scale, y, y_scale=None, up=None, up_scale=None, bias=None, act=None,
+                     residual=None, stream=None) -> None:
+    """bread_matmul_fp8: y[t] = act(W x[t] + bias) + residual[t], or act(W x[t]) *
+    (Up x[t]) + residual[t], for codes w, up float8_e4m3fn [rows][cols] with scales
+    float32 [ceil(rows / 128)][ceil(cols / 128)] and x float8_e4m3fn
+    [n_tokens][cols] with x_scale float32 [n_tokens][ceil(cols / 128)].  y
+    [n_tokens][rows]: float16, bfloat16, float32, or float8_e4m3fn with y_scale
+    float32 [n_tokens][ceil(rows / 128)].  residual (may be y) has y's type, bias
+    is float32 [rows]; rows of x, y and the scales of tokens may be strided."""
+    if w.dim() != 2 or x.dim() != 2 or y.dim() != 2:
+        raise ValueError("w, x and y must be 2-d")
+    rows, cols = w.shape
+    T = x.shape[0]
+    _weights_of(w, w_scale, "w", w.shape)
+    bp = rp = None
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (rows,) or not bias.is_contiguous():
+            raise ValueError("bias must be float32 [rows]")
+        bp = bias.data_ptr()
+    if residual is not None:
+        if (residual.dtype != y.dtype or residual.shape != y.shape
+                or _rows_of(residual, "residual", rows) != _rows_of(y, "y", rows)):
+            raise ValueError("residual must have y's type, shape and stride")
+        rp = residual.data_ptr()
+    a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, rows, cols, T, T, bp, rp)
+    st = _on(stream, (w, w_scale, x, x_scale, y, y_scale, up, up_scale, bias, residual))
+    rc = lib.bread_matmul_fp8(ctypes.byref(a), st)
+    if rc:
+        check(rc, "bread_matmul_fp8")
+
+
+def _rows_index(t, name: str) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be dense int32")
+    return t.shape[0]
+
+
+def bread_matmul_fp8_grouped(w, w_scale, x, x_scale, offsets, y, y_scale=None, up=None, up_scale=None, act=None,
+                             x_rows=None, y_rows=None, stream=None) -> None:
+    """bread_matmul_fp8_grouped: row i of offsets[g] <= i < offsets[g + 1] (int32
+    [n_groups + 1]) is row x_rows[i] of x through matrix g of w [n_groups][rows][cols],
+    written to row y_rows[i] of y (int32, None: i itself); scales and results as
+    bread_matmul_fp8.  There are as many rows i as x_rows, y_rows or else x has."""
+    if w.dim() != 3 or x.dim() != 2 or y.dim() != 2:
+        raise ValueError("w must be 3-d, x and y 2-d")
+    G, rows, cols = w.shape
+    _weights_of(w, w_scale, "w", w.shape)
+    if _rows_index(offsets, "offsets") != G + 1:
+        raise ValueError("offsets must hold n_groups + 1 values")
+    T, xrp, yrp, n_x, n_y = x.shape[0], None, None, 0, 0
+    if x_rows is not None:
+        n_x, T, xrp = T, _rows_index(x_rows, "x_rows"), x_rows.data_ptr()
+    if y_rows is not None:
+        if _rows_index(y_rows, "y_rows") != T:
+            raise ValueError("y_rows must name a row of y for every row")
+        n_y, yrp = y.shape[0], y_rows.data_ptr()
+    a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, rows, cols, T,
+                         T if y_rows is None else n_y, None, None)
+    st = _on(stream, (w, w_scale, x, x_scale, offsets, y, y_scale, up, up_scale, x_rows, y_rows))
+    rc = lib.bread_matmul_fp8_grouped(ctypes.byref(a), ctypes.byref(_lib.Fp8Groups(G, offsets.data_ptr(), xrp, n_x,
+                                                                                   yrp, n_y)), st)
+    if rc:
+        check(rc, "bread_matmul_fp8_grouped")
+
+
+class Fp8Experts:
+    """bread_fp8_experts_t: a layer's routed experts as float8_e4m3fn codes, gate and
+    up [n_experts][inter][hidden], down [n_experts][hidden][inter], each with float32
+    scales [n_experts][ceil(rows / 128)][ceil(cols / 128)].  Holds the tensors."""
+
+    def __init__(self, gate, gate_scale, up, up_scale, down, down_scale):
+        if gate.dim() != 3:
+            raise ValueError("gate must be 3-d")
+        E, I, H = gate.shape
+        _weights_of(gate, gate_scale, "gate", (E, I, H))
+        _weights_of(up, up_scale, "up", (E, I, H))
+        _weights_of(down, down_scale, "down", (E, H, I))
+        self.shape = (E, I, H)
+        self.tensors = (gate, up, down, gate_scale, up_scale, down_scale)
+        self.desc = _lib.Fp8ExpertsDesc(*(t.data_ptr() for t in self.tensors))
+        self.ref = ctypes.byref(self.desc)
 
 
 # ---------------------------------------------------------------- synth
@@ -691,6 +874,35 @@ class MoeContext:
         assert idx.dtype == torch.int32 and w.dtype == torch.float32
         check(lib.bread_moe_expert_block(self._h, ctypes.byref(layer), _p(x), _p(hidden), n_tokens, _p(idx),
                                          _p(w), _s(stream)), "bread_moe_expert_block")
+
+    def expert_block_fp8(self, experts: Fp8Experts, x: torch.Tensor, x_scale: torch.Tensor, hidden: torch.Tensor,
+                         idx: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = None,
+                         stream=None) -> None:
+        """bread_moe_expert_block_fp8: hidden = residual + sum_k w[t][k] * expert_{idx[t][k]}(x_t)
+        with 8-bit experts and the caller's routing (residual None: hidden itself, which the sum
+        is added to).  x float8_e4m3fn [n_tokens][H], x_scale float32 [n_tokens][H / 128], hidden and
+        residual float16, bfloat16 or float32 [n_tokens][H], idx int32 and w float32
+        [n_tokens][K], all dense."""
+        s = self.shape
+        if experts.shape != (s.n_experts, s.expert_inter, s.hidden):
+            raise ValueError("the experts are of another shape than the context")
+        T, H, K = x.shape[0], s.hidden, s.top_k
+        h_type = _WIDE_TYPES.get(hidden.dtype)
+        if h_type is None:
+            raise ValueError("hidden must be float16, bfloat16 or float32")
+        if residual is None:
+            residual = hidden
+        for t, name, kind, cols in ((x, "x", _F8, H), (x_scale, "x_scale", torch.float32, -(-H // 128)),
+                                    (hidden, "hidden", hidden.dtype, H), (residual, "residual", hidden.dtype, H),
+                                    (idx, "idx", torch.int32, K), (w, "w", torch.float32, K)):
+            if t.dtype != kind or t.shape != (T, cols) or not t.is_contiguous():
+                raise ValueError(f"{name} must be dense {kind} [{T}][{cols}]")
+        st = _on(stream, (x, x_scale, hidden, residual, idx, w, *experts.tensors))
+        rc = lib.bread_moe_expert_block_fp8(self._h, experts.ref, x.data_ptr(), x_scale.data_ptr(),
+                                            residual.data_ptr(), hidden.data_ptr(), h_type, T, idx.data_ptr(),
+                                            w.data_ptr(), st)
+        if rc:
+            check(rc, "bread_moe_expert_block_fp8")
 
     def forward_f16(self, layer: MoeLayer, hidden: torch.Tensor, normed: torch.Tensor, n_tokens: int,
                     norm_w=None, want_routing: bool = False, stream=None):

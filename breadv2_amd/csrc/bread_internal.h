@@ -83,6 +83,7 @@ struct bread_grouped_ws {
     int *pos_of = nullptr;                // sorted position of pair (t, k) [max_tokens*K]
     void *tiles = nullptr;                // tiles of the expert GEMMs
     int *n_tiles = nullptr;               // routed tiles, and all with the shared expert's
+    int *offsets = nullptr;               // first sorted pair of each expert of the 8-bit block [E + 1]
     float *eo = nullptr;                  // expert outputs by pair [max_tokens*(K+1)][H]
 };
 

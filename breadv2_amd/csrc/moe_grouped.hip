@@ -1298,6 +1298,7 @@ int bread_grouped_alloc(bread_moe_ctx_t *c)
     if (e == hipSuccess) e = hipMalloc((void **)&g.pos_of, T * K * sizeof(int));
     if (e == hipSuccess) e = hipMalloc(&g.tiles, (size_t)max_tiles(s, c->max_tokens) * sizeof(MtTile));
     if (e == hipSuccess) e = hipMalloc((void **)&g.n_tiles, 2 * sizeof(int));
+    if (e == hipSuccess) e = hipMalloc((void **)&g.offsets, ((size_t)s.n_experts + 1) * sizeof(int));
     if (e == hipSuccess) e = hipMalloc((void **)&g.eo, P * H * sizeof(float));
     return e == hipSuccess ? BREAD_OK : (e == hipErrorOutOfMemory ? BREAD_ERR_NOMEM : BREAD_ERR_HIP);
 }
@@ -1312,6 +1313,7 @@ void bread_grouped_free(bread_moe_ctx_t *c)
     (void)hipFree(g.pos_of);
     (void)hipFree(g.tiles);
     (void)hipFree(g.n_tiles);
+    (void)hipFree(g.offsets);
     (void)hipFree(g.eo);
     g = bread_grouped_ws{};
 }

@@ -41,6 +41,9 @@ typedef struct ihipStream_t *bread_stream_t;
 #define BREAD_QTYPE_Q8_0 8
 #define BREAD_QTYPE_Q4_K 12
 #define BREAD_QTYPE_Q6_K 14
+#define BREAD_QTYPE_BF16 30
+/* e4m3 codes with fp32 scales: no GGML type, an id of this library */
+#define BREAD_QTYPE_E4M3 0x1000
 
 #define BREAD_QK_K            256 /* elements per K-quant superblock */
 #define BREAD_Q4K_BLOCK_BYTES 144 /* d, dmin, 12 B scales, 128 B nibbles (kernels.cu:3-7) */
@@ -134,6 +137,112 @@ typedef struct {
  * overlap. */
 int bread_matmul(const void *w, const uint16_t *x, void *y, int rows, int cols, int qtype, int n_tokens,
                  const bread_matmul_opts_t *opts, bread_stream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* 8-bit floating point                                                */
+/* ------------------------------------------------------------------ */
+
+/* Values held as e4m3 codes (sign, 4 bits of exponent, 3 of mantissa, largest
+ * 448, NaN 0x7F and 0xFF) with fp32 scales: activations a scale for every 128
+ * columns of a token ([n_tokens][ceil(cols / 128)]), weights a scale for every
+ * block of 128 rows by 128 columns ([ceil(rows / 128)][ceil(cols / 128)]);
+ * the value is code * scale.  The last block of a row or matrix may be
+ * smaller.  Quantising a block of a token's columns gives
+ *   scale = max(max|v| / 448, 2^-126),  code = e4m3(v / scale)
+ * to nearest, ties to even; a block with an infinity or a NaN gets a scale of
+ * NaN and codes of NaN, which keeps the token's products NaN.  The reference
+ * has no 8-bit floating point; models whose routing rules
+ * bread_route_select knows are published in it. */
+
+/* RMSNorm with the residual's addition and quantised results:
+ *   h = x + residual (rounded to x's type);  v = h / sqrt(mean(h^2) + eps) * weight
+ *   hidden = h, normed = v (rounded), codes and scales = v quantised
+ * for n_tokens rows of n columns: bread_rmsnorm_f32 for what feeds
+ * bread_matmul_fp8, and unquantised for a router.  n is a multiple of 16 up to
+ * 32768.  Strides in elements, 0: packed.  codes are 16-byte aligned with a
+ * stride that is a multiple of 16, the others aligned to their elements.
+ * hidden may be x or residual itself; nothing else may overlap.  Results
+ * between one row's end and the next row's start are left as they were. */
+typedef struct {
+    const void *x;
+    const void *residual; /* x's type, or NULL */
+    void *hidden;         /* x's type, or NULL */
+    int x_type;           /* BREAD_QTYPE_F32, _F16 or _BF16 */
+    int64_t x_stride, residual_stride, hidden_stride;
+    const float *weight;  /* fp32 [n], or NULL: ones */
+    float eps;
+    int n, n_tokens;
+    uint8_t *codes;       /* [n_tokens][n] */
+    int64_t codes_stride;
+    float *scales;        /* [n_tokens][ceil(n / 128)] */
+    int64_t scales_stride;
+    void *normed;         /* normed_type, or NULL */
+    int normed_type;      /* BREAD_QTYPE_F32, _F16 or _BF16 */
+    int64_t normed_stride;
+} bread_rmsnorm_fp8_t;
+
+int bread_rmsnorm_fp8(const bread_rmsnorm_fp8_t *args, bread_stream_t stream);
+
+/* Several tokens through one matrix, both in 8-bit floating point:
+ *   v[t][r] = sum_b x_scale[t][b] w_scale[r / 128][b] sum_{c in b} x[t][c] w[r][c]
+ *   y[t][r] = act(v[t][r] + bias[r]) + residual[t][r]
+ * or, with a second matrix of the same shape (a gated unit; no bias),
+ *   y[t][r] = act(v[t][r]) * v_up[t][r] + residual[t][r].
+ * The 8-bit form of bread_matmul.  y is fp16, bf16, fp32 or quantised again
+ * (BREAD_QTYPE_E4M3: codes in y and scales in y_scale; rows a multiple of 16,
+ * no residual).  Sums are fp32.  For fp32 and quantised y, and for a few tokens,
+ * products are exact; for fp16 and bf16 y and many tokens they are summed by
+ * the 8-bit matrix instructions, which cut each product of eight neighbours
+ * below 2^-13 of the largest one's leading bit (5e-5 of a sum and less for
+ * ordinary values: under half a step of fp16).
+ * cols is a multiple of 16 up to 2^20, rows up to 2^24, n_tokens up to 2^24.
+ * Strides in elements, 0: packed.  w, up and x are 16-byte aligned with an
+ * x_stride that is a multiple of 16 (and codes in y alike); the others are
+ * aligned to their elements.  y and y_scale overlap no input; residual is y or
+ * does not overlap it.  What lies between one row of y and the next is left as
+ * it was.  A NaN in a token's codes or scales stays in its results, one in the
+ * weights in the rows of its block.  n_tokens or rows 0: nothing is done.  No workspace:
+ * calls on different streams may overlap. */
+typedef struct {
+    const void *w;        /* e4m3 [rows][cols] */
+    const float *w_scale;
+    const void *up;       /* e4m3 [rows][cols], or NULL */
+    const float *up_scale;
+    const void *x;        /* e4m3 [n_tokens][cols] */
+    const float *x_scale;
+    int64_t x_stride, x_scale_stride;
+    void *y;              /* [n_tokens][rows] */
+    float *y_scale;       /* [n_tokens][ceil(rows / 128)], with BREAD_QTYPE_E4M3 */
+    int64_t y_stride, y_scale_stride; /* y_stride: residual's too */
+    int y_type;           /* BREAD_QTYPE_F32, _F16, _BF16 or _E4M3 */
+    const float *bias;    /* fp32 [rows], or NULL */
+    const void *residual; /* y's type, or NULL */
+    int act;              /* BREAD_ACT_* */
+    int rows, cols, n_tokens;
+} bread_matmul_fp8_t;
+
+int bread_matmul_fp8(const bread_matmul_fp8_t *args, bread_stream_t stream);
+
+/* The same by groups of rows, each with weights of its own (the experts of a
+ * layer): row i of offsets[g] <= i < offsets[g + 1] is x row x_rows[i] through
+ * matrix g of w [n_groups][rows][cols] (w_scale, up and up_scale alike, all
+ * packed), written to y row y_rows[i].  n_tokens is the number of rows i.
+ * offsets, x_rows and y_rows are on the device.  offsets ascend from 0 or more
+ * to n_tokens or less (they are held to that range, and a group that ends
+ * before it begins is empty); rows of no group are not computed, and their y
+ * rows are left as they were.  A row whose x_rows entry is outside [0, n_x)
+ * counts as zeros; one whose y_rows entry is outside [0, n_y) is not written.
+ * No y row is named twice.  No bias and no residual.  n_groups up to 1024. */
+typedef struct {
+    int n_groups;
+    const int32_t *offsets; /* [n_groups + 1] */
+    const int32_t *x_rows;  /* [n_tokens], or NULL: i itself */
+    int n_x;                /* rows of x, with x_rows */
+    const int32_t *y_rows;  /* [n_tokens], or NULL: i itself */
+    int n_y;                /* rows of y, with y_rows */
+} bread_fp8_groups_t;
+
+int bread_matmul_fp8_grouped(const bread_matmul_fp8_t *args, const bread_fp8_groups_t *groups, bread_stream_t stream);
 
 /* ------------------------------------------------------------------ */
 /* MoE layer                                                           */
@@ -379,6 +488,30 @@ int bread_moe_forward_by_rule(bread_moe_ctx_t *ctx, const bread_moe_layer_t *lay
 int bread_moe_expert_block(bread_moe_ctx_t *ctx, const bread_moe_layer_t *layer, const float *d_x,
                            float *d_hidden, int n_tokens, const int32_t *d_idx, const float *d_w,
                            bread_stream_t stream);
+
+/* Routed experts in 8-bit floating point, packed: gate and up e4m3
+ * [n_experts][expert_inter][hidden], down [n_experts][hidden][expert_inter],
+ * each with its scales [n_experts][ceil(rows / 128)][ceil(cols / 128)];
+ * 16-byte aligned codes. */
+typedef struct {
+    const void *gate, *up, *down;
+    const float *gate_scale, *up_scale, *down_scale;
+} bread_fp8_experts_t;
+
+/* bread_moe_expert_block with 8-bit experts:
+ *   hidden[t] = residual[t] + sum_k w[t][k] * expert_{idx[t][k]}(x_t)
+ *   expert(x) = down(q(silu(gate x) * (up x)))
+ * in rank order, q the quantising of blocks of 128 columns above.  d_x e4m3
+ * [n_tokens][H] and d_x_scale [n_tokens][H / 128] as bread_rmsnorm_fp8 gives
+ * them (packed, 16-byte aligned), d_residual and d_hidden [n_tokens][H] fp32,
+ * fp16 or bf16 (hidden_type) aligned to 16 bytes; d_residual may be d_hidden, NULL is zeros.
+ * Products are exact and sums fp32; an expert's result is held in fp32 until
+ * the sum is rounded once.  An index outside [0, n_experts) is left out and sets bit 32 of the
+ * error word (bread_moe_ctx_check).  d_idx and d_w as bread_route_select gives
+ * them. */
+int bread_moe_expert_block_fp8(bread_moe_ctx_t *ctx, const bread_fp8_experts_t *experts, const void *d_x,
+                               const float *d_x_scale, const void *d_residual, void *d_hidden, int hidden_type,
+                               int n_tokens, const int32_t *d_idx, const float *d_w, bread_stream_t stream);
 
 /* The MoE block of one_layer_forward on the reference's fp16 residual stream
  * (one_layer.cu:1800-1986, the d_hidden / d_normed2 interface of :1812-1815).
