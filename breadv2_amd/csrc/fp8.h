@@ -82,5 +82,6 @@ struct F8Args {
     int n_x, n_y;
 };
 
-// Launches without checks (fp8_matmul.hip)
+// Launches without checks (fp8_matmul.hip, fp8_grouped.hip)
 int bread_launch_fp8_matmul(const F8Args &a, hipStream_t st);
+int bread_launch_fp8_grouped(const F8Args &a, hipStream_t st);

@@ -113,6 +113,7 @@ extern "C" int bread_moe_expert_block_fp8(bread_moe_ctx_t *c, const bread_fp8_ex
                       (((uintptr_t)x_scale | (uintptr_t)idx | (uintptr_t)w) & 3) == 0,
                   BREAD_ERR_ALIGN, "x, residual and hidden must be 16-byte aligned, the others 4-byte aligned");
     const bread_moe_shape_t &s = c->shape;
+    BREAD_REQUIRE((int64_t)T * s.hidden <= 1ll << 31, BREAD_ERR_SHAPE, "x of more than 2^31 bytes");
     const int H = s.hidden, I = s.expert_inter, K = s.top_k, P = T * K;
     const hipStream_t st = to_hip(stream);
     c->last_stream = st;

@@ -195,8 +195,9 @@ int bread_rmsnorm_fp8(const bread_rmsnorm_fp8_t *args, bread_stream_t stream);
  * the 8-bit matrix instructions, which cut each product of eight neighbours
  * below 2^-13 of the largest one's leading bit (5e-5 of a sum and less for
  * ordinary values: under half a step of fp16).
- * cols is a multiple of 16 up to 2^20, rows up to 2^24, n_tokens up to 2^24.
- * Strides in elements, 0: packed.  w, up and x are 16-byte aligned with an
+ * cols is a multiple of 16 up to 2^20, rows and n_tokens up to 2^24, rows *
+ * n_tokens up to 2^33 and rows * cols up to 2^40.  Strides in elements, 0:
+ * packed; x_stride up to 2^22, x_scale_stride up to 2^20.  w, up and x are 16-byte aligned with an
  * x_stride that is a multiple of 16 (and codes in y alike); the others are
  * aligned to their elements.  y and y_scale overlap no input; residual is y or
  * does not overlap it.  What lies between one row of y and the next is left as
@@ -232,7 +233,9 @@ int bread_matmul_fp8(const bread_matmul_fp8_t *args, bread_stream_t stream);
  * before it begins is empty); rows of no group are not computed, and their y
  * rows are left as they were.  A row whose x_rows entry is outside [0, n_x)
  * counts as zeros; one whose y_rows entry is outside [0, n_y) is not written.
- * No y row is named twice.  No bias and no residual.  n_groups up to 1024. */
+ * No y row is named twice.  No bias and no residual.  n_groups up to 1024,
+ * rows * n_groups up to 2^28; with x_rows, x and its scales hold up to 2^31
+ * bytes each. */
 typedef struct {
     int n_groups;
     const int32_t *offsets; /* [n_groups + 1] */
@@ -503,7 +506,7 @@ typedef struct {
  *   expert(x) = down(q(silu(gate x) * (up x)))
  * in rank order, q the quantising of blocks of 128 columns above.  d_x e4m3
  * [n_tokens][H] and d_x_scale [n_tokens][H / 128] as bread_rmsnorm_fp8 gives
- * them (packed, 16-byte aligned), d_residual and d_hidden [n_tokens][H] fp32,
+ * them (packed, 16-byte aligned, up to 2^31 bytes), d_residual and d_hidden [n_tokens][H] fp32,
  * fp16 or bf16 (hidden_type) aligned to 16 bytes; d_residual may be d_hidden, NULL is zeros.
  * Products are exact and sums fp32; an expert's result is held in fp32 until
  * the sum is rounded once.  An index outside [0, n_experts) is left out and sets bit 32 of the

@@ -58,7 +58,9 @@ BAD = [
     (dict(n_tokens=-1), _lib.ERR_ARG), (dict(act=5), _lib.ERR_ARG), (dict(act=-1), _lib.ERR_ARG),
     (dict(y_type=8), _lib.ERR_QTYPE), (dict(y_type=12), _lib.ERR_QTYPE), (dict(cols=264), _lib.ERR_SHAPE),
     (dict(cols=(1 << 20) + 16), _lib.ERR_SHAPE), (dict(rows=(1 << 24) + 1), _lib.ERR_SHAPE),
-    (dict(n_tokens=(1 << 24) + 1), _lib.ERR_SHAPE), (dict(x_stride=240), _lib.ERR_SHAPE),
+    (dict(n_tokens=(1 << 24) + 1), _lib.ERR_SHAPE), (dict(rows=1 << 20, n_tokens=(1 << 13) + 1), _lib.ERR_SHAPE),
+    (dict(rows=(1 << 20) + 1, cols=1 << 20), _lib.ERR_SHAPE), (dict(x_stride=(1 << 22) + 16), _lib.ERR_SHAPE),
+    (dict(x_scale_stride=(1 << 20) + 1), _lib.ERR_SHAPE), (dict(x_stride=240), _lib.ERR_SHAPE),
     (dict(x_scale_stride=1), _lib.ERR_SHAPE), (dict(y_stride=63), _lib.ERR_SHAPE),
     (dict(y_type=0x1000, y_scale=P, rows=65), _lib.ERR_SHAPE), (dict(y_type=0x1000, y_scale=P, rows=256, y_scale_stride=1), _lib.ERR_SHAPE),
     (dict(y_type=0x1000, y_scale=P, residual=P), _lib.ERR_ARG), (dict(up=P, up_scale=P, bias=P), _lib.ERR_ARG),
@@ -80,7 +82,8 @@ def test_matmul_refuses(kw, want):
 
 @pytest.mark.parametrize("groups,kw,want", [
     (dict(n_groups=-1), {}, _lib.ERR_ARG), (dict(n_groups=1025), {}, _lib.ERR_SHAPE), (dict(offsets=None), {}, _lib.ERR_ARG),
-    (dict(offsets=P + 2), {}, _lib.ERR_ALIGN), (dict(x_rows=P + 2, n_x=2), {}, _lib.ERR_ALIGN),
+    (dict(x_rows=P, n_x=(1 << 23) + 1), {}, _lib.ERR_SHAPE), (dict(x_rows=P, n_x=1 << 23), dict(x_scale_stride=65), _lib.ERR_SHAPE),
+    (dict(n_groups=1024), dict(rows=(1 << 18) + 1), _lib.ERR_SHAPE), (dict(offsets=P + 2), {}, _lib.ERR_ALIGN), (dict(x_rows=P + 2, n_x=2), {}, _lib.ERR_ALIGN),
     (dict(y_rows=P + 1, n_y=2), {}, _lib.ERR_ALIGN), (dict(x_rows=P, n_x=-1), {}, _lib.ERR_ARG),
     (dict(y_rows=P, n_y=-1), {}, _lib.ERR_ARG), ({}, dict(bias=P), _lib.ERR_ARG), ({}, dict(residual=P), _lib.ERR_ARG)])
 def test_groups_refuse(groups, kw, want):
