@@ -14,6 +14,7 @@ another stream that uses them waits for it and records itself on them
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -191,28 +192,25 @@ def bread_rmsnorm_f32(x, w, out, n: int, n_tokens: int, eps: float, stream=None)
 
 _F8 = torch.float8_e4m3fn
 _WIDE_TYPES = {torch.float16: _lib.QTYPE_F16, torch.bfloat16: _lib.QTYPE_BF16, torch.float32: _lib.QTYPE_F32}
+# The argument structs as bytes, field by field (a ctypes structure takes longer to make than a small call runs)
+_NORM_ARGS = struct.Struct("@PPPiqqqPfiiPqPqPiq")
+_MATMUL_ARGS = struct.Struct("@PPPPPPqqPPqqiPPiiii")
+_GROUP_ARGS = struct.Struct("@iPPiPi")
 
 
-def _codes_of(t: torch.Tensor, name: str, cols: int) -> int:
-    if t.dtype != _F8:
-        raise ValueError(f"{name} must be float8_e4m3fn")
-    return _rows_of(t, name, cols)
+def _step(t: torch.Tensor, name: str, kind, n: int, cols: int) -> int:
+    """Elements from one row of an [n][cols] tensor of a type to the next (rows themselves dense)."""
+    if t.dtype != kind or t.shape != (n, cols):
+        raise ValueError(f"{name} must be {kind} [{n}][{cols}], is {t.dtype} {list(t.shape)}")
+    return cols if t.is_contiguous() else _rows_of(t, name, cols)
 
 
-def _scales_of(t: torch.Tensor, name: str, n: int, cols: int) -> int:
-    """Floats from one token's scales to the next: float32 [n][ceil(cols / 128)]."""
-    if t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] != n:
-        raise ValueError(f"{name} must be float32 with a row a token")
-    return _rows_of(t, name, -(-cols // 128))
-
-
-def _weights_of(w, scale, name: str, shape) -> None:
-    """Dense codes of a shape [..., rows, cols] and their dense scales."""
+def _weights_of(w, scale, name: str, shape, scale_shape) -> None:
+    """Dense codes and scales of matrices."""
     if w.dtype != _F8 or w.shape != shape or not w.is_contiguous():
         raise ValueError(f"{name} must be dense float8_e4m3fn {list(shape)}")
-    want = (*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128))
-    if scale is None or scale.dtype != torch.float32 or scale.shape != want or not scale.is_contiguous():
-        raise ValueError(f"{name}'s scales must be dense float32 {list(want)}")
+    if scale is None or scale.dtype != torch.float32 or scale.shape != scale_shape or not scale.is_contiguous():
+        raise ValueError(f"{name}'s scales must be dense float32 {list(scale_shape)}")
 
 
 def bread_rmsnorm_fp8(x, w, codes, scales, eps: float, residual=None, hidden=None, normed=None, stream=None) -> None:
@@ -226,63 +224,58 @@ def bread_rmsnorm_fp8(x, w, codes, scales, eps: float, residual=None, hidden=Non
     if x_type is None or x.dim() != 2:
         raise ValueError("x must be float16, bfloat16 or float32 [n_tokens][n]")
     T, n = x.shape
-    xs, cs, ss = _rows_of(x, "x", n), _codes_of(codes, "codes", n), _scales_of(scales, "scales", T, n)
-    if codes.shape[0] != T:
-        raise ValueError("codes must have a row a token")
-    wp = rp = hp = op = None
-    rs = hs = os = out_type = 0
+    xs = n if x.is_contiguous() else _rows_of(x, "x", n)
+    cs, ss = _step(codes, "codes", _F8, T, n), _step(scales, "scales", torch.float32, T, (n + 127) // 128)
+    wp = rp = hp = op = rs = hs = os = out_type = 0
     if w is not None:
         if w.dtype != torch.float32 or w.shape != (n,) or not w.is_contiguous():
             raise ValueError("w must be float32 [n]")
         wp = w.data_ptr()
     if residual is not None:
-        if residual.dtype != kind or residual.shape != x.shape:
-            raise ValueError("residual must have x's type and shape")
-        rs, rp = _rows_of(residual, "residual", n), residual.data_ptr()
+        rs, rp = _step(residual, "residual", kind, T, n), residual.data_ptr()
     if hidden is not None:
-        if hidden.dtype != kind or hidden.shape != x.shape:
-            raise ValueError("hidden must have x's type and shape")
-        hs, hp = _rows_of(hidden, "hidden", n), hidden.data_ptr()
+        hs, hp = _step(hidden, "hidden", kind, T, n), hidden.data_ptr()
     if normed is not None:
         out_type = _WIDE_TYPES.get(normed.dtype)
-        if out_type is None or normed.shape != x.shape:
-            raise ValueError("normed must be float16, bfloat16 or float32 of x's shape")
-        os, op = _rows_of(normed, "normed", n), normed.data_ptr()
+        if out_type is None:
+            raise ValueError("normed must be float16, bfloat16 or float32")
+        os, op = _step(normed, "normed", normed.dtype, T, n), normed.data_ptr()
     st = _on(stream, (x, w, codes, scales, residual, hidden, normed))
-    rc = lib.bread_rmsnorm_fp8(ctypes.byref(_lib.RmsnormFp8Args(
-        x.data_ptr(), rp, hp, x_type, xs, rs, hs, wp, eps, n, T, codes.data_ptr(), cs, scales.data_ptr(), ss, op,
-        out_type, os)), st)
+    rc = lib.bread_rmsnorm_fp8(_NORM_ARGS.pack(x.data_ptr(), rp, hp, x_type, xs, rs, hs, wp, eps, n, T,
+                                               codes.data_ptr(), cs, scales.data_ptr(), ss, op, out_type, os), st)
     if rc:
         check(rc, "bread_rmsnorm_fp8")
 
 
-def _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, rows, cols, T, n_y, bp, rp):
+def _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, shape, n_x, n_y, T, bp, rp):
+    """bread_matmul_fp8_t of checked tensors; shape: the weights'."""
+    rows, cols = shape[-2:]
+    nb, nr = (cols + 127) // 128, (rows + 127) // 128
     a = ACTS.get(act)
     if a is None:
         raise ValueError(f"unknown activation {act!r}")
-    xs, ss = _codes_of(x, "x", cols), _scales_of(x_scale, "x_scale", x.shape[0], cols)
+    scale_shape = (*shape[:-2], nr, nb)
+    _weights_of(w, w_scale, "w", shape, scale_shape)
+    upp = usp = ysp = yss = 0
+    if up is not None:
+        _weights_of(up, up_scale, "up", shape, scale_shape)
+        upp, usp = up.data_ptr(), up_scale.data_ptr()
+    xs, ss = _step(x, "x", _F8, n_x, cols), _step(x_scale, "x_scale", torch.float32, n_x, nb)
     kind = y.dtype
-    ysp, yss = None, 0
     if kind == _F8:
         y_type = _lib.QTYPE_E4M3
         if y_scale is None:
             raise ValueError("quantised results need y_scale")
-        yss, ysp = _scales_of(y_scale, "y_scale", n_y, rows), y_scale.data_ptr()
+        yss, ysp = _step(y_scale, "y_scale", torch.float32, n_y, nr), y_scale.data_ptr()
     else:
         y_type = _WIDE_TYPES.get(kind)
         if y_type is None:
             raise ValueError("y must be float16, bfloat16, float32 or float8_e4m3fn")
         if y_scale is not None:
             raise ValueError("y_scale is for quantised results")
-    ys = _rows_of(y, "y", rows)
-    if y.shape[0] != n_y:
-        raise ValueError("y has another number of rows than the call writes")
-    upp = usp = None
-    if up is not None:
-        _weights_of(up, up_scale, "up", w.shape)
-        upp, usp = up.data_ptr(), up_scale.data_ptr()
-    return _lib.MatmulFp8Args(w.data_ptr(), w_scale.data_ptr(), upp, usp, x.data_ptr(), x_scale.data_ptr(), xs, ss,
-                              y.data_ptr(), ysp, ys, yss, y_type, bp, rp, a, rows, cols, T)
+    ys = _step(y, "y", kind, n_y, rows)
+    return _MATMUL_ARGS.pack(w.data_ptr(), w_scale.data_ptr(), upp, usp, x.data_ptr(), x_scale.data_ptr(), xs, ss,
+                             y.data_ptr(), ysp, ys, yss, y_type, bp, rp, a, rows, cols, T)
 
 
 def bread_matmul_fp8(w, w_scale, x, x_scale, y, y_scale=None, up=None, up_scale=None, bias=None, act=None,
@@ -294,24 +287,21 @@ def bread_matmul_fp8(w, w_scale, x, x_scale, y, y_scale=None, up=None, up_scale=
     [n_tokens][rows]: float16, bfloat16, float32, or float8_e4m3fn with y_scale
     float32 [n_tokens][ceil(rows / 128)].  residual (may be y) has y's type, bias
     is float32 [rows]; rows of x, y and the scales of tokens may be strided."""
-    if w.dim() != 2 or x.dim() != 2 or y.dim() != 2:
-        raise ValueError("w, x and y must be 2-d")
-    rows, cols = w.shape
+    shape = w.shape
+    if len(shape) != 2 or x.dim() != 2:
+        raise ValueError("w and x must be 2-d")
     T = x.shape[0]
-    _weights_of(w, w_scale, "w", w.shape)
-    bp = rp = None
+    bp = rp = 0
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape != (rows,) or not bias.is_contiguous():
+        if bias.dtype != torch.float32 or bias.shape != shape[:1] or not bias.is_contiguous():
             raise ValueError("bias must be float32 [rows]")
         bp = bias.data_ptr()
     if residual is not None:
-        if (residual.dtype != y.dtype or residual.shape != y.shape
-                or _rows_of(residual, "residual", rows) != _rows_of(y, "y", rows)):
+        if residual.dtype != y.dtype or residual.shape != y.shape or residual.stride() != y.stride():
             raise ValueError("residual must have y's type, shape and stride")
         rp = residual.data_ptr()
-    a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, rows, cols, T, T, bp, rp)
-    st = _on(stream, (w, w_scale, x, x_scale, y, y_scale, up, up_scale, bias, residual))
-    rc = lib.bread_matmul_fp8(ctypes.byref(a), st)
+    a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, shape, T, T, T, bp, rp)
+    rc = lib.bread_matmul_fp8(a, _on(stream, (w, w_scale, x, x_scale, y, y_scale, up, up_scale, bias, residual)))
     if rc:
         check(rc, "bread_matmul_fp8")
 
@@ -328,24 +318,25 @@ def bread_matmul_fp8_grouped(w, w_scale, x, x_scale, offsets, y, y_scale=None, u
     [n_groups + 1]) is row x_rows[i] of x through matrix g of w [n_groups][rows][cols],
     written to row y_rows[i] of y (int32, None: i itself); scales and results as
     bread_matmul_fp8.  There are as many rows i as x_rows, y_rows or else x has."""
-    if w.dim() != 3 or x.dim() != 2 or y.dim() != 2:
+    shape = w.shape
+    if len(shape) != 3 or x.dim() != 2 or y.dim() != 2:
         raise ValueError("w must be 3-d, x and y 2-d")
-    G, rows, cols = w.shape
-    _weights_of(w, w_scale, "w", w.shape)
+    G = shape[0]
     if _rows_index(offsets, "offsets") != G + 1:
         raise ValueError("offsets must hold n_groups + 1 values")
-    T, xrp, yrp, n_x, n_y = x.shape[0], None, None, 0, 0
+    T = n_x = x.shape[0]
+    xrp = yrp = 0
     if x_rows is not None:
-        n_x, T, xrp = T, _rows_index(x_rows, "x_rows"), x_rows.data_ptr()
+        T, xrp = _rows_index(x_rows, "x_rows"), x_rows.data_ptr()
+    n_y = T
     if y_rows is not None:
         if _rows_index(y_rows, "y_rows") != T:
             raise ValueError("y_rows must name a row of y for every row")
         n_y, yrp = y.shape[0], y_rows.data_ptr()
-    a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, rows, cols, T,
-                         T if y_rows is None else n_y, None, None)
-    st = _on(stream, (w, w_scale, x, x_scale, offsets, y, y_scale, up, up_scale, x_rows, y_rows))
-    rc = lib.bread_matmul_fp8_grouped(ctypes.byref(a), ctypes.byref(_lib.Fp8Groups(G, offsets.data_ptr(), xrp, n_x,
-                                                                                   yrp, n_y)), st)
+    a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, shape, n_x, n_y, T, 0, 0)
+    rc = lib.bread_matmul_fp8_grouped(
+        a, _GROUP_ARGS.pack(G, offsets.data_ptr(), xrp, n_x, yrp, n_y),
+        _on(stream, (w, w_scale, x, x_scale, offsets, y, y_scale, up, up_scale, x_rows, y_rows)))
     if rc:
         check(rc, "bread_matmul_fp8_grouped")
 
@@ -359,9 +350,10 @@ class Fp8Experts:
         if gate.dim() != 3:
             raise ValueError("gate must be 3-d")
         E, I, H = gate.shape
-        _weights_of(gate, gate_scale, "gate", (E, I, H))
-        _weights_of(up, up_scale, "up", (E, I, H))
-        _weights_of(down, down_scale, "down", (E, H, I))
+        i, h = -(-I // 128), -(-H // 128)
+        _weights_of(gate, gate_scale, "gate", (E, I, H), (E, i, h))
+        _weights_of(up, up_scale, "up", (E, I, H), (E, i, h))
+        _weights_of(down, down_scale, "down", (E, H, I), (E, h, i))
         self.shape = (E, I, H)
         self.tensors = (gate, up, down, gate_scale, up_scale, down_scale)
         self.desc = _lib.Fp8ExpertsDesc(*(t.data_ptr() for t in self.tensors))

@@ -161,3 +161,13 @@ def test_python_block_refuses():
                dict(w=torch.zeros(3, K).half()), dict(w=torch.zeros(2, 3).t()), dict(experts=B.Fp8Experts(gate[:2], gs[:2], gate[:2], gs[:2], down[:2], ds[:2]))):
         with pytest.raises(ValueError):
             ctx.expert_block_fp8(**{**good, **kw})
+
+
+def test_packed_arguments_are_the_structures():
+    """The bytes that the Python calls pass lie as the C structures of the header do."""
+    for packed, cls in ((api._NORM_ARGS, _lib.RmsnormFp8Args), (api._MATMUL_ARGS, _lib.MatmulFp8Args),
+                        (api._GROUP_ARGS, _lib.Fp8Groups)):
+        values = [i + 1 for i in range(len(cls._fields_))]
+        s = cls.from_buffer_copy(packed.pack(*values).ljust(ctypes.sizeof(cls), b"\0"))
+        assert packed.size <= ctypes.sizeof(cls) and packed.size > getattr(cls, cls._fields_[-1][0]).offset
+        assert [getattr(s, name) for name, _ in cls._fields_] == values
