@@ -4,26 +4,37 @@
 
 namespace {
 
-// Workgroups that fill the card
-constexpr int64_t FILL = 200;
+// Forms by tokens and rows.  us at the sizes named:
+// Largest tiles, 128 x 128, for launches that fill the card (FILL).  4096 tokens, 8192 x 2048: bf16 (8-bit matrix
+// instructions) 87, of 4 x 2 waves with 2 x 4 tiles each 100, with 4 x 4 90; fp32 (exact) 130.  Gated, 4096 x 2048 to
+// e4m3 131 and to bf16 79; a wave's tiles 1 x 4 of each matrix in place of 2 x 4 169 and 111.  1000 tokens, 2048 x 4096 to
+// e4m3, 128 tiles: 40, of 64 tokens 28.
+// To e4m3, where a workgroup needs whole blocks of 128 rows: 16 tokens as long as all workgroups run at a time (CUS), two
+// sets of waves by columns; then 64.  131 tokens, 2048 x 4096: 17 and 26; 512 tokens 31 and 26; 131 gated, 512 x 2048:
+// 13.5 and 24.
+// Else 32 rows, four sets of waves by columns (9 tokens, 8192 x 2048: 5.9; eight sets 7.6), or 64 rows by 64 tokens
+// with two (131 tokens, 2048 x 4096: 13.4; one set 21).
+constexpr int64_t FILL = 200, CUS = 256;
 
 template <bool GLU>
 int launch_dense(const F8Args &a, hipStream_t st)
 {
     const bool q = a.y_type == BREAD_QTYPE_E4M3, exact = q || a.y_type == BREAD_QTYPE_F32;
     auto tiles = [&](int64_t t, int64_t r) { return (a.T + t - 1) / t * ((a.rows + r - 1) / r); };
-    if (GLU ? tiles(64, 128) >= FILL && a.T > 64 : tiles(128, 128) >= FILL && a.T > 64) {
-        if constexpr (GLU) {
-            return exact ? launch<8, 1, 1, 1, 4, 1, true, false, 2, false, false>(a, st)
-                         : launch<8, 1, 1, 1, 4, 1, true, true, 2, false, false>(a, st);
-        } else {
+    if (a.T > 64 && tiles(128, 128) >= FILL) {
+        if constexpr (GLU)
+            return exact ? launch<4, 2, 1, 2, 4, 1, true, false, 2, false, false>(a, st)
+                         : launch<4, 2, 1, 2, 4, 1, true, true, 2, false, false>(a, st);
+        else
             return exact ? launch<2, 2, 1, 4, 4, 1, false, false, 2, false, false>(a, st)
-                         : launch<4, 2, 1, 2, 4, 1, false, true, 4, false, false>(a, st);
-        }
+                         : launch<2, 2, 1, 4, 4, 1, false, true, 2, false, false>(a, st);
     }
     if (q) {
-        if (a.T <= 16) return launch<8, 1, 2, 1, 1, GLU ? 2 : 4, GLU, false, 4, true, false>(a, st);
-        return launch<8, 1, 1, 1, 4, GLU ? 1 : 2, GLU, false, 2, true, false>(a, st);
+        if (tiles(16, 128) <= CUS) return launch<8, 1, 2, 1, 1, GLU ? 2 : 4, GLU, false, 4, true, false>(a, st);
+        if constexpr (GLU)
+            return launch<8, 1, 1, 1, 4, 1, true, false, 2, true, false>(a, st);
+        else
+            return launch<4, 1, 2, 2, 4, 2, false, false, 2, true, false>(a, st);
     }
     if (a.T <= 16) return launch<2, 1, 4, 1, 1, GLU ? 4 : 8, GLU, false, 2, true, false>(a, st);
     return launch<2, 2, 2, 1, 2, GLU ? 2 : 4, GLU, false, 2, true, false>(a, st);

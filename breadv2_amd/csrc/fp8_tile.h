@@ -3,9 +3,9 @@
 // for tokens t and weight rows r, with the epilogue y = act(v + bias) [* v_up] + residual,
 // rounded to fp16, bf16 or fp32, or quantised again by blocks of 128 rows.
 //
-// A block's products are summed by matrix instructions from zero, and the
-// product of the two scales is applied to that sum: one fused multiply-add a
-// block of 128 columns and element of y.
+// A block's products are summed in fp32 by matrix instructions from zero, and
+// the product of the two scales is applied to that sum: one fused multiply-add
+// a block of 128 columns and element of y.
 #pragma once
 
 #include <type_traits>
@@ -22,69 +22,100 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // Bytes that a buffer of activations holds at most, and an offset beyond every buffer
 constexpr uint32_t BEYOND = 1u << 31;
 
-// s_waitcnt vmcnt(0): this wave's direct-to-LDS loads have landed
+// All of this wave's loads have landed (in registers or LDS)
 __device__ __forceinline__ void wait_loads()
 {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), lgkmcnt and expcnt at their maxima
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0); lgkmcnt and expcnt at their maxima
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Sixteen codes as two operands of v_mfma_f32_16x16x32_f16 (exact)
-__device__ __forceinline__ void widen(const uint4 &q, h8 &a, h8 &b)
+// A buffer: its first byte, and the bytes from which on loads give zeros
+typedef uint32_t Buffer __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ Buffer buffer(const void *p, uint32_t bytes)
 {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    h2 p[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        p[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.0f, false);
-        p[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.0f, true);
-    }
-    a = h8{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
-    b = h8{p[4][0], p[4][1], p[5][0], p[5][1], p[6][0], p[6][1], p[7][0], p[7][1]};
+    const uint64_t at = uniform64(reinterpret_cast<uint64_t>(p));
+    return Buffer{(uint32_t)at, (uint32_t)(at >> 32) & 0xffff, (uint32_t)uniform((int)bytes), BUF_WORD3};
 }
 
-// The 128 columns of a row that a lane holds, 32 codes: which of the row's columns they are is free as long as
-// weights and activations agree.
+// Loads to LDS, 4 or 16 bytes a lane, which lie behind one another from `to` on.  (Written out: of the builtin's loads the
+// compiler doesn't see which buffer they fill, and waits for those in flight before any read of LDS.  Nothing but LDS is
+// written.  The five wait states are those between a vector instruction that writes a scalar register and a load that reads
+// it.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0, which nothing else here uses)
+template <int BYTES>
+__device__ __forceinline__ void load_lds(const Buffer &b, uint32_t to, uint32_t off, uint32_t soff)
+{
+    to = (uint32_t)uniform((int)to), soff = (uint32_t)uniform((int)soff);
+    asm("" : "+s"(soff));  // a register, also of a constant
+    const Buffer u{(uint32_t)uniform((int)b[0]), (uint32_t)uniform((int)b[1]), (uint32_t)uniform((int)b[2]),
+                   (uint32_t)uniform((int)b[3])};
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(u), "s"(soff) : "m0", "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(u), "s"(soff) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ uint32_t lds_at(const void *p)
+{
+    return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)p);
+}
+
+// A barrier for what lies in LDS, which leaves loads in flight (__syncthreads waits for them)
+__device__ __forceinline__ void barrier()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt at their maxima
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The 128 columns of a row that a lane holds, 32 codes in eight words: which of the row's columns they are is free as
+// long as weights and activations agree.  PARTS matrix instructions take them.  FAST: the codes themselves.  Else they are
+// widened (exactly) to fp16, two at a time in STEPS steps.
 template <bool FAST> struct Frag;
 
 template <> struct Frag<true> {
+    static constexpr int PARTS = 1, STEPS = 0;
     i32x8 v;
-    __device__ __forceinline__ void set(const uint4 &a, const uint4 &b)
+    __device__ __forceinline__ void begin(const uint4 &a, const uint4 &b)
     {
         v = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    }
+    __device__ __forceinline__ void step(int) {}
+    // z: weight rows 4 (l / 16) + i of lane l in element i, token l % 16
+    static __device__ __forceinline__ f32x4 product(const Frag &w, const Frag &x, int, const f32x4 &z)
+    {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, z, 0, 0, 0, 0, 0, 0);
     }
 };
 
 template <> struct Frag<false> {
-    h8 v[4];
-    __device__ __forceinline__ void set(const uint4 &a, const uint4 &b)
+    static constexpr int PARTS = 4, STEPS = 16;
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    uint32_t q[8];
+    Words v[4];
+    __device__ __forceinline__ void begin(const uint4 &a, const uint4 &b)
     {
-        widen(a, v[0], v[1]);
-        widen(b, v[2], v[3]);
+        q[0] = a.x, q[1] = a.y, q[2] = a.z, q[3] = a.w, q[4] = b.x, q[5] = b.y, q[6] = b.z, q[7] = b.w;
+    }
+    __device__ __forceinline__ void step(int i)
+    {
+        const int w = (int)q[i / 2];
+        v[i / 4][i % 4] = __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                                             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    }
+    static __device__ __forceinline__ f32x4 product(const Frag &w, const Frag &x, int k, const f32x4 &z)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w.v[k]), __builtin_bit_cast(h8, x.v[k]), z, 0, 0, 0);
     }
 };
-
-// z[t] = sums of 128 columns: weight rows 4 (l / 16) + i of lane l in element i, token l % 16 of tile t
-template <int TX>
-__device__ __forceinline__ void products(const Frag<true> &w, const Frag<true> (&x)[TX], f32x4 (&z)[TX])
-{
-#pragma unroll
-    for (int t = 0; t < TX; t++)
-        z[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x[t].v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-}
-
-template <int TX>
-__device__ __forceinline__ void products(const Frag<false> &w, const Frag<false> (&x)[TX], f32x4 (&z)[TX])
-{
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int t = 0; t < TX; t++)
-            z[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], x[t].v[i], i ? z[t] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-}
 
 // ---------------------------------------------------------------------------
 // Epilogue
@@ -136,29 +167,31 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
     }
 }
 
-// act(v + bias) or act(v) * u of rows r .. r + 3
-__device__ __forceinline__ void finish4(const F8Args &a, int r, float (&v)[4])
-{
-    if (a.bias) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) v[k] += a.bias[min(r + k, a.rows - 1)];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = activate(v[k], a.act);
-}
-
 // ---------------------------------------------------------------------------
 // The product
 // ---------------------------------------------------------------------------
-// A workgroup takes tiles of 16 TX NWX tokens by OR weight rows (of one or two matrices) in turn.  Its columns come in
-// stages of KSB blocks of 128, by loads to LDS that are one stage ahead, across the tiles' ends too.  Rows lie 128 bytes
-// apart, the eight pieces of 16 bytes of row r at piece ^ (r % 8), so that a read of a piece of 16 rows covers the banks.
-// NWW x NWX waves have TO row tiles by TX token tiles each; NWK such sets of waves share a stage's blocks and add their
-// sums through LDS.
+// A workgroup takes tiles of 16 TX NWX tokens by OR weight rows (of one or two matrices).  Its columns come in stages of
+// KSB blocks of 128, by loads to LDS that are one stage ahead, across the tiles' ends too where it takes several (KEEP).
+// Rows lie 128 bytes apart, the eight pieces of 16 bytes of row r at piece ^ (r % 8), so that a read of a piece of 16 rows
+// covers the banks.  NWW x NWX waves have TO row tiles by TX token tiles each; NWK such sets of waves share a stage's
+// blocks and add their sums through LDS.
+//
+// FAST, the 8-bit matrix instructions: they cut products more than 2^13 below the largest of their eight, which is
+// 1.5e-5 to 2.3e-5 of a result: a twentieth of fp16's own rounding, a hundred and seventieth of bf16's.  Not for fp32
+// results, nor for e4m3, whose scales are fp32.  Else the codes are widened to fp16 (exact, and their products sum in fp32).
+//
+// What bounds them.  A compute unit's four SIMDs take an fp16 instruction of 16 x 16 x 32 in 16 cycles, and a widening,
+// a scaled addition or any other vector instruction in 4 to 5; the widenings are 16 (N + TX), the additions 4 N TX of
+// 4 N TX matrix instructions, so a wave's tiles want to be many and square: N, TX = 4 is what 256 registers hold.
+// Measured over long columns, 4096 tokens: exact 1.15 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.59.
+// Around it a tile costs 5 to 8 us of first loads and results.  Tried and not kept: three and four stages (no faster: it is
+// not latency), tokens widened once and shared as fp16 through LDS (1.15 too), loads spread over a stage's products
+// (the same), columns that begin elsewhere for each tile (slower by 5 %: weights are shared in step).
 
 // Where a tile lies: weights' group, first row and number of rows (of the call's T), first weight row
 struct Place {
     int g, p0, n, row0;
+    bool large;
 };
 
 template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAST> struct Shape {
@@ -175,30 +208,29 @@ template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAS
     static_assert((KSB * WR) % PASS == 0 && WR % 8 == 0 && BX % 8 == 0 && 16 * TO <= F8_BLOCK, "whole passes");
 };
 
-template <class S> struct Lds {
-    __attribute__((aligned(16))) uint8_t buf[2][S::STAGE];
-    __attribute__((aligned(16))) uint8_t sums[S::SUMS ? S::SUMS : 16];
-    uint32_t mags[S::OR / 16][S::BX];
-};
-
 constexpr int GROUPS_MAX = 1024;
 
-// tiles[g]: token tiles of the groups before g, for g <= G
+// A group's token tiles are large, or one is small: with at most half of a tile's tokens.  A word counts both.
+constexpr int SMALL_BITS = 11;  // (at most one a group, and 2^24 / 16 large ones)
+
+// begin[g]: the groups' first rows, tiles[g]: token tiles of the groups before g, for g <= G
 template <int THREADS>
-__device__ __forceinline__ void count_tiles(const F8Args &a, int bx, int *tiles, int *sums)
+__device__ __forceinline__ void count_tiles(const F8Args &a, int bx, int *begin, uint32_t *tiles, int *sums)
 {
+    for (int g = (int)threadIdx.x; g <= a.G; g += THREADS) begin[g] = min(max(a.offsets[g], 0), a.T);
+    __syncthreads();
     const int per = (a.G + THREADS - 1) / THREADS, g0 = (int)threadIdx.x * per;
     auto of = [&](int g) __attribute__((always_inline)) {
-        const int lo = min(max(a.offsets[g], 0), a.T), hi = min(max(a.offsets[g + 1], 0), a.T);
-        return hi > lo ? (hi - lo + bx - 1) / bx : 0;
+        const int n = max(begin[g + 1] - begin[g], 0), rest = n % bx;
+        return (uint32_t)(n / bx + (2 * rest > bx)) << SMALL_BITS | (uint32_t)(rest && 2 * rest <= bx);
     };
-    int mine = 0;
+    uint32_t mine = 0;
     for (int g = g0; g < min(g0 + per, a.G); g++) mine += of(g);
-    const int incl = wave_scan_incl(mine);
-    if (lane_id() == WAVE - 1) sums[threadIdx.x / WAVE] = incl;
+    const uint32_t incl = (uint32_t)wave_scan_incl((int)mine);
+    if (lane_id() == WAVE - 1) sums[threadIdx.x / WAVE] = (int)incl;
     __syncthreads();
-    int before = incl - mine;
-    for (int i = 0; i < (int)threadIdx.x / WAVE; i++) before += sums[i];
+    uint32_t before = incl - mine;
+    for (int i = 0; i < (int)threadIdx.x / WAVE; i++) before += (uint32_t)sums[i];
     for (int g = g0; g < min(g0 + per, a.G); g++) {
         tiles[g] = before;
         before += of(g);
@@ -207,45 +239,66 @@ __device__ __forceinline__ void count_tiles(const F8Args &a, int bx, int *tiles,
     __syncthreads();
 }
 
+// LDS of a workgroup but for the stages
+template <class S, bool GRP> struct Lds {
+    __attribute__((aligned(16))) uint8_t sums[S::SUMS ? S::SUMS : 16];
+    int begin[GRP ? GROUPS_MAX + 1 : 1], scan[S::WAVES];
+    uint32_t tiles[GRP ? GROUPS_MAX + 1 : 1];
+};
+
 template <class S, int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAST, bool KEEP, bool GRP>
-__device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n_xt, Lds<S> &lds, int *gtiles, int *gsums)
+__device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n_xt, Lds<S, GRP> &lds, uint8_t *buf)
 {
     constexpr int M = S::M, N = S::N, OR = S::OR, BX = S::BX, WR = S::WR, PASS = S::PASS;
     const int tid = (int)threadIdx.x, wv = wave_id(), l = lane_id();
     const int wk = wv / (NWW * NWX), ww = wv % NWW, wx = wv / NWW % NWX;
     const int r = l & 15, g = l >> 4, nb = f8_blocks(a.cols), nrb = f8_blocks(a.rows), steps = (nb + KSB - 1) / KSB;
+    // An XCD has consecutive tiles, whose workgroups then share an L2; of groups, first of the large ones and then of the
+    // small ones, so that workgroups that take tiles in turn have about the same work.
+    const int xcd = (int)blockIdx.x % 8, stride = (int)gridDim.x / 8;
+    int n_small = 0;
     if constexpr (GRP) {
-        count_tiles<S::THREADS>(a, BX, gtiles, gsums);
-        n_xt = uniform(gtiles[a.G]);
+        count_tiles<S::THREADS>(a, BX, lds.begin, lds.tiles, lds.scan);
+        n_xt = uniform((int)(lds.tiles[a.G] >> SMALL_BITS));
+        n_small = uniform((int)(lds.tiles[a.G] & ((1 << SMALL_BITS) - 1)));
     }
-    // consecutive tiles on one XCD, whose workgroups then share an L2
-    const int total = n_xt * n_wt, per = (total + 7) / 8, stride = (int)gridDim.x / 8, xcd = (int)blockIdx.x % 8;
-    const int end = min(per * (xcd + 1), total);
-    int tile = per * xcd + (int)blockIdx.x / 8;
+    const int per = (n_xt * n_wt + 7) / 8, large0 = min(per * xcd, n_xt * n_wt), n_large = min(per, n_xt * n_wt - large0);
+    const int per_s = (n_small * n_wt + 7) / 8, small0 = min(per_s * xcd, n_small * n_wt);
+    const int end = n_large + min(per_s, n_small * n_wt - small0);
+    int tile = (int)blockIdx.x / 8;  // of the XCD's
     if (tile >= end) return;
 
-    auto place = [&](int i, int from) __attribute__((always_inline)) {
+    // where the XCD's tile j lies; before: a place that is not behind it
+    auto place = [&](int j, const Place &before) __attribute__((always_inline)) {
         Place p;
         if constexpr (GRP) {
-            // the last group with tiles[g] <= xt, from one that is not behind it, 64 groups at a time
-            const int xt = i / n_wt;
-            int lo = from;
+            // the last group with no more than xt tiles of the kind before it, 64 groups at a time
+            const bool large = j < n_large;
+            const int i = large ? large0 + j : small0 + j - n_large, xt = i / n_wt;
+            auto of = [&](uint32_t v) __attribute__((always_inline)) {
+                return (int)(large ? v >> SMALL_BITS : v & ((1 << SMALL_BITS) - 1));
+            };
+            int lo = large == before.large ? before.g : 0;
             for (;;) {
                 const int ahead = lo + 1 + l;
-                const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ahead < a.G && gtiles[ahead] <= xt));
+                const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ahead < a.G && of(lds.tiles[ahead]) <= xt));
                 lo += n;
                 if (n < WAVE) break;
             }
-            const int at = min(max(a.offsets[lo], 0), a.T), e = min(max(a.offsets[lo + 1], 0), a.T);
+            const uint32_t t = lds.tiles[lo], t1 = lds.tiles[lo + 1];
+            const int in_group = large ? xt - of(t) : (int)(t1 >> SMALL_BITS) - (int)(t >> SMALL_BITS);
+            p.large = large;
             p.g = lo;
-            p.p0 = uniform(at + (xt - uniform(gtiles[lo])) * BX);
-            p.n = uniform(min(e - p.p0, BX));
+            // (held to the call's rows also where offsets fall)
+            p.p0 = uniform(min(lds.begin[lo] + max(in_group, 0) * BX, a.T));
+            p.n = uniform(max(min(lds.begin[lo + 1] - p.p0, BX), 0));
             p.row0 = (i - xt * n_wt) * OR;
         } else {
             // bands of eight token tiles: the tiles that an XCD works on at a time are a square
-            const int band = i / (8 * n_wt), j = i - band * 8 * n_wt, high = min(8, n_xt - 8 * band), w = j / high;
+            const int i = large0 + j, band = i / (8 * n_wt), k = i - band * 8 * n_wt, high = min(8, n_xt - 8 * band), w = k / high;
+            p.large = true;
             p.g = 0;
-            p.p0 = (8 * band + j - w * high) * BX;
+            p.p0 = (8 * band + k - w * high) * BX;
             p.n = min(a.T - p.p0, BX);
             p.row0 = w * OR;
         }
@@ -256,54 +309,55 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     // Loads give zeros beyond their buffer: for rows that are none, and the columns behind a row's end.
     const int srow = tid / 8, piece = (tid % 8) ^ (srow & 7);
     uint32_t xoff[S::PX], xsoff = BEYOND;
-    __amdgpu_buffer_rsrc_t wb, ub, xb, xsb, wsb, usb;
-    int srb0 = 0;
+    Buffer wb, ub, xb, xsb, wsb, usb;
+    int srb0 = 0, xrow[S::PX], xsrow = -1;
+    // x rows of the tile rows that the thread loads, -1 for none
+    auto look = [&](const Place &p) __attribute__((always_inline)) {
+        auto x_row = [&](int i) __attribute__((always_inline)) {
+            if (i >= p.n) return -1;
+            if (!GRP || !a.x_rows) return i;
+            return a.x_rows[p.p0 + i];
+        };
+#pragma unroll
+        for (int i = 0; i < S::PX; i++) {
+            const int at = i * PASS + srow;
+            xrow[i] = KSB * BX % PASS && at >= KSB * BX ? -1 : x_row(at % BX);
+        }
+        if (wv < S::NXS) xsrow = x_row(wv % S::XSW * WAVE + l);
+    };
     auto aim = [&](const Place &p) __attribute__((always_inline)) {
         const uint32_t bytes = (uint32_t)min(OR, a.rows - p.row0) * (uint32_t)a.cols;
         const size_t first = ((size_t)p.g * a.rows + p.row0) * a.cols, scale = (size_t)p.g * nrb * nb;
         const int64_t xr0 = GRP && a.x_rows ? 0 : p.p0;  // x row that offsets count from
-        wb = rsrc(a.w + first, bytes);
-        ub = rsrc(GLU ? a.up + first : a.w + first, bytes);
-        wsb = rsrc(a.ws + scale, 4u * (uint32_t)nrb * (uint32_t)nb);
-        usb = rsrc(GLU ? a.us + scale : a.ws + scale, 4u * (uint32_t)nrb * (uint32_t)nb);
-        xb = rsrc(a.x + xr0 * a.x_stride, BEYOND);
-        xsb = rsrc(a.xs + xr0 * a.xs_stride, BEYOND);
+        const int n_x = GRP && a.x_rows ? a.n_x : a.T;
+        wb = buffer(a.w + first, bytes);
+        ub = buffer(GLU ? a.up + first : a.w + first, bytes);
+        wsb = buffer(a.ws + scale, 4u * (uint32_t)nrb * (uint32_t)nb);
+        usb = buffer(GLU ? a.us + scale : a.ws + scale, 4u * (uint32_t)nrb * (uint32_t)nb);
+        xb = buffer(a.x + xr0 * a.x_stride, BEYOND);
+        xsb = buffer(a.xs + xr0 * a.xs_stride, BEYOND);
         srb0 = p.row0 / F8_BLOCK;
-        auto x_row = [&](int i) __attribute__((always_inline)) {  // x row of tile row i, -1 for none
-            if (i >= p.n) return -1;
-            if (!GRP || !a.x_rows) return i;
-            const int v = a.x_rows[p.p0 + i];
-            return (unsigned)v < (unsigned)a.n_x ? v : -1;
-        };
 #pragma unroll
-        for (int i = 0; i < S::PX; i++) {
-            const int at = i * PASS + srow, v = KSB * BX % PASS && at >= KSB * BX ? -1 : x_row(at % BX);
-            xoff[i] = v < 0 ? BEYOND : (uint32_t)v * (uint32_t)a.x_stride + 16 * piece;
-        }
-        if (wv < S::NXS) {
-            const int v = x_row(wv % S::XSW * WAVE + l);
-            xsoff = v < 0 ? BEYOND : 4u * (uint32_t)v * (uint32_t)a.xs_stride;
-        }
+        for (int i = 0; i < S::PX; i++)
+            xoff[i] = (unsigned)xrow[i] < (unsigned)n_x ? (uint32_t)xrow[i] * (uint32_t)a.x_stride + 16 * piece : BEYOND;
+        xsoff = (unsigned)xsrow < (unsigned)n_x ? 4u * (uint32_t)xsrow * (uint32_t)a.xs_stride : BEYOND;
     };
     uint32_t woff[S::PW];
 #pragma unroll
     for (int i = 0; i < S::PW; i++) woff[i] = (uint32_t)((i * PASS + srow) % OR) * (uint32_t)a.cols + 16 * piece;
-    auto stage = [&](uint8_t *to, int step) __attribute__((always_inline)) {
-        uint8_t *b = to + wv * 8 * F8_BLOCK;
+    auto stage = [&](uint32_t to, int step) __attribute__((always_inline)) {
+        const uint32_t b = to + wv * 8 * F8_BLOCK;
         const int k0 = step * KSB * F8_BLOCK;
-        // scales first: the next barrier waits for all of a stage's loads
 #pragma unroll
         for (int i = 0; i < (S::NXS + S::WAVES - 1) / S::WAVES; i++) {
             const int j = wv + i * S::WAVES, kb = step * KSB + j / S::XSW;  // (a wave's loads are of the same tokens)
-            if (j < S::NXS)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xsb, to + S::XS_AT + 4 * j * WAVE, 4, kb < nb ? xsoff : BEYOND,
-                                                         kb < nb ? 4 * kb : 0, 0, 0);
+            if (j < S::NXS) load_lds<4>(xsb, to + S::XS_AT + 4 * j * WAVE, kb < nb ? xsoff : BEYOND, kb < nb ? 4 * kb : 0);
         }
         if (wv == S::WAVES - 1) {
             const int kb = step * KSB + l / S::OB, rb = srb0 + l % S::OB;
             const uint32_t off = l < KSB * S::OB && kb < nb && rb < nrb ? 4u * (uint32_t)(rb * nb + kb) : BEYOND;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wsb, to + S::WS_AT, 4, off, 0, 0, 0);
-            if constexpr (GLU) __builtin_amdgcn_raw_ptr_buffer_load_lds(usb, to + S::WS_AT + 4 * WAVE, 4, off, 0, 0, 0);
+            load_lds<4>(wsb, to + S::WS_AT, off, 0);
+            if constexpr (GLU) load_lds<4>(usb, to + S::WS_AT + 4 * WAVE, off, 0);
         }
 #pragma unroll
         for (int i = 0; i < S::PW; i++) {
@@ -311,24 +365,21 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
             const int c = k0 + (PASS > WR ? (i * PASS + srow) / WR : kk) * F8_BLOCK;
             const uint32_t off = c + 16 * piece < a.cols ? woff[i] + (PASS > WR ? c - k0 : 0) : BEYOND;
             const int soff = PASS > WR ? k0 : k0 + kk * F8_BLOCK;
-            if (!GLU || (PASS <= OR ? row < OR : srow % WR < OR))
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, b + i * PASS * F8_BLOCK, 16, off, soff, 0, 0);
+            // (a wave's eight rows are of one matrix)
+            if (!GLU || (PASS <= OR ? row < OR : wv * 8 % WR < OR))
+                load_lds<16>(wb, b + i * PASS * F8_BLOCK, off, soff);
             else
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ub, b + i * PASS * F8_BLOCK, 16, off, soff, 0, 0);
+                load_lds<16>(ub, b + i * PASS * F8_BLOCK, off, soff);
         }
 #pragma unroll
         for (int i = 0; i < S::PX; i++) {
             if (KSB * BX % PASS && i * PASS + wv * 8 >= KSB * BX) break;
             const int c = (i * PASS + srow) / BX * F8_BLOCK;
             const uint32_t off = k0 + c + 16 * piece < a.cols && xoff[i] != BEYOND ? xoff[i] + c : BEYOND;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, b + S::W_BYTES + i * PASS * F8_BLOCK, 16, off, k0, 0, 0);
+            load_lds<16>(xb, b + S::W_BYTES + i * PASS * F8_BLOCK, off, k0);
         }
     };
     // -------------------------------------------------------------- products
-    struct Ops {  // a block's operands as they lie in LDS
-        uint4 x[TX][2], w[N][2];
-        float xs[TX], ws[M];
-    };
     f32x4 acc[N][TX];
     auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -338,51 +389,70 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     };
     const int wr0 = 16 * TO * ww;  // the wave's first row in the tile
     const int at0 = r * F8_BLOCK + 16 * (g ^ (r & 7)), at1 = at0 ^ 64;
-    auto read = [&](Ops &q, const uint8_t *b, int kk) __attribute__((always_inline)) {
+    // Block kk of a stage with the wave's first C token tiles.  Each matrix instruction is followed by vector instructions
+    // that take about its time: the next row tile is widened and the last one's sums are scaled and added meanwhile.  (The
+    // compiler would put them in rows of one kind, and a SIMD's two waves, which a barrier lets go together, both wait.)
+    auto multiply = [&](const uint8_t *__restrict__ b, int kk, auto count) __attribute__((always_inline)) {
+        constexpr int C = decltype(count)::value;
+        using F = Frag<FAST>;
+        auto frag = [&](F &f, const uint8_t *__restrict__ p) __attribute__((always_inline)) {
+            f.begin(*reinterpret_cast<const uint4 *>(p + at0), *reinterpret_cast<const uint4 *>(p + at1));
+        };
+        auto weights = [&](F &f, int i) __attribute__((always_inline)) {
+            frag(f, b + (kk * WR + i / TO * OR + wr0 + 16 * (i % TO)) * F8_BLOCK);
+        };
+        F x[C], w[N];
+        float xs[C], ws[M];
+        weights(w[0], 0);
 #pragma unroll
-        for (int t = 0; t < TX; t++) {
-            const uint8_t *p = b + S::W_BYTES + (kk * BX + 16 * (t * NWX + wx)) * F8_BLOCK;
-            q.x[t][0] = *reinterpret_cast<const uint4 *>(p + at0);
-            q.x[t][1] = *reinterpret_cast<const uint4 *>(p + at1);
-            q.xs[t] = *reinterpret_cast<const float *>(b + S::XS_AT + 4 * (kk * S::XSW * WAVE + 16 * (t * NWX + wx) + r));
-        }
+        for (int t = 0; t < C; t++) frag(x[t], b + S::W_BYTES + (kk * BX + 16 * (t * NWX + wx)) * F8_BLOCK);
+        if constexpr (N > 1) weights(w[1], 1);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint8_t *p = b + (kk * WR + i / TO * OR + wr0 + 16 * (i % TO)) * F8_BLOCK;
-            q.w[i][0] = *reinterpret_cast<const uint4 *>(p + at0);
-            q.w[i][1] = *reinterpret_cast<const uint4 *>(p + at1);
-        }
+        for (int t = 0; t < C; t++)
+            xs[t] = *reinterpret_cast<const float *>(b + S::XS_AT + 4 * (kk * S::XSW * WAVE + 16 * (t * NWX + wx) + r));
 #pragma unroll
         for (int m = 0; m < M; m++)
-            q.ws[m] = *reinterpret_cast<const float *>(b + S::WS_AT + 4 * (m * WAVE + kk * S::OB + wr0 / F8_BLOCK));
-    };
-    // with the wave's first C token tiles; a row tile's sums are added while the next one's are made
-    auto multiply = [&](const Ops &q, auto count) __attribute__((always_inline)) {
-        constexpr int C = decltype(count)::value;
-        Frag<FAST> x[C];
-#pragma unroll
-        for (int t = 0; t < C; t++) x[t].set(q.x[t][0], q.x[t][1]);
+            ws[m] = *reinterpret_cast<const float *>(b + S::WS_AT + 4 * (m * WAVE + kk * S::OB + wr0 / F8_BLOCK));
         f32x4 z[2][C];
-        auto add = [&](int i) __attribute__((always_inline)) {
+        float s = 0.f;
+        auto add = [&](int i, int j) __attribute__((always_inline)) {  // element j of the row tile's 4 C
+            const int t = j / 4, e = j % 4;
+            if (e == 0) s = xs[t] * ws[i / TO];
+            acc[i][t][e] = fmaf(s, z[i & 1][t][e], acc[i][t][e]);
+        };
+        constexpr int ALL = F::PARTS * C;  // matrix instructions of a row tile
+        auto widen = [&](int n) __attribute__((always_inline)) {  // what the n-th of them takes of the tokens
 #pragma unroll
-            for (int t = 0; t < C; t++) {
-                const float s = q.xs[t] * q.ws[i / TO];
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][t][e] = fmaf(s, z[i & 1][t][e], acc[i][t][e]);
-            }
+            for (int j = 0; j < F::STEPS / F::PARTS; j++) x[n % C].step(n / C * F::STEPS / F::PARTS + j);
         };
 #pragma unroll
+        for (int j = 0; j < F::STEPS; j++) w[0].step(j);
+        widen(0);
+#pragma unroll
         for (int i = 0; i < N; i++) {
-            Frag<FAST> w;
-            w.set(q.w[i][0], q.w[i][1]);
-            products(w, x, z[i & 1]);
-            if (i) add(i - 1);
+#pragma unroll
+            for (int n = 0; n < ALL; n++) {
+                const int k = n / C, t = n % C;
+                if (i + 2 < N && n == ALL / 2) weights(w[i + 2], i + 2);
+                z[i & 1][t] = F::product(w[i], x[t], k, k ? z[i & 1][t] : f32x4{0.f, 0.f, 0.f, 0.f});
+                if (i == 0 && n + 1 < ALL) widen(n + 1);
+                if (i + 1 < N) {
+#pragma unroll
+                    for (int j = n * F::STEPS / ALL; j < (n + 1) * F::STEPS / ALL; j++) w[i + 1].step(j);
+                }
+                if (i) {
+#pragma unroll
+                    for (int j = n * 4 * C / ALL; j < (n + 1) * 4 * C / ALL; j++) add(i - 1, j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        add(N - 1);
+#pragma unroll
+        for (int j = 0; j < 4 * C; j++) add(N - 1, j);
     };
 
     // -------------------------------------------------------------- results
-    auto finish = [&](const Place &p) __attribute__((always_inline)) {
+    auto finish = [&](const Place &p, uint8_t *spare) __attribute__((always_inline)) {
         if constexpr (NWK > 1) {
             f32x4 *part = reinterpret_cast<f32x4 *>(lds.sums);
             constexpr int W = NWW * NWX;
@@ -392,7 +462,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
 #pragma unroll
                     for (int t = 0; t < TX; t++) part[(((wv - W) * N + i) * TX + t) * WAVE + l] = acc[i][t];
             }
-            __syncthreads();
+            barrier();
             if (wk == 0) {
 #pragma unroll
                 for (int k = 0; k < NWK - 1; k++)
@@ -409,15 +479,41 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
             const int v = a.y_rows[p.p0 + i];
             return (unsigned)v < (unsigned)a.n_y ? v : -1;
         };
-        auto result = [&](int o, int t, float (&v)[4]) __attribute__((always_inline)) {
+        // act(v + bias) [* v_up] in acc[0 .. TO - 1]; the kind of activation outside of the loops: its code once a value
+        auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = acc[o][t][e];
-            finish4(a, p.row0 + wr0 + 16 * o + 4 * g, v);
-            if constexpr (GLU) {
+            for (int o = 0; o < TO; o++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] *= acc[N - TO + o][t][e];
-            }
+                for (int t = 0; t < TX; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[o][t][e] = f(acc[o][t][e], o, t, e);
         };
+        if (wk == 0) {
+            if (!GLU && a.bias) {
+                float bias[TO][4];
+#pragma unroll
+                for (int o = 0; o < TO; o++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) bias[o][e] = a.bias[min(p.row0 + wr0 + 16 * o + 4 * g + e, a.rows - 1)];
+                each([&](float v, int o, int, int e) __attribute__((always_inline)) { return v + bias[o][e]; });
+            }
+            switch (a.act) {
+            case BREAD_ACT_SILU:
+                each([](float v, int, int, int) __attribute__((always_inline)) { return activate(v, BREAD_ACT_SILU); });
+                break;
+            case BREAD_ACT_GELU:
+                each([](float v, int, int, int) __attribute__((always_inline)) { return activate(v, BREAD_ACT_GELU); });
+                break;
+            case BREAD_ACT_GELU_TANH:
+                each([](float v, int, int, int) __attribute__((always_inline)) { return activate(v, BREAD_ACT_GELU_TANH); });
+                break;
+            case BREAD_ACT_RELU:
+                each([](float v, int, int, int) __attribute__((always_inline)) { return activate(v, BREAD_ACT_RELU); });
+                break;
+            }
+            if constexpr (GLU)
+                each([&](float v, int o, int t, int e) __attribute__((always_inline)) { return v * acc[N - TO + o][t][e]; });
+        }
         const bool quantised = OR % F8_BLOCK == 0 && a.y_type == BREAD_QTYPE_E4M3;
         if (!quantised) {
             if (wk == 0) {
@@ -427,8 +523,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
 #pragma unroll
                     for (int o = 0; o < TO; o++) {
                         const int row = p.row0 + wr0 + 16 * o + 4 * g;
-                        float v[4];
-                        result(o, t, v);
+                        const float v[4] = {acc[o][t][0], acc[o][t][1], acc[o][t][2], acc[o][t][3]};
                         if (yr >= 0 && row < a.rows) put4(a, yr, row, v);
                     }
                 }
@@ -439,32 +534,31 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
                 // a token's largest magnitude in its lanes, then over the waves of the block's rows.  (rows is a
                 // multiple of 16, so a row tile is whole or absent.)
                 constexpr int WPB = F8_BLOCK / (16 * TO);  // waves a block
+                uint32_t(*mags)[BX] = reinterpret_cast<uint32_t(*)[BX]>(spare);
+                static_assert(4 * NWW * BX <= S::STAGE, "fits");
+                barrier();  // all have read the last stage
                 if (wk == 0) {
 #pragma unroll
                     for (int t = 0; t < TX; t++) {
                         uint32_t m = 0;
 #pragma unroll
                         for (int o = 0; o < TO; o++) {
-                            float v[4];
-                            result(o, t, v);
+                            if (p.row0 + wr0 + 16 * o >= a.rows) break;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                acc[o][t][e] = v[e];
-                                if (p.row0 + wr0 + 16 * o < a.rows) m = max(m, f8_mag(v[e]));
-                            }
+                            for (int e = 0; e < 4; e++) m = max(m, f8_mag(acc[o][t][e]));
                         }
                         m = max(m, (uint32_t)__shfl_xor((int)m, 16));
                         m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-                        if (g == 0) lds.mags[ww][16 * (t * NWX + wx) + r] = m;
+                        if (g == 0) mags[ww][16 * (t * NWX + wx) + r] = m;
                     }
                 }
-                __syncthreads();
+                barrier();
                 if (wk == 0) {
 #pragma unroll
                     for (int t = 0; t < TX; t++) {
                         uint32_t m = 0;
 #pragma unroll
-                        for (int i = 0; i < WPB; i++) m = max(m, lds.mags[ww / WPB * WPB + i][16 * (t * NWX + wx) + r]);
+                        for (int i = 0; i < WPB; i++) m = max(m, mags[ww / WPB * WPB + i][16 * (t * NWX + wx) + r]);
                         const float s = f8_scale(m), inv = 1.0f / s;
                         const int yr = y_row(t);
                         if (yr < 0) continue;
@@ -483,49 +577,68 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
         }
     };
 
-    Place now = place(tile, 0), next = now;
+    // Stages of columns are loaded one ahead of the products, over the ends of tiles too; a tile's x rows are looked
+    // up while the one before is loaded.
+    const uint32_t at = lds_at(buf);
+    Place now = place(tile, Place{0, 0, 0, 0, true}), next = now, after = now;
+    int ltile = tile, lstep = 0;  // the next stage to load
+    int b = 0, lb = 0;            // buffers
+    bool begun = false;
+    look(now);
     aim(now);
-    stage(lds.buf[0], 0);
-    clear();
-    int cur = 0;
-    for (;;) {
-        const int active = min(max((now.n - 16 * wx + 16 * NWX - 1) / (16 * NWX), 0), TX);  // token tiles of the wave
-        for (int step = 0; step < steps; step++) {
-            wait_loads();
-            __syncthreads();
-            // Every operand of the stage is read before the next stage's loads are issued: the compiler waits for all
-            // loads to LDS before a read of LDS behind them.
-            Ops q[S::KPW];
-#pragma unroll
-            for (int i = 0; i < S::KPW; i++) read(q[i], lds.buf[cur], wk + i * NWK);
-            __builtin_amdgcn_sched_barrier(0);
-            if (step + 1 < steps) {
-                stage(lds.buf[cur ^ 1], step + 1);
-            } else if (KEEP && tile + stride < end) {
-                next = place(tile + stride, now.g);
-                aim(next);
-                stage(lds.buf[cur ^ 1], 0);
+    if (KEEP && tile + stride < end) {
+        after = place(tile + stride, now);
+        look(after);
+    }
+    auto load = [&]() __attribute__((always_inline)) {
+        if (ltile >= end) return;
+        if (KEEP && lstep == 0 && begun) {
+            next = after;
+            aim(next);
+            if (ltile + stride < end) {
+                after = place(ltile + stride, next);
+                look(after);
             }
+        }
+        begun = true;
+        stage(at + lb * S::STAGE, lstep);
+        lb ^= 1;
+        if (++lstep == steps) {
+            lstep = 0;
+            ltile = KEEP ? ltile + stride : end;
+        }
+    };
+    for (bool first = true; tile < end; tile = KEEP ? tile + stride : end) {
+        clear();
+        int active = 0;  // the wave's token tiles that hold any
+        for (int i = first ? -1 : 0; i < steps; i++) {
+            if (i >= 0) {
+                wait_loads();
+                barrier();
+            }
+            load();
+            if (i < 0) continue;
+            if (i == 0) active = min(max((now.n - 16 * wx + 16 * NWX - 1) / (16 * NWX), 0), TX);
+            const uint8_t *cur = buf + b * S::STAGE;
+            b ^= 1;
 #pragma unroll
-            for (int i = 0; i < S::KPW; i++) {
-                if (KSB > 1 && step * KSB + wk + i * NWK >= nb) break;
+            for (int k = 0; k < S::KPW; k++) {
+                const int kk = wk + k * NWK;
+                if (i * KSB + kk >= nb) break;
                 if (!GRP) {
-                    multiply(q[i], std::integral_constant<int, TX>());
+                    multiply(cur, kk, std::integral_constant<int, TX>());
                 } else if (TX >= 4 && active <= TX / 4) {
-                    if (active) multiply(q[i], std::integral_constant<int, (TX + 3) / 4>());
+                    if (active) multiply(cur, kk, std::integral_constant<int, (TX + 3) / 4>());
                 } else if (TX >= 2 && active <= TX / 2) {
-                    if (active) multiply(q[i], std::integral_constant<int, (TX + 1) / 2>());
+                    if (active) multiply(cur, kk, std::integral_constant<int, (TX + 1) / 2>());
                 } else {
-                    if (active) multiply(q[i], std::integral_constant<int, TX>());
+                    if (active) multiply(cur, kk, std::integral_constant<int, TX>());
                 }
             }
-            cur ^= 1;
         }
-        finish(now);
-        tile += stride;
-        if (!KEEP || tile >= end) break;
+        first = false;
+        finish(now, buf + (b ^ 1) * S::STAGE);  // (nothing is loaded yet to the last stage's buffer)
         now = next;
-        clear();
     }
 }
 
@@ -534,17 +647,17 @@ template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAS
 __global__ __launch_bounds__(NWW * NWX * NWK * WAVE, WPE) void k_f8_matmul(const F8Args a, const int n_wt, const int n_xt)
 {
     using S = Shape<NWW, NWX, NWK, TO, TX, KSB, GLU, FAST>;
-    __shared__ Lds<S> lds;
-    __shared__ int gtiles[GRP ? GROUPS_MAX + 1 : 1], gsums[GRP ? S::WAVES : 1];
-    run_tiles<S, NWW, NWX, NWK, TO, TX, KSB, GLU, FAST, KEEP, GRP>(a, n_wt, n_xt, lds, gtiles, gsums);
+    __shared__ Lds<S, GRP> lds;
+    __shared__ __attribute__((aligned(16))) uint8_t buf[2 * S::STAGE];
+    run_tiles<S, NWW, NWX, NWK, TO, TX, KSB, GLU, FAST, KEEP, GRP>(a, n_wt, n_xt, lds, buf);
 }
 
-// WPE: waves a SIMD, which the registers are held to
+// WPE: waves a SIMD, which the registers are held to; KEEP: workgroups take tiles in turn
 template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAST, int WPE, bool KEEP, bool GRP>
 int launch(const F8Args &a, hipStream_t st)
 {
     using S = Shape<NWW, NWX, NWK, TO, TX, KSB, GLU, FAST>;
-    constexpr int lds = (int)sizeof(Lds<S>) + (GRP ? 4 * (GROUPS_MAX + 1 + S::WAVES) : 8);
+    constexpr int lds = (int)sizeof(Lds<S, GRP>) + 2 * S::STAGE;
     constexpr int by_lds = 160 * 1024 / lds, by_waves = 4 * WPE / S::WAVES, resident = by_lds < by_waves ? by_lds : by_waves;
     static_assert(resident >= 1, "a workgroup fits");
     BREAD_REQUIRE(GLU == (a.up != nullptr) && GRP == (a.G > 0) && (a.y_type != BREAD_QTYPE_E4M3 || S::OR % F8_BLOCK == 0), BREAD_ERR_SHAPE,
@@ -556,7 +669,7 @@ int launch(const F8Args &a, hipStream_t st)
     BREAD_REQUIRE(total <= (KEEP ? 1 << 30 : 1 << 22), BREAD_ERR_SHAPE, "more tiles than a launch counts");
     bread_clear_stale_error();
     hipLaunchKernelGGL((k_f8_matmul<NWW, NWX, NWK, TO, TX, KSB, GLU, FAST, WPE, KEEP, GRP>),
-                       dim3((unsigned)((total < most ? total : most) + 7) / 8 * 8), dim3(S::THREADS), 0, st, a, (int)n_wt,
+                       dim3((unsigned)(total + 14 < most ? total + 14 : most) / 8 * 8), dim3(S::THREADS), 0, st, a, (int)n_wt,
                        (int)n_xt);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
