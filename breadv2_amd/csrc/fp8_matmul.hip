@@ -12,8 +12,9 @@ namespace {
 // To e4m3, where a workgroup needs whole blocks of 128 rows: 16 tokens as long as all workgroups run at a time (CUS), two
 // sets of waves by columns; then 64.  131 tokens, 2048 x 4096: 17 and 26; 512 tokens 31 and 26; 131 gated, 512 x 2048:
 // 13.5 and 24.
-// Else 32 rows, four sets of waves by columns (9 tokens, 8192 x 2048: 5.9; eight sets 7.6), or 64 rows by 64 tokens
-// with two (131 tokens, 2048 x 4096: 13.4; one set 21).
+// Else the smallest tiles whose workgroups all run at a time, sets of waves by columns: 16, 32 or 64 tokens by 32 rows, and
+// 64 by 64 for more.  us, 2048 x 4096: 40 tokens 7.0 9.1 12.3 -; 131: 17.5 16.4 13.4 17.8; 300: -  23 24 17.9.  8192 x
+// 2048: 9 tokens 5.9 - - -; 24: 8.3 6.8 8.3 -; 300: - 43 32 28.
 constexpr int64_t FILL = 200, CUS = 256;
 
 template <bool GLU>
@@ -36,8 +37,10 @@ int launch_dense(const F8Args &a, hipStream_t st)
         else
             return launch<4, 1, 2, 2, 4, 2, false, false, 2, true, false>(a, st);
     }
-    if (a.T <= 16) return launch<2, 1, 4, 1, 1, GLU ? 4 : 8, GLU, false, 2, true, false>(a, st);
-    return launch<2, 2, 2, 1, 2, GLU ? 2 : 4, GLU, false, 2, true, false>(a, st);
+    if (tiles(16, 32) <= CUS) return launch<2, 1, 4, 1, 1, GLU ? 4 : 8, GLU, false, 2, true, false>(a, st);
+    if (tiles(32, 32) <= CUS) return launch<2, 1, 4, 1, 2, 4, GLU, false, 2, true, false>(a, st);
+    if (tiles(64, 32) <= CUS) return launch<2, 2, 2, 1, 2, GLU ? 2 : 4, GLU, false, 2, true, false>(a, st);
+    return launch<2, 2, 2, 2, 2, 2, GLU, false, 2, true, false>(a, st);
 }
 
 }  // namespace
