@@ -139,3 +139,25 @@ def test_every_code_is_reached_and_ties_go_to_even():
     assert torch.equal(got[exact], want[exact])
     if ratio == 0:  # the midpoints are ties
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_codes_are_those_of_exact_numbers(kind):
+    """A block's codes are of h w 448 / max|h w|, where the row's factor is not: each is the nearest one, but where the
+    exact number lies on a tie (to 1e-14 of it, of three roundings of 2^-53)."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(400, 4096, generator=g).to(KINDS[kind])
+    w = 1 + 0.3 * torch.randn(4096, generator=g)
+    codes = torch.empty(400, 4096, dtype=F8, device="cuda")
+    scales = torch.empty(400, 32, device="cuda")
+    B.bread_rmsnorm_fp8(x.cuda(), w.cuda(), codes, scales, 1e-6)
+    u = (x.double() * w.double()).view(400, 32, 128)
+    ratio = (u * (448.0 / u.abs().amax(2, keepdim=True))).view(400, 4096)
+    values = R.decode(torch.arange(127, dtype=torch.uint8).view(F8)).double()
+    middle = (values[1:] + values[:-1]) / 2
+    at = torch.searchsorted(middle, ratio.abs())
+    near = middle[torch.clamp(torch.stack([at - 1, at]), 0, 125)]
+    tie = ((near - ratio.abs()).abs() <= 1e-14 * near).any(0)
+    got = R.decode(codes.cpu()).double()
+    assert tie.sum() < 1000
+    assert torch.equal(got[~tie], (values[at] * ratio.sign())[~tie])
