@@ -183,10 +183,13 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
 // What bounds them.  A compute unit's four SIMDs take an fp16 instruction of 16 x 16 x 32 in 16 cycles, and a widening,
 // a scaled addition or any other vector instruction in 4 to 5; the widenings are 16 (N + TX), the additions 4 N TX of
 // 4 N TX matrix instructions, so a wave's tiles want to be many and square: N, TX = 4 is what 256 registers hold.
-// Measured over long columns, 4096 tokens: exact 1.15 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.59.
-// Around it a tile costs 5 to 8 us of first loads and results.  Tried and not kept: three and four stages (no faster: it is
-// not latency), tokens widened once and shared as fp16 through LDS (1.15 too), loads spread over a stage's products
-// (the same), columns that begin elsewhere for each tile (slower by 5 %: weights are shared in step).
+// Measured over long columns, 4096 tokens: exact 1.2 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.85.
+// Of an exact stage's 1.78 us (128 x 128 x 128 twice on a compute unit) the matrix instructions alone take 0.94, with the
+// reads of LDS 1.23, with widening and scaling 1.37, and the loads to LDS add 0.42.  Around its stages a tile costs 5 to
+// 8 us of first loads and results.
+// Tried and not kept: three stages (no faster: it is not latency), tokens widened once and shared as fp16 through LDS (the
+// same), the loads spread over a stage's products (slower by 6 to 17 %), columns that begin elsewhere for each tile (5 %:
+// weights are shared in step), a wave's token tiles one after the other, for wider tiles (15 %).
 
 // Where a tile lies: weights' group, first row and number of rows (of the call's T), first weight row
 struct Place {
