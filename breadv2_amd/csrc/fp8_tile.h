@@ -262,8 +262,10 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     int n_small = 0;
     if constexpr (GRP) {
         count_tiles<S::THREADS>(a, BX, lds.begin, lds.tiles, lds.scan);
-        n_xt = uniform((int)(lds.tiles[a.G] >> SMALL_BITS));
-        n_small = uniform((int)(lds.tiles[a.G] & ((1 << SMALL_BITS) - 1)));
+        // (n_xt: no more tiles than offsets that ascend can give; others are held to it)
+        const int large = min(uniform((int)(lds.tiles[a.G] >> SMALL_BITS)), n_xt);
+        n_small = min(uniform((int)(lds.tiles[a.G] & ((1 << SMALL_BITS) - 1))), n_xt - large);
+        n_xt = large;
     }
     const int per = (n_xt * n_wt + 7) / 8, large0 = min(per * xcd, n_xt * n_wt), n_large = min(per, n_xt * n_wt - large0);
     const int per_s = (n_small * n_wt + 7) / 8, small0 = min(per_s * xcd, n_small * n_wt);

@@ -98,6 +98,13 @@ def test_routing(T, route):
     block(T, 9, 256, 256, 4, torch.float32, route, seed=T)
 
 
+@pytest.mark.parametrize("T", [1, 4])
+@pytest.mark.parametrize("E,K,I,H", [(5, 3, 1024, 512), (33, 32, 256, 256), (12, 9, 512, 768)])
+def test_a_few_tokens(T, E, K, I, H):
+    """Lanes a pair by the inner size, and more pairs than go at a time."""
+    block(T, E, I, H, K, torch.float16, seed=T + K)
+
+
 def test_at_the_decode_shape():
     block(1, 16, 512, 2048, 8, torch.float16, seed=1)
     block(9, 16, 512, 2048, 8, torch.float32, seed=2)

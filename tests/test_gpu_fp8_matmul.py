@@ -87,6 +87,18 @@ def test_many_tokens(T, rows, cols, y):
     dense(T, rows, cols, y=y, seed=T)
 
 
+@pytest.mark.parametrize("y,glu", [("f32", False), ("bf16", False), ("e4m3", False), ("f32", True), ("f16", True), ("e4m3", True)])
+def test_the_largest_tiles(y, glu):
+    dense(1300, 2600 if y != "e4m3" else 2608, 272, y, "silu" if glu else None, glu, pad=1, seed=31)
+
+
+@pytest.mark.parametrize("T,rows", [(24, 8200), (40, 4112), (130, 1504), (300, 2064), (700, 800)])
+@pytest.mark.parametrize("y,glu", [("f32", False), ("e4m3", False), ("bf16", True), ("e4m3", True)])
+def test_tiles_between(T, rows, y, glu):
+    """More tiles than run at a time, or just as many, of each size."""
+    dense(T, rows if y != "e4m3" else rows // 16 * 16, 400, y, None, glu, seed=T)
+
+
 def test_residual_in_place():
     g = gen(5)
     x, xs = R.random_activations(9, 256, g)
@@ -197,6 +209,62 @@ def test_groups_of_many_rows(y):
 def test_groups_at_the_expert_shape():
     grouped(12, 40, 512, 2048, y="e4m3", glu=True, index="gather", seed=12)
     grouped(12, 40, 2048, 512, y="f32", index="scatter", seed=13)
+
+
+@pytest.mark.parametrize("y,glu", [("f32", False), ("e4m3", True), ("bf16", True), ("f16", False)])
+@pytest.mark.parametrize("n", [700, 2100, 9000])
+def test_groups_of_more_tiles_than_run_at_a_time(n, y, glu):
+    """Workgroups that take several tiles, full ones and rests of every size, over groups of 0 to some hundred rows."""
+    grouped(70, n, 528, 272, y=y, glu=glu, index="gather", spare=2, first=1, seed=n)
+
+
+def test_offsets_that_fall():
+    """Groups that overlap, end before they begin or leave the rows: nothing behind the rows is written, and groups in
+    order before them are right."""
+    g = gen(21)
+    n, rows, cols, G = 300, 144, 128, 200
+    x, xs = R.random_activations(n, cols, g)
+    w, ws = R.random_weights(rows, cols, g, groups=G)
+    off = torch.randint(-2**31, 2**31 - 1, (G + 1,), generator=g)
+    off[2::3] = torch.randint(0, n, off[2::3].shape, generator=g)
+    for up in (None, w.cuda()):
+        for y_type in (torch.float32, torch.bfloat16, F8):
+            y = torch.full((n + 64, rows), 3.0, device="cuda").to(y_type)
+            s = torch.full((n + 64, 2), 3.0, device="cuda") if y_type == F8 else None
+            B.bread_matmul_fp8_grouped(w.cuda(), ws.cuda(), x.cuda(), xs.cuda(), off.int().cuda(), y[:n],
+                                       y_scale=None if s is None else s[:n], up=up, up_scale=None if up is None else ws.cuda())
+            torch.cuda.synchronize()
+            assert (y[n:].float() == 3.0).all() and (s is None or (s[n:] == 3.0).all())
+
+
+def test_products_on_two_streams_at_once():
+    """Calls keep no workspace: products that overlap give what they give alone."""
+    g = gen(22)
+    x, xs = (t.cuda() for t in R.random_activations(600, 512, g))
+    w, ws = (t.cuda() for t in R.random_weights(1024, 512, g, groups=8))
+    off = torch.tensor([0, 50, 50, 130, 300, 301, 420, 600, 600], dtype=torch.int32, device="cuda")
+    one, two = [torch.empty(600, 1024, device="cuda") for _ in range(2)]
+    codes, scale = torch.empty(600, 1024, dtype=F8, device="cuda"), torch.empty(600, 8, device="cuda")
+
+    def dense_call():
+        B.bread_matmul_fp8(w[0], ws[0], x, xs, codes, y_scale=scale, up=w[1], up_scale=ws[1], act="silu")
+
+    B.bread_matmul_fp8_grouped(w, ws, x, xs, off, one)
+    dense_call()
+    torch.cuda.synchronize()
+    alone = one.clone(), codes.view(torch.uint8).clone(), scale.clone()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        one.fill_(0), two.fill_(0), scale.fill_(0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            B.bread_matmul_fp8_grouped(w, ws, x, xs, off, one)
+            B.bread_matmul_fp8_grouped(w, ws, x, xs, off, two)
+        with torch.cuda.stream(b):
+            dense_call()
+        torch.cuda.synchronize()
+        assert torch.equal(one, alone[0]) and torch.equal(two, alone[0])
+        assert torch.equal(codes.view(torch.uint8), alone[1]) and torch.equal(scale, alone[2])
 
 
 @pytest.mark.parametrize("n", [3, 200])
