@@ -183,7 +183,7 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
 // What bounds them.  A compute unit's four SIMDs take an fp16 instruction of 16 x 16 x 32 in 16 cycles, and a widening,
 // a scaled addition or any other vector instruction in 4 to 5; the widenings are 16 (N + TX), the additions 4 N TX of
 // 4 N TX matrix instructions, so a wave's tiles want to be many and square: N, TX = 4 is what 256 registers hold.
-// Measured over long columns, 4096 tokens: exact 1.2 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.85.
+// Measured over long columns, 4096 tokens: exact 1.25 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.85.
 // Of an exact stage's 1.78 us (128 x 128 x 128 twice on a compute unit) the matrix instructions alone take 0.94, with the
 // reads of LDS 1.23, with widening and scaling 1.37, and the loads to LDS add 0.42.  Around its stages a tile costs 5 to
 // 8 us of first loads and results.
@@ -433,6 +433,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
 #pragma unroll
         for (int j = 0; j < F::STEPS; j++) w[0].step(j);
         widen(0);
+        if (!GRP) __builtin_amdgcn_s_setprio(1);  // ahead of the other wave's loads: 2 to 5 % (of groups none)
 #pragma unroll
         for (int i = 0; i < N; i++) {
 #pragma unroll
@@ -454,6 +455,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
         }
 #pragma unroll
         for (int j = 0; j < 4 * C; j++) add(N - 1, j);
+        if (!GRP) __builtin_amdgcn_s_setprio(0);
     };
 
     // -------------------------------------------------------------- results
