@@ -1,28 +1,40 @@
 // fp8_matmul.hip — bread_matmul_fp8 and bread_matmul_fp8_grouped: arguments,
 // and the forms of fp8_tile.h's kernel for one matrix.  (Groups: fp8_grouped.hip.)
+#include <algorithm>
+
 #include "fp8_tile.h"
 
 namespace {
 
-// Forms by tokens and rows.  us at the sizes named:
-// Largest tiles, 128 x 128, for launches that fill the card (FILL).  4096 tokens, 8192 x 2048: bf16 (8-bit matrix
-// instructions) 87, of 4 x 2 waves with 2 x 4 tiles each 100, with 4 x 4 90; fp32 (exact) 130.  Gated, 4096 x 2048 to
-// e4m3 131 and to bf16 79; a wave's tiles 1 x 4 of each matrix in place of 2 x 4 169 and 111.  1000 tokens, 2048 x 4096 to
-// e4m3, 128 tiles: 40, of 64 tokens 28.
-// To e4m3, where a workgroup needs whole blocks of 128 rows: 16 tokens as long as all workgroups run at a time (CUS), two
-// sets of waves by columns; then 64.  131 tokens, 2048 x 4096: 17 and 26; 512 tokens 31 and 26; 131 gated, 512 x 2048:
-// 13.5 and 24.
-// Else the smallest tiles whose workgroups all run at a time, sets of waves by columns: 16, 32 or 64 tokens by 32 rows, and
-// 64 by 64 for more.  us, 2048 x 4096: 40 tokens 7.0 9.1 12.3 -; 131: 17.5 16.4 13.4 17.8; 300: -  23 24 17.9.  8192 x
-// 2048: 9 tokens 5.9 - - -; 24: 8.3 6.8 8.3 -; 300: - 43 32 28.
-constexpr int64_t FILL = 200, CUS = 256;
+// Compute units
+constexpr int64_t CUS = 256;
 
+// The tiles are those that give a compute unit the fewest rows of weights and tokens to load, over all its tiles: a unit
+// has about 40 KB of loads under way, which is 40 KB a microsecond, and that is what all but the largest calls wait for.
+// us and rows of a unit for tiles of 16, 32, 48, 64 tokens by 32 rows, 64 by 64 and 128 by 128 (bf16 results):
+//   24 tokens, 2048 x 4096    7.2 (48)   9.3 (64)  11.1 (80)  12.2 (96)  17.4 (128)  24.7 (256)
+//   40, 8192 x 2048          11.7 (144) 11.6 (128)  8.5 (80)   8.9 (96)  11.3 (128)  15.5 (256)
+//   131, 2048 x 4096         17.2 (144) 16.7 (128) 11.6 (80)  12.8 (96)  17.5 (128)  26.1 (256)
+//   500, 2048 x 4096         39.9 (384) 30.8 (256) 29.5 (240) 23.5 (192) 18.4 (128)  26.8 (256)
+//   700, 4096 x 2048         64.5       48.1       45.4       37.9       28.7 (384)  17.5 (256)
+// and 16, 32 and 128 tokens by 128 rows, to e4m3, where a workgroup needs whole blocks:
+//   131, 2048 x 4096         17.1 (144) 21.4 (160) 39.3 (256);    500: 30.6 (288) 22.5 (160) 39.5 (256)
+//   700, 4096 x 2048         49.1 (864) 35.5 (480) 24.6 (256)
+// (gated alike; of 44 measured calls the rule took the fastest form each time).  Small tiles have two to four sets of waves
+// by columns: 9 tokens, 8192 x 2048 5.9 with four, 7.6 with eight.  The largest, 4096 tokens, 8192 x 2048 to bf16: 87; of
+// 4 x 2 waves with 2 x 4 tiles each 100, with 4 x 4 90.  Gated, 4096 x 2048 to e4m3 131 and to bf16 79; a wave's tiles 1 x 4
+// of each matrix in place of 2 x 4 169 and 111.
 template <bool GLU>
 int launch_dense(const F8Args &a, hipStream_t st)
 {
     const bool q = a.y_type == BREAD_QTYPE_E4M3, exact = q || a.y_type == BREAD_QTYPE_F32;
-    auto tiles = [&](int64_t t, int64_t r) { return (a.T + t - 1) / t * ((a.rows + r - 1) / r); };
-    if (a.T > 64 && tiles(128, 128) >= FILL) {
+    auto load = [&](int64_t t, int64_t r) {
+        const int64_t tiles = (a.T + t - 1) / t * ((a.rows + r - 1) / r);
+        return (tiles + CUS - 1) / CUS * (t + (GLU ? 2 : 1) * r);
+    };
+    const int64_t least = q ? std::min(load(16, 128), load(32, 128))
+                            : std::min({load(16, 32), load(32, 32), load(48, 32), load(64, 32), load(64, 64)});
+    if (load(128, 128) <= least) {
         if constexpr (GLU)
             return exact ? launch<4, 2, 1, 2, 4, 1, true, false, 2, false, false>(a, st)
                          : launch<4, 2, 1, 2, 4, 1, true, true, 2, false, false>(a, st);
@@ -31,15 +43,16 @@ int launch_dense(const F8Args &a, hipStream_t st)
                          : launch<2, 2, 1, 4, 4, 1, false, true, 2, false, false>(a, st);
     }
     if (q) {
-        if (tiles(16, 128) <= CUS) return launch<8, 1, 2, 1, 1, GLU ? 2 : 4, GLU, false, 4, true, false>(a, st);
+        if (load(16, 128) == least) return launch<8, 1, 2, 1, 1, GLU ? 2 : 4, GLU, false, 4, true, false>(a, st);
         if constexpr (GLU)
-            return launch<8, 1, 1, 1, 4, 1, true, false, 2, true, false>(a, st);
+            return launch<8, 1, 1, 1, 2, 1, true, false, 2, true, false>(a, st);
         else
-            return launch<4, 1, 2, 2, 4, 2, false, false, 2, true, false>(a, st);
+            return launch<8, 1, 2, 1, 2, 2, false, false, 4, true, false>(a, st);
     }
-    if (tiles(16, 32) <= CUS) return launch<2, 1, 4, 1, 1, GLU ? 4 : 8, GLU, false, 2, true, false>(a, st);
-    if (tiles(32, 32) <= CUS) return launch<2, 1, 4, 1, 2, 4, GLU, false, 2, true, false>(a, st);
-    if (tiles(64, 32) <= CUS) return launch<2, 2, 2, 1, 2, GLU ? 2 : 4, GLU, false, 2, true, false>(a, st);
+    if (load(16, 32) == least) return launch<2, 1, 4, 1, 1, GLU ? 4 : 8, GLU, false, 2, true, false>(a, st);
+    if (load(32, 32) == least) return launch<2, 1, 4, 1, 2, 4, GLU, false, 2, true, false>(a, st);
+    if (load(48, 32) == least) return launch<2, 1, 4, 1, 3, 4, GLU, false, 2, true, false>(a, st);
+    if (load(64, 32) == least) return launch<2, 2, 2, 1, 2, GLU ? 2 : 4, GLU, false, 2, true, false>(a, st);
     return launch<2, 2, 2, 2, 2, 2, GLU, false, 2, true, false>(a, st);
 }
 

@@ -92,7 +92,7 @@ def test_the_largest_tiles(y, glu):
     dense(1300, 2600 if y != "e4m3" else 2608, 272, y, "silu" if glu else None, glu, pad=1, seed=31)
 
 
-@pytest.mark.parametrize("T,rows", [(24, 8200), (40, 4112), (130, 1504), (300, 2064), (700, 800)])
+@pytest.mark.parametrize("T,rows", [(24, 8200), (40, 4112), (100, 4080), (130, 1504), (131, 2064), (300, 2064), (700, 800)])
 @pytest.mark.parametrize("y,glu", [("f32", False), ("e4m3", False), ("bf16", True), ("e4m3", True)])
 def test_tiles_between(T, rows, y, glu):
     """More tiles than run at a time, or just as many, of each size."""
