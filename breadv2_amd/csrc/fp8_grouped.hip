@@ -1,32 +1,59 @@
 // fp8_grouped.hip — the forms of fp8_tile.h's kernel for groups of rows.
+#include <stdint.h>
+
+#include <algorithm>
+
 #include "fp8_tile.h"
 
 namespace {
 
-// By the rows of a group, on average.  us of 256 groups, of tiles of 16, 32, 64 and 128 tokens by 128 rows:
-//   gated, 512 x 2048, to e4m3         8 rows 113 119 -   123;  16: 134 123 129 137;  32: 188 147 135 146;
-//                                      64: -  225 164 177;  128: -   -   262 233
-//   2048 x 512, to fp32                8 rows 68  66  -   81;   16: 78  75  -   88;   32: 112 94  -   94;
-//                                      64: -  144 -   116;  128: -   -   190 169
-// (The weights alone take 103 and 52 at the copy rate.)  Small tiles hold fewer rows that are none, large ones are
-// widened less often a product.  Workgroups that take tiles in turn load the next one's first columns under the last
-// one's results; the largest tiles leave no registers for it.  fp16 and bf16 results of the largest tiles use the 8-bit
-// matrix instructions (fp8_tile.h): 181 of 252 at 128 gated rows.
+// The tiles are those that give a compute unit the fewest rows of weights and tokens to load, as for one matrix
+// (fp8_matmul.hip), of about so many token tiles: half a tile more a group than the rows fill, and no fewer than groups.
+// us and rows of a unit for tiles of 16, 32, 64 tokens by 32 rows, 64 by 64, 32 by 128 and 128 by 128, to fp32:
+//   10 groups, 203 rows, 256 x 2048       6.8 (48)   7.9 (64)   9.2 (96)  11.7 (128)  15.2 (160)  20.2 (256)
+//   8, 540, 512 x 2048                   13.2 (144) 12.0 (128) 10.1 (96)  12.3 (128)  14.9 (160)  25.4 (256)
+//   54, 3452, 192 x 2048                 24.6 (288) 22.3 (256) 18.0 (192) 13.6 (128)  18.5 (320)  25.9 (256)
+//   12, 5022, 256 x 2048                 41.1       31.2       24.5       22.2 (256)  19.4 (320)  26.4 (256)
+//   256, 4096, 512 x 2048                89.1       84.2       98.5       76.3        45.9 (640)  55.3 (1024)
+//   256, 16384, 2048 x 512                                                            144         116
+//   256, 32768, 2048 x 512                                                            190         169
+// and 16, 64 and 128 tokens by 128 rows, gated, to e4m3:
+//   10, 203, 256 x 2048                  15.8 (272) 23.4 (320) 28.0 (384)
+//   12, 5022, 256 x 2048                 40.3 (816) 29.6 (320) 38.1 (384)
+//   29, 4936, 512 x 2048                 76.9       54.6 (640) 39.2 (384)
+//   256, 4096, 512 x 2048                134        111        121;      256, 32768: -  262  233
+// Tiles of 32 by 128 are small enough for two workgroups a unit, which over several rounds take three quarters of the time.
+// Workgroups that take tiles in turn load the next one's first columns under the last one's results; the largest tiles
+// leave no registers for it.  fp16 and bf16 results of the largest tiles use the 8-bit matrix instructions (fp8_tile.h):
+// gated, 256 groups, 32768 rows, 512 x 2048: 181 of 233.
 template <bool GLU>
 int launch_groups(const F8Args &a, hipStream_t st)
 {
-    const bool exact = a.y_type == BREAD_QTYPE_E4M3 || a.y_type == BREAD_QTYPE_F32;
-    const int64_t rows = a.T / a.G;
+    const bool q = a.y_type == BREAD_QTYPE_E4M3, exact = q || a.y_type == BREAD_QTYPE_F32;
+    const int64_t groups = std::min(a.G, a.T);
+    auto load = [&](int64_t t, int64_t r) {
+        const int64_t tiles = std::max(groups, (2 * a.T / t + groups + 1) / 2) * ((a.rows + r - 1) / r);
+        const int64_t rows = t + (GLU ? 2 : 1) * r, all = (tiles + CUS - 1) / CUS * rows;
+        return t == 32 && r == 128 ? std::max(rows, 3 * all / 4) : all;
+    };
+    const int64_t wide = q ? INT64_MAX : std::min({load(16, 32), load(32, 32), load(64, 32), load(64, 64)});
+    const int64_t least = std::min({wide, load(128, 128), GLU ? load(64, 128) : load(32, 128), q ? load(16, 128) : INT64_MAX});
     if constexpr (GLU) {
-        if (rows <= 12) return launch<8, 1, 1, 1, 1, 2, true, false, 2, true, true>(a, st);
-        if (rows <= 96) return launch<8, 1, 1, 1, 4, 1, true, false, 2, true, true>(a, st);
-        return exact ? launch<4, 2, 1, 2, 4, 1, true, false, 2, false, true>(a, st)
-                     : launch<4, 2, 1, 2, 4, 1, true, true, 2, false, true>(a, st);
+        if (load(128, 128) == least)
+            return exact ? launch<4, 2, 1, 2, 4, 1, true, false, 2, false, true>(a, st)
+                         : launch<4, 2, 1, 2, 4, 1, true, true, 2, false, true>(a, st);
+        if (load(64, 128) == least) return launch<8, 1, 1, 1, 4, 1, true, false, 2, true, true>(a, st);
     } else {
-        if (rows <= 32) return launch<4, 1, 1, 2, 2, 1, false, false, 2, true, true>(a, st);
-        return exact ? launch<2, 2, 1, 4, 4, 1, false, false, 2, false, true>(a, st)
-                     : launch<2, 2, 1, 4, 4, 1, false, true, 2, false, true>(a, st);
+        if (load(128, 128) == least)
+            return exact ? launch<2, 2, 1, 4, 4, 1, false, false, 2, false, true>(a, st)
+                         : launch<2, 2, 1, 4, 4, 1, false, true, 2, false, true>(a, st);
+        if (load(32, 128) == least) return launch<4, 1, 1, 2, 2, 1, false, false, 2, true, true>(a, st);
     }
+    if (q) return launch<8, 1, 2, 1, 1, GLU ? 2 : 4, GLU, false, 4, true, true>(a, st);
+    if (load(16, 32) == least) return launch<2, 1, 4, 1, 1, GLU ? 4 : 8, GLU, false, 2, true, true>(a, st);
+    if (load(32, 32) == least) return launch<2, 1, 4, 1, 2, 4, GLU, false, 2, true, true>(a, st);
+    if (load(64, 32) == least) return launch<2, 2, 2, 1, 2, GLU ? 2 : 4, GLU, false, 2, true, true>(a, st);
+    return launch<2, 2, 2, 2, 2, 2, GLU, false, 2, true, true>(a, st);
 }
 
 }  // namespace

@@ -6,9 +6,6 @@
 
 namespace {
 
-// Compute units
-constexpr int64_t CUS = 256;
-
 // The tiles are those that give a compute unit the fewest rows of weights and tokens to load, over all its tiles: a unit
 // has about 40 KB of loads under way, which is 40 KB a microsecond, and that is what all but the largest calls wait for.
 // us and rows of a unit for tiles of 16, 32, 48, 64 tokens by 32 rows, 64 by 64 and 128 by 128 (bf16 results):

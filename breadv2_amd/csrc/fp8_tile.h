@@ -174,7 +174,7 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
 // KSB blocks of 128, by loads to LDS that are one stage ahead, across the tiles' ends too where it takes several (KEEP).
 // Rows lie 128 bytes apart, the eight pieces of 16 bytes of row r at piece ^ (r % 8), so that a read of a piece of 16 rows
 // covers the banks.  NWW x NWX waves have TO row tiles by TX token tiles each; NWK such sets of waves share a stage's
-// blocks and add their sums through LDS.
+// blocks and add their sums in the last stage's place.
 //
 // FAST, the 8-bit matrix instructions: they cut products more than 2^13 below the largest of their eight, which is
 // 1.5e-5 to 2.3e-5 of a result: a twentieth of fp16's own rounding, a hundred and seventieth of bf16's.  Not for fp32
@@ -244,7 +244,6 @@ __device__ __forceinline__ void count_tiles(const F8Args &a, int bx, int *begin,
 
 // LDS of a workgroup but for the stages
 template <class S, bool GRP> struct Lds {
-    __attribute__((aligned(16))) uint8_t sums[S::SUMS ? S::SUMS : 16];
     int begin[GRP ? GROUPS_MAX + 1 : 1], scan[S::WAVES];
     uint32_t tiles[GRP ? GROUPS_MAX + 1 : 1];
 };
@@ -459,10 +458,12 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     };
 
     // -------------------------------------------------------------- results
+    // spare: the last stage's buffer, for sums and magnitudes
     auto finish = [&](const Place &p, uint8_t *spare) __attribute__((always_inline)) {
         if constexpr (NWK > 1) {
-            f32x4 *part = reinterpret_cast<f32x4 *>(lds.sums);
+            f32x4 *part = reinterpret_cast<f32x4 *>(spare);
             constexpr int W = NWW * NWX;
+            barrier();  // all have read the last stage
             if (wk) {
 #pragma unroll
                 for (int i = 0; i < N; i++)
@@ -541,9 +542,9 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
                 // a token's largest magnitude in its lanes, then over the waves of the block's rows.  (rows is a
                 // multiple of 16, so a row tile is whole or absent.)
                 constexpr int WPB = F8_BLOCK / (16 * TO);  // waves a block
-                uint32_t(*mags)[BX] = reinterpret_cast<uint32_t(*)[BX]>(spare);
-                static_assert(4 * NWW * BX <= S::STAGE, "fits");
-                barrier();  // all have read the last stage
+                uint32_t(*mags)[BX] = reinterpret_cast<uint32_t(*)[BX]>(spare + S::SUMS);
+                static_assert(S::SUMS + 4 * NWW * BX <= S::STAGE, "fits");
+                if (NWK == 1) barrier();  // all have read the last stage
                 if (wk == 0) {
 #pragma unroll
                     for (int t = 0; t < TX; t++) {
@@ -659,6 +660,8 @@ __global__ __launch_bounds__(NWW * NWX * NWK * WAVE, WPE) void k_f8_matmul(const
     run_tiles<S, NWW, NWX, NWK, TO, TX, KSB, GLU, FAST, KEEP, GRP>(a, n_wt, n_xt, lds, buf);
 }
 
+constexpr int64_t CUS = 256;  // compute units
+
 // WPE: waves a SIMD, which the registers are held to; KEEP: workgroups take tiles in turn
 template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAST, int WPE, bool KEEP, bool GRP>
 int launch(const F8Args &a, hipStream_t st)
@@ -672,7 +675,7 @@ int launch(const F8Args &a, hipStream_t st)
     const int64_t n_wt = (a.rows + S::OR - 1) / S::OR;
     // groups: a tile more for each that ends inside one
     const int64_t n_xt = GRP ? a.T / S::BX + (a.G < a.T ? a.G : a.T) : (a.T + S::BX - 1) / S::BX;
-    const int64_t total = n_wt * n_xt, most = KEEP ? 256 * resident : 1 << 22;
+    const int64_t total = n_wt * n_xt, most = KEEP ? CUS * resident : 1 << 22;
     BREAD_REQUIRE(total <= (KEEP ? 1 << 30 : 1 << 22), BREAD_ERR_SHAPE, "more tiles than a launch counts");
     bread_clear_stale_error();
     hipLaunchKernelGGL((k_f8_matmul<NWW, NWX, NWK, TO, TX, KSB, GLU, FAST, WPE, KEEP, GRP>),

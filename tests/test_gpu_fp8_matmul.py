@@ -218,6 +218,12 @@ def test_groups_of_more_tiles_than_run_at_a_time(n, y, glu):
     grouped(70, n, 528, 272, y=y, glu=glu, index="gather", spare=2, first=1, seed=n)
 
 
+@pytest.mark.parametrize("y,glu", [("f32", False), ("f32", True), ("e4m3", False), ("e4m3", True)])
+@pytest.mark.parametrize("G,n,rows", [(20, 300, 272), (24, 1500, 528), (40, 900, 1040), (8, 540, 512), (54, 1500, 192)])
+def test_groups_of_every_tile(G, n, rows, y, glu):
+    grouped(G, n, rows, 400, y=y, glu=glu, index="scatter", seed=G)
+
+
 def test_offsets_that_fall():
     """Groups that overlap, end before they begin or leave the rows: nothing behind the rows is written, and groups in
     order before them are right."""
