@@ -3,7 +3,7 @@
 //   hidden[t] = residual[t] + sum_k w[t][k] down_e(q(silu(gate_e x) * (up_e x))),  e = idx[t][k].
 // Pairs (token, rank) are sorted by expert; gate and up are one grouped product
 // that ends in codes by pair, down another (fp8_grouped.hip), and the pairs of a
-// token are added in rank order.  A few tokens skip the sorting: a wave a row,
+// token are added in rank order.  Few pairs skip the sorting: a wave a row,
 // one kernel for gate and up and one for the rest.
 #include "activate.h"
 #include "fp8.h"
@@ -290,8 +290,15 @@ __global__ __launch_bounds__(256) void k_f8_combine(const float *__restrict__ eo
     }
 }
 
-// Tokens that skip the sorting
-constexpr int FEW_TOKENS = 4;
+// Whether calls skip the sorting: by estimates of both, ns, fitted to 27 shapes of 9 to 256 experts.  Without it every pair
+// reads its expert's weights (of some of them from the L2), and every token takes a wave for each of its values; with it
+// four launches follow one another.  us without and with: 256 experts of 512, hidden 2048, top 8, 2 tokens 16 and 32, 4 24
+// and 39, 6 33 and 46, 8 41 and 47; 10 experts of 256, hidden 2048, top 7, 8 tokens 18 and 33, 29 50 and 31; 12 of 256,
+// hidden 512, top 2, 40 tokens 17 and 20, 100 34 and 20.
+bool few(int64_t T, int64_t pairs, int64_t H, int64_t I)
+{
+    return pairs * 3 * H * I / 6250 + T * H / 4 <= 14000 + 7 * H;
+}
 
 }  // namespace
 
@@ -321,7 +328,7 @@ extern "C" int bread_moe_expert_block_fp8(bread_moe_ctx_t *c, const bread_fp8_ex
     bread_grouped_ws &g = c->gws;
     bread_clear_stale_error();
     const int few_lds = K * I + 4 * K * f8_blocks(I);
-    if (T <= FEW_TOKENS && (I == 256 || I == 512 || I == 1024) && few_lds <= 64 * 1024) {
+    if (few(T, P, H, I) && (I == 256 || I == 512 || I == 1024) && few_lds <= 64 * 1024) {
         FewArgs f;
         f.gate = static_cast<const uint8_t *>(ex->gate);
         f.up = static_cast<const uint8_t *>(ex->up);

@@ -105,6 +105,30 @@ def test_a_few_tokens(T, E, K, I, H):
     block(T, E, I, H, K, torch.float16, seed=T + K)
 
 
+@pytest.mark.parametrize("E,K,I,H", [(1, 1, 256, 256), (8, 8, 256, 256), (300, 3, 256, 256), (4, 2, 512, 1024), (6, 2, 768, 256)])
+def test_many_pairs(E, K, I, H):
+    """Pairs sorted by expert."""
+    block(400, E, I, H, K, torch.bfloat16, seed=E + K, residual="apart")
+
+
+def test_repeated_experts_and_ones_that_are_none_among_many_pairs():
+    block(300, 9, 256, 512, 4, torch.float32, "repeated", seed=7)
+    g = torch.Generator().manual_seed(5)
+    t = experts(8, 256, 256, g)
+    x, xs = R.random_activations(600, 256, g)
+    idx = torch.stack([torch.randperm(8, generator=g)[:2] for _ in range(600)]).int()
+    idx[::7, 0], idx[3::50, 1] = -1, 8
+    w, r = torch.rand(600, 2, generator=g), torch.randn(600, 256, generator=g)
+    ctx = B.MoeContext(B.shape(256, 256, 256, 8, 2), max_tokens=600)
+    hidden = r.cuda()
+    ctx.expert_block_fp8(B.Fp8Experts(*[v.cuda() for v in t]), x.cuda(), xs.cuda(), hidden, idx.cuda(), w.cuda())
+    with pytest.raises(B.BreadError) as e:
+        ctx.check_device()
+    assert e.value.device_error == 32
+    want, tol = reference(t, x, xs, idx, w, r)
+    R.check_wide(hidden, want, tol)
+
+
 def test_at_the_decode_shape():
     block(1, 16, 512, 2048, 8, torch.float16, seed=1)
     block(9, 16, 512, 2048, 8, torch.float32, seed=2)
