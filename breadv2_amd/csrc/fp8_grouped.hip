@@ -40,13 +40,13 @@ int launch_groups(const F8Args &a, hipStream_t st)
     const int64_t least = std::min({wide, load(128, 128), GLU ? load(64, 128) : load(32, 128), q ? load(16, 128) : INT64_MAX});
     if constexpr (GLU) {
         if (load(128, 128) == least)
-            return exact ? launch<4, 2, 1, 2, 4, 1, true, false, 2, false, true>(a, st)
-                         : launch<4, 2, 1, 2, 4, 1, true, true, 2, false, true>(a, st);
+            return exact ? launch<4, 2, 1, 2, 4, 1, true, false, 2, true, true>(a, st)
+                         : launch<4, 2, 1, 2, 4, 1, true, true, 2, true, true>(a, st);
         if (load(64, 128) == least) return launch<8, 1, 1, 1, 4, 1, true, false, 2, true, true>(a, st);
     } else {
         if (load(128, 128) == least)
-            return exact ? launch<2, 2, 1, 4, 4, 1, false, false, 2, false, true>(a, st)
-                         : launch<2, 2, 1, 4, 4, 1, false, true, 2, false, true>(a, st);
+            return exact ? launch<2, 2, 1, 4, 4, 1, false, false, 2, true, true>(a, st)
+                         : launch<2, 2, 1, 4, 4, 1, false, true, 2, true, true>(a, st);
         if (load(32, 128) == least) return launch<4, 1, 1, 2, 2, 1, false, false, 2, true, true>(a, st);
     }
     if (q) return launch<8, 1, 2, 1, 1, GLU ? 2 : 4, GLU, false, 4, true, true>(a, st);

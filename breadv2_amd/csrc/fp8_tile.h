@@ -8,8 +8,6 @@
 // a block of 128 columns and element of y.
 #pragma once
 
-#include <type_traits>
-
 #include "activate.h"
 #include "fp8.h"
 
@@ -194,7 +192,6 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
 // Where a tile lies: weights' group, first row and number of rows (of the call's T), first weight row
 struct Place {
     int g, p0, n, row0;
-    bool large;
 };
 
 template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAST> struct Shape {
@@ -213,9 +210,6 @@ template <int NWW, int NWX, int NWK, int TO, int TX, int KSB, bool GLU, bool FAS
 
 constexpr int GROUPS_MAX = 1024;
 
-// A group's token tiles are large, or one is small: with at most half of a tile's tokens.  A word counts both.
-constexpr int SMALL_BITS = 11;  // (at most one a group, and 2^24 / 16 large ones)
-
 // begin[g]: the groups' first rows, tiles[g]: token tiles of the groups before g, for g <= G
 template <int THREADS>
 __device__ __forceinline__ void count_tiles(const F8Args &a, int bx, int *begin, uint32_t *tiles, int *sums)
@@ -223,10 +217,7 @@ __device__ __forceinline__ void count_tiles(const F8Args &a, int bx, int *begin,
     for (int g = (int)threadIdx.x; g <= a.G; g += THREADS) begin[g] = min(max(a.offsets[g], 0), a.T);
     __syncthreads();
     const int per = (a.G + THREADS - 1) / THREADS, g0 = (int)threadIdx.x * per;
-    auto of = [&](int g) __attribute__((always_inline)) {
-        const int n = max(begin[g + 1] - begin[g], 0), rest = n % bx;
-        return (uint32_t)(n / bx + (2 * rest > bx)) << SMALL_BITS | (uint32_t)(rest && 2 * rest <= bx);
-    };
+    auto of = [&](int g) __attribute__((always_inline)) { return (uint32_t)((max(begin[g + 1] - begin[g], 0) + bx - 1) / bx); };
     uint32_t mine = 0;
     for (int g = g0; g < min(g0 + per, a.G); g++) mine += of(g);
     const uint32_t incl = (uint32_t)wave_scan_incl((int)mine);
@@ -255,54 +246,40 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     const int tid = (int)threadIdx.x, wv = wave_id(), l = lane_id();
     const int wk = wv / (NWW * NWX), ww = wv % NWW, wx = wv / NWW % NWX;
     const int r = l & 15, g = l >> 4, nb = f8_blocks(a.cols), nrb = f8_blocks(a.rows), steps = (nb + KSB - 1) / KSB;
-    // An XCD has consecutive tiles, whose workgroups then share an L2; of groups, first of the large ones and then of the
-    // small ones, so that workgroups that take tiles in turn have about the same work.
-    const int xcd = (int)blockIdx.x % 8, stride = (int)gridDim.x / 8;
-    int n_small = 0;
     if constexpr (GRP) {
         count_tiles<S::THREADS>(a, BX, lds.begin, lds.tiles, lds.scan);
-        // (n_xt: no more tiles than offsets that ascend can give; others are held to it)
-        const int large = min(uniform((int)(lds.tiles[a.G] >> SMALL_BITS)), n_xt);
-        n_small = min(uniform((int)(lds.tiles[a.G] & ((1 << SMALL_BITS) - 1))), n_xt - large);
-        n_xt = large;
+        // (n_xt: as many as offsets that ascend can give; others are held to it)
+        n_xt = (int)min((uint32_t)uniform((int)lds.tiles[a.G]), (uint32_t)n_xt);
     }
-    const int per = (n_xt * n_wt + 7) / 8, large0 = min(per * xcd, n_xt * n_wt), n_large = min(per, n_xt * n_wt - large0);
-    const int per_s = (n_small * n_wt + 7) / 8, small0 = min(per_s * xcd, n_small * n_wt);
-    const int end = n_large + min(per_s, n_small * n_wt - small0);
-    int tile = (int)blockIdx.x / 8;  // of the XCD's
+    // consecutive tiles on one XCD, whose workgroups then share an L2
+    const int total = n_xt * n_wt, per = (total + 7) / 8, stride = (int)gridDim.x / 8, xcd = (int)blockIdx.x % 8;
+    const int end = min(per * (xcd + 1), total);
+    int tile = per * xcd + (int)blockIdx.x / 8;
     if (tile >= end) return;
 
-    // where the XCD's tile j lies; before: a place that is not behind it
-    auto place = [&](int j, const Place &before) __attribute__((always_inline)) {
+    // where tile i lies; from: a group that is not behind it
+    auto place = [&](int i, int from) __attribute__((always_inline)) {
         Place p;
         if constexpr (GRP) {
-            // the last group with no more than xt tiles of the kind before it, 64 groups at a time
-            const bool large = j < n_large;
-            const int i = large ? large0 + j : small0 + j - n_large, xt = i / n_wt;
-            auto of = [&](uint32_t v) __attribute__((always_inline)) {
-                return (int)(large ? v >> SMALL_BITS : v & ((1 << SMALL_BITS) - 1));
-            };
-            int lo = large == before.large ? before.g : 0;
+            // the last group with no more than xt tiles before it, 64 groups at a time
+            const int xt = i / n_wt;
+            int lo = from;
             for (;;) {
                 const int ahead = lo + 1 + l;
-                const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ahead < a.G && of(lds.tiles[ahead]) <= xt));
+                const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ahead < a.G && lds.tiles[ahead] <= (uint32_t)xt));
                 lo += n;
                 if (n < WAVE) break;
             }
-            const uint32_t t = lds.tiles[lo], t1 = lds.tiles[lo + 1];
-            const int in_group = large ? xt - of(t) : (int)(t1 >> SMALL_BITS) - (int)(t >> SMALL_BITS);
-            p.large = large;
             p.g = lo;
             // (held to the call's rows also where offsets fall)
-            p.p0 = uniform(min(lds.begin[lo] + max(in_group, 0) * BX, a.T));
+            p.p0 = uniform(min(lds.begin[lo] + max(xt - (int)lds.tiles[lo], 0) * BX, a.T));
             p.n = uniform(max(min(lds.begin[lo + 1] - p.p0, BX), 0));
             p.row0 = (i - xt * n_wt) * OR;
         } else {
             // bands of eight token tiles: the tiles that an XCD works on at a time are a square
-            const int i = large0 + j, band = i / (8 * n_wt), k = i - band * 8 * n_wt, high = min(8, n_xt - 8 * band), w = k / high;
-            p.large = true;
+            const int band = i / (8 * n_wt), j = i - band * 8 * n_wt, high = min(8, n_xt - 8 * band), w = j / high;
             p.g = 0;
-            p.p0 = (8 * band + k - w * high) * BX;
+            p.p0 = (8 * band + j - w * high) * BX;
             p.n = min(a.T - p.p0, BX);
             p.row0 = w * OR;
         }
@@ -393,11 +370,11 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     };
     const int wr0 = 16 * TO * ww;  // the wave's first row in the tile
     const int at0 = r * F8_BLOCK + 16 * (g ^ (r & 7)), at1 = at0 ^ 64;
-    // Block kk of a stage with the wave's first C token tiles.  Each matrix instruction is followed by vector instructions
-    // that take about its time: the next row tile is widened and the last one's sums are scaled and added meanwhile.  (The
-    // compiler would put them in rows of one kind, and a SIMD's two waves, which a barrier lets go together, both wait.)
-    auto multiply = [&](const uint8_t *__restrict__ b, int kk, auto count) __attribute__((always_inline)) {
-        constexpr int C = decltype(count)::value;
+    // Block kk of a stage.  Each matrix instruction is followed by vector instructions that take about its time: the next
+    // row tile is widened and the last one's sums are scaled and added meanwhile.  (The compiler would put them in rows of
+    // one kind, and a SIMD's two waves, which a barrier lets go together, both wait.  Token tiles that hold no tokens are
+    // multiplied too: forms of fewer cost the registers that let a workgroup load its next tile ahead.)
+    auto multiply = [&](const uint8_t *__restrict__ b, int kk) __attribute__((always_inline)) {
         using F = Frag<FAST>;
         auto frag = [&](F &f, const uint8_t *__restrict__ p) __attribute__((always_inline)) {
             f.begin(*reinterpret_cast<const uint4 *>(p + at0), *reinterpret_cast<const uint4 *>(p + at1));
@@ -405,29 +382,29 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
         auto weights = [&](F &f, int i) __attribute__((always_inline)) {
             frag(f, b + (kk * WR + i / TO * OR + wr0 + 16 * (i % TO)) * F8_BLOCK);
         };
-        F x[C], w[N];
-        float xs[C], ws[M];
+        F x[TX], w[N];
+        float xs[TX], ws[M];
         weights(w[0], 0);
 #pragma unroll
-        for (int t = 0; t < C; t++) frag(x[t], b + S::W_BYTES + (kk * BX + 16 * (t * NWX + wx)) * F8_BLOCK);
+        for (int t = 0; t < TX; t++) frag(x[t], b + S::W_BYTES + (kk * BX + 16 * (t * NWX + wx)) * F8_BLOCK);
         if constexpr (N > 1) weights(w[1], 1);
 #pragma unroll
-        for (int t = 0; t < C; t++)
+        for (int t = 0; t < TX; t++)
             xs[t] = *reinterpret_cast<const float *>(b + S::XS_AT + 4 * (kk * S::XSW * WAVE + 16 * (t * NWX + wx) + r));
 #pragma unroll
         for (int m = 0; m < M; m++)
             ws[m] = *reinterpret_cast<const float *>(b + S::WS_AT + 4 * (m * WAVE + kk * S::OB + wr0 / F8_BLOCK));
-        f32x4 z[2][C];
+        f32x4 z[2][TX];
         float s = 0.f;
-        auto add = [&](int i, int j) __attribute__((always_inline)) {  // element j of the row tile's 4 C
+        auto add = [&](int i, int j) __attribute__((always_inline)) {  // element j of the row tile's 4 TX
             const int t = j / 4, e = j % 4;
             if (e == 0) s = xs[t] * ws[i / TO];
             acc[i][t][e] = fmaf(s, z[i & 1][t][e], acc[i][t][e]);
         };
-        constexpr int ALL = F::PARTS * C;  // matrix instructions of a row tile
+        constexpr int ALL = F::PARTS * TX;  // matrix instructions of a row tile
         auto widen = [&](int n) __attribute__((always_inline)) {  // what the n-th of them takes of the tokens
 #pragma unroll
-            for (int j = 0; j < F::STEPS / F::PARTS; j++) x[n % C].step(n / C * F::STEPS / F::PARTS + j);
+            for (int j = 0; j < F::STEPS / F::PARTS; j++) x[n % TX].step(n / TX * F::STEPS / F::PARTS + j);
         };
 #pragma unroll
         for (int j = 0; j < F::STEPS; j++) w[0].step(j);
@@ -437,7 +414,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
         for (int i = 0; i < N; i++) {
 #pragma unroll
             for (int n = 0; n < ALL; n++) {
-                const int k = n / C, t = n % C;
+                const int k = n / TX, t = n % TX;
                 if (i + 2 < N && n == ALL / 2) weights(w[i + 2], i + 2);
                 z[i & 1][t] = F::product(w[i], x[t], k, k ? z[i & 1][t] : f32x4{0.f, 0.f, 0.f, 0.f});
                 if (i == 0 && n + 1 < ALL) widen(n + 1);
@@ -447,13 +424,13 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
                 }
                 if (i) {
 #pragma unroll
-                    for (int j = n * 4 * C / ALL; j < (n + 1) * 4 * C / ALL; j++) add(i - 1, j);
+                    for (int j = n * 4 * TX / ALL; j < (n + 1) * 4 * TX / ALL; j++) add(i - 1, j);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4 * C; j++) add(N - 1, j);
+        for (int j = 0; j < 4 * TX; j++) add(N - 1, j);
         if (!GRP) __builtin_amdgcn_s_setprio(0);
     };
 
@@ -588,14 +565,14 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     // Stages of columns are loaded one ahead of the products, over the ends of tiles too; a tile's x rows are looked
     // up while the one before is loaded.
     const uint32_t at = lds_at(buf);
-    Place now = place(tile, Place{0, 0, 0, 0, true}), next = now, after = now;
+    Place now = place(tile, 0), next = now, after = now;
     int ltile = tile, lstep = 0;  // the next stage to load
     int b = 0, lb = 0;            // buffers
     bool begun = false;
     look(now);
     aim(now);
     if (KEEP && tile + stride < end) {
-        after = place(tile + stride, now);
+        after = place(tile + stride, now.g);
         look(after);
     }
     auto load = [&]() __attribute__((always_inline)) {
@@ -604,7 +581,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
             next = after;
             aim(next);
             if (ltile + stride < end) {
-                after = place(ltile + stride, next);
+                after = place(ltile + stride, next.g);
                 look(after);
             }
         }
@@ -618,7 +595,7 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
     };
     for (bool first = true; tile < end; tile = KEEP ? tile + stride : end) {
         clear();
-        int active = 0;  // the wave's token tiles that hold any
+        bool any = true;  // whether the wave has tokens
         for (int i = first ? -1 : 0; i < steps; i++) {
             if (i >= 0) {
                 wait_loads();
@@ -626,22 +603,14 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
             }
             load();
             if (i < 0) continue;
-            if (i == 0) active = min(max((now.n - 16 * wx + 16 * NWX - 1) / (16 * NWX), 0), TX);
+            if (GRP && NWX > 1 && i == 0) any = now.n > 16 * wx;
             const uint8_t *cur = buf + b * S::STAGE;
             b ^= 1;
 #pragma unroll
             for (int k = 0; k < S::KPW; k++) {
                 const int kk = wk + k * NWK;
                 if (i * KSB + kk >= nb) break;
-                if (!GRP) {
-                    multiply(cur, kk, std::integral_constant<int, TX>());
-                } else if (TX >= 4 && active <= TX / 4) {
-                    if (active) multiply(cur, kk, std::integral_constant<int, (TX + 3) / 4>());
-                } else if (TX >= 2 && active <= TX / 2) {
-                    if (active) multiply(cur, kk, std::integral_constant<int, (TX + 1) / 2>());
-                } else {
-                    if (active) multiply(cur, kk, std::integral_constant<int, TX>());
-                }
+                if (any) multiply(cur, kk);
             }
         }
         first = false;
@@ -679,7 +648,7 @@ int launch(const F8Args &a, hipStream_t st)
     BREAD_REQUIRE(total <= (KEEP ? 1 << 30 : 1 << 22), BREAD_ERR_SHAPE, "more tiles than a launch counts");
     bread_clear_stale_error();
     hipLaunchKernelGGL((k_f8_matmul<NWW, NWX, NWK, TO, TX, KSB, GLU, FAST, WPE, KEEP, GRP>),
-                       dim3((unsigned)(total + 14 < most ? total + 14 : most) / 8 * 8), dim3(S::THREADS), 0, st, a, (int)n_wt,
+                       dim3((unsigned)((total < most ? total : most) + 7) / 8 * 8), dim3(S::THREADS), 0, st, a, (int)n_wt,
                        (int)n_xt);
     BREAD_HIP(hipGetLastError());
     return BREAD_OK;
