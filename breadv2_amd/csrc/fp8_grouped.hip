@@ -10,22 +10,24 @@ namespace {
 // The tiles are those that give a compute unit the fewest rows of weights and tokens to load, as for one matrix
 // (fp8_matmul.hip), of about so many token tiles: half a tile more a group than the rows fill, and no fewer than groups.
 // us and rows of a unit for tiles of 16, 32, 64 tokens by 32 rows, 64 by 64, 32 by 128 and 128 by 128, to fp32:
-//   10 groups, 203 rows, 256 x 2048       6.8 (48)   7.9 (64)   9.2 (96)  11.7 (128)  15.2 (160)  20.2 (256)
-//   8, 540, 512 x 2048                   13.2 (144) 12.0 (128) 10.1 (96)  12.3 (128)  14.9 (160)  25.4 (256)
-//   54, 3452, 192 x 2048                 24.6 (288) 22.3 (256) 18.0 (192) 13.6 (128)  18.5 (320)  25.9 (256)
-//   12, 5022, 256 x 2048                 41.1       31.2       24.5       22.2 (256)  19.4 (320)  26.4 (256)
-//   256, 4096, 512 x 2048                89.1       84.2       98.5       76.3        45.9 (640)  55.3 (1024)
-//   256, 16384, 2048 x 512                                                            144         116
-//   256, 32768, 2048 x 512                                                            190         169
+//   10 groups, 203 rows, 256 x 2048       6.6 (48)   7.6 (64)   9.6 (96)  11.8 (128)  14.7 (160)  24.0 (256)
+//   8, 540, 512 x 2048                   12.7 (144) 11.7 (128)  9.8 (96)  12.2 (128)  14.6 (160)  24.6 (256)
+//   54, 3452, 192 x 2048                 23.3 (288) 21.7 (256) 17.4 (192) 13.4 (128)  17.9 (320)  25.3 (256)
+//   12, 5022, 256 x 2048                 38.4       29.9       23.7       22.0 (256)  18.4 (320)  25.8 (256)
+//   256, 4096, 512 x 2048                87.0       85.2      105         78.5        44.9 (640)  67.2 (1024)
+//   256, 16384, 2048 x 512              593        369        273        190         123 (6400)  108 (4096)
+//   256, 32768, 2048 x 512             1114        653        451        314         213         164 (6144)
 // and 16, 64 and 128 tokens by 128 rows, gated, to e4m3:
-//   10, 203, 256 x 2048                  15.8 (272) 23.4 (320) 28.0 (384)
-//   12, 5022, 256 x 2048                 40.3 (816) 29.6 (320) 38.1 (384)
-//   29, 4936, 512 x 2048                 76.9       54.6 (640) 39.2 (384)
-//   256, 4096, 512 x 2048                134        111        121;      256, 32768: -  262  233
-// Tiles of 32 by 128 are small enough for two workgroups a unit, which over several rounds take three quarters of the time.
-// Workgroups that take tiles in turn load the next one's first columns under the last one's results; the largest tiles
-// leave no registers for it.  fp16 and bf16 results of the largest tiles use the 8-bit matrix instructions (fp8_tile.h):
-// gated, 256 groups, 32768 rows, 512 x 2048: 181 of 233.
+//   10, 203, 256 x 2048                  15.2 (272) 25.6 (320) 34.4 (384)
+//   12, 5022, 256 x 2048                 38.1 (816) 26.6 (320) 35.3 (384)
+//   29, 4936, 512 x 2048                 75.4       51.1 (640) 38.0 (384)
+//   256, 4096, 512 x 2048                124        118 (1280) 129 (1536)
+//   256, 32768, 512 x 2048               466        250        211 (2304)
+// (Of 30 measured calls the rule took the fastest form 28 times, and lost 20 % in the others.)  Tiles of 32 by 128 are small
+// enough for two workgroups a unit, which over several rounds take three quarters of the time: with that the rule takes
+// them in those two calls as well.  Workgroups take tiles in turn and load the next one's first columns under the last
+// one's results: a tile's two to four microseconds of lookups and first loads, 160 of 177 at 2048 x 512.  fp16 and bf16
+// results of the largest tiles use the 8-bit matrix instructions (fp8_tile.h): gated, 256 groups, 32768 rows 177 of 211.
 template <bool GLU>
 int launch_groups(const F8Args &a, hipStream_t st)
 {

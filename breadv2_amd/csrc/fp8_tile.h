@@ -184,10 +184,11 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
 // Measured over long columns, 4096 tokens: exact 1.25 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.85.
 // Of an exact stage's 1.78 us (128 x 128 x 128 twice on a compute unit) the matrix instructions alone take 0.94, with the
 // reads of LDS 1.23, with widening and scaling 1.37, and the loads to LDS add 0.42.  Around its stages a tile costs 5 to
-// 8 us of first loads and results.
+// 8 us of lookups, first loads and results, or those of the results where a workgroup takes the next one meanwhile.
 // Tried and not kept: three stages (no faster: it is not latency), tokens widened once and shared as fp16 through LDS (the
 // same), the loads spread over a stage's products (slower by 6 to 17 %), columns that begin elsewhere for each tile (5 %:
-// weights are shared in step), a wave's token tiles one after the other, for wider tiles (15 %).
+// weights are shared in step), a wave's token tiles one after the other, for wider tiles (15 %), forms that skip the token
+// tiles of a group's rest that hold none (registers: 10 %), a group's rests behind all full tiles (2 %).
 
 // Where a tile lies: weights' group, first row and number of rows (of the call's T), first weight row
 struct Place {
