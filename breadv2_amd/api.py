@@ -297,7 +297,8 @@ def bread_matmul_fp8(w, w_scale, x, x_scale, y, y_scale=None, up=None, up_scale=
             raise ValueError("bias must be float32 [rows]")
         bp = bias.data_ptr()
     if residual is not None:
-        if residual.dtype != y.dtype or residual.shape != y.shape or residual.stride() != y.stride():
+        if (residual.dtype != y.dtype or residual.shape != y.shape
+                or (residual.stride() != y.stride() if T > 1 else not residual.is_contiguous())):
             raise ValueError("residual must have y's type, shape and stride")
         rp = residual.data_ptr()
     a = _matmul_fp8_args(w, w_scale, x, x_scale, y, y_scale, up, up_scale, act, shape, T, T, T, bp, rp)

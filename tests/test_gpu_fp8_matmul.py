@@ -110,6 +110,18 @@ def test_residual_in_place():
     R.check_wide(out, *R.epilogue(v, tol, residual=y))
 
 
+def test_residual_of_one_token_out_of_a_wider_buffer():
+    """One row has no stride: the residual's and y's may differ."""
+    g = gen(6)
+    x, xs = R.random_activations(1, 256, g)
+    w, ws = R.random_weights(40, 256, g)
+    y = torch.randn(1, 64, generator=g)
+    out = torch.zeros(1, 40, device="cuda")
+    B.bread_matmul_fp8(w.cuda(), ws.cuda(), x.cuda(), xs.cuda(), out, residual=y.cuda()[:, :40])
+    v, tol = R.product(x, xs, w, ws)
+    R.check_wide(out, *R.epilogue(v, tol, residual=y[:, :40]))
+
+
 @pytest.mark.parametrize("T", [1, 20, 140])
 def test_nan_stays_in_its_token(T):
     """NaN codes, scales and infinite scales of one token reach that token's results and no other's."""
