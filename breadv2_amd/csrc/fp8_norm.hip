@@ -189,7 +189,8 @@ extern "C" int bread_rmsnorm_fp8(const bread_rmsnorm_fp8_t *args, bread_stream_t
     BREAD_REQUIRE(f8_wide_type(o.x_type) && (!o.normed || f8_wide_type(o.normed_type)), BREAD_ERR_QTYPE,
                   "x_type and normed_type must be 0 (F32), 1 (F16) or 30 (BF16)");
     BREAD_REQUIRE(o.n % 16 == 0 && o.n <= 32768, BREAD_ERR_SHAPE, "n must be a multiple of 16, at most 32768");
-    BREAD_REQUIRE(o.n_tokens <= 1 << 22, BREAD_ERR_SHAPE, "n_tokens above 2^22");
+    // (a launch holds fewer than 2^32 threads, of which a long row takes 1024)
+    BREAD_REQUIRE(o.n_tokens < 1 << 22, BREAD_ERR_SHAPE, "n_tokens of 2^22 or more");
     const int64_t nb = f8_blocks(o.n);
     const int64_t xs = o.x_stride ? o.x_stride : o.n, rs = o.residual_stride ? o.residual_stride : o.n;
     const int64_t hs = o.hidden_stride ? o.hidden_stride : o.n, cs = o.codes_stride ? o.codes_stride : o.n;

@@ -42,6 +42,11 @@ def test_norm_refuses(kw, want):
     assert "bread_rmsnorm_fp8" in lib.bread_last_error().decode()
 
 
+def test_norm_refuses_more_rows_than_a_launch_holds():
+    """2^22 rows of 1024 threads each are 2^32 threads, one more than a launch counts."""
+    assert norm(n=32768, n_tokens=1 << 22) == _lib.ERR_SHAPE
+
+
 def matmul(groups=None, **kw):
     base = dict(w=P, w_scale=P, x=P, x_scale=P, y=P, y_type=0, rows=64, cols=256, n_tokens=2)
     a = fill(_lib.MatmulFp8Args, base, kw)
