@@ -316,6 +316,9 @@ extern "C" int bread_moe_expert_block_fp8(bread_moe_ctx_t *c, const bread_fp8_ex
                       (((uintptr_t)ex->gate_scale | (uintptr_t)ex->up_scale | (uintptr_t)ex->down_scale) & 3) == 0,
                   BREAD_ERR_ALIGN, "weights must be 16-byte aligned, scales 4-byte aligned");
     if (T == 0) return BREAD_OK;
+    int device;
+    BREAD_HIP(hipGetDevice(&device));
+    BREAD_REQUIRE(device == c->device, BREAD_ERR_ARG, "the context was made on another device than the current one");
     BREAD_REQUIRE(x && x_scale && hidden && idx && w, BREAD_ERR_ARG, "NULL pointer");
     BREAD_REQUIRE((((uintptr_t)x | (uintptr_t)hidden | (uintptr_t)residual) & 15) == 0 &&
                       (((uintptr_t)x_scale | (uintptr_t)idx | (uintptr_t)w) & 3) == 0,

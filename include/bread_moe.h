@@ -509,7 +509,7 @@ typedef struct {
  * them (packed, 16-byte aligned, up to 2^31 bytes), d_residual and d_hidden [n_tokens][H] fp32,
  * fp16 or bf16 (hidden_type) aligned to 16 bytes; d_residual may be d_hidden, NULL is zeros.
  * Products are exact and sums fp32; an expert's result is held in fp32 until
- * the sum is rounded once.  An index outside [0, n_experts) is left out and sets bit 32 of the
+ * the sum is rounded once.  The current device is the context's.  An index outside [0, n_experts) is left out and sets bit 32 of the
  * error word (bread_moe_ctx_check).  d_idx and d_w as bread_route_select gives
  * them. */
 int bread_moe_expert_block_fp8(bread_moe_ctx_t *ctx, const bread_fp8_experts_t *experts, const void *d_x,

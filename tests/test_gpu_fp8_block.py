@@ -266,3 +266,18 @@ def test_a_layer_captured_and_on_another_stream(T):
             out = layer(*d)[0]
             side.synchronize()
             assert torch.equal(out, e)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_a_context_of_another_device_is_refused():
+    with torch.cuda.device(1):
+        t = experts(4, 256, 256, torch.Generator().manual_seed(4))
+        e = B.Fp8Experts(*[v.cuda() for v in t])
+    with torch.cuda.device(0):
+        ctx = B.MoeContext(B.shape(256, 256, 256, 4, 2), max_tokens=2)
+    with torch.cuda.device(1):
+        o = lambda n, d: torch.zeros(1, n, dtype=d, device="cuda")  # noqa: E731
+        with pytest.raises(B.BreadError) as err:
+            ctx.expert_block_fp8(e, o(256, torch.uint8).view(F8), o(2, torch.float32), o(256, torch.float32),
+                                 o(2, torch.int32), o(2, torch.float32))
+    assert err.value.status == _lib.ERR_ARG
