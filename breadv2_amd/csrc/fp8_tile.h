@@ -347,7 +347,9 @@ __device__ __forceinline__ void run_tiles(const F8Args &a, const int n_wt, int n
             const int kk = i * PASS / WR, row = i * PASS % WR;  // (PASS divides WR or is a multiple of it)
             const int c = k0 + (PASS > WR ? (i * PASS + srow) / WR : kk) * F8_BLOCK;
             const uint32_t off = c + 16 * piece < a.cols ? woff[i] + (PASS > WR ? c - k0 : 0) : BEYOND;
-            const int soff = PASS > WR ? k0 : k0 + kk * F8_BLOCK;
+            // (a block behind the last column: from the buffer's start, for a scalar offset beyond a short buffer would be
+            // taken from its size)
+            const int first = PASS > WR ? k0 : k0 + kk * F8_BLOCK, soff = first < a.cols ? first : 0;
             // (a wave's eight rows are of one matrix)
             if (!GLU || (PASS <= OR ? row < OR : wv * 8 % WR < OR))
                 load_lds<16>(wb, b + i * PASS * F8_BLOCK, off, soff);
