@@ -190,7 +190,12 @@ int bread_rmsnorm_fp8(const bread_rmsnorm_fp8_t *args, bread_stream_t stream);
  *   y[t][r] = act(v[t][r]) * v_up[t][r] + residual[t][r].
  * The 8-bit form of bread_matmul.  y is fp16, bf16, fp32 or quantised again
  * (BREAD_QTYPE_E4M3: codes in y and scales in y_scale; rows a multiple of 16,
- * no residual).  Sums are fp32.  For fp32 and quantised y, and for a few tokens,
+ * no residual).  Sums are fp32.  So is the product of the two scales, which is
+ * rounded before it meets the block's sum: its magnitude has to stay below 2^128
+ * (from there on the block counts as infinite, or as NaN where its sum is zero),
+ * and below 2^-126 it has fewer bits, by which a block's part of a result is off
+ * by 2^-125 at most (a block of zeros then still adds zero).
+ * For fp32 and quantised y, and for a few tokens,
  * products are exact; for fp16 and bf16 y and many tokens they are summed by
  * the 8-bit matrix instructions, which cut each product of eight neighbours
  * below 2^-13 of the largest one's leading bit (5e-5 of a sum and less for
@@ -509,7 +514,7 @@ typedef struct {
  * them (packed, 16-byte aligned, up to 2^31 bytes), d_residual and d_hidden [n_tokens][H] fp32,
  * fp16 or bf16 (hidden_type) aligned to 16 bytes; d_residual may be d_hidden, NULL is zeros.
  * Products are exact and sums fp32; an expert's result is held in fp32 until
- * the sum is rounded once.  The current device is the context's.  An index outside [0, n_experts) is left out and sets bit 32 of the
+ * the sum is rounded once; products of scales as for bread_matmul_fp8.  The current device is the context's.  An index outside [0, n_experts) is left out and sets bit 32 of the
  * error word (bread_moe_ctx_check).  d_idx and d_w as bread_route_select gives
  * them. */
 int bread_moe_expert_block_fp8(bread_moe_ctx_t *ctx, const bread_fp8_experts_t *experts, const void *d_x,
