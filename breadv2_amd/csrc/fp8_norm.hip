@@ -112,15 +112,35 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fp8(const NormAr
             if (c < a.n) store8(a.h, row * a.hs + c, XT, v[i]);
         }
     }
-    sum = wave_sum(sum);
-    if constexpr (WPR > 1) {
-        if (lane == 0) part[threadIdx.x / WAVE] = sum;
-        __syncthreads();
-        sum = 0.f;
+    auto row_sum = [&](float mine) __attribute__((always_inline)) {
+        mine = wave_sum(mine);
+        if constexpr (WPR > 1) {
+            if (lane == 0) part[threadIdx.x / WAVE] = mine;
+            __syncthreads();
+            mine = 0.f;
 #pragma unroll
-        for (int i = 0; i < WPR; i++) sum += part[i];
+            for (int i = 0; i < WPR; i++) mine += part[i];
+        }
+        return mine;
+    };
+    sum = row_sum(sum);
+    float mean = sum / (float)a.n + a.eps;
+    // Squares beyond fp32, or too small for it with an eps that is no larger: the row (all its threads see the same sum)
+    // times a power of two.  (In a row of numbers beyond 2^56, those below 2^-54 lose bits by it, 2^-110 of the others.)
+    if (__builtin_expect(sum == INFINITY || mean < 0x1p-100f, 0)) {
+        const float p = sum == INFINITY ? 0x1p-72f : 0x1p100f;
+        float again = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                v[i][k] *= p;
+                again = fmaf(v[i][k], v[i][k], again);
+            }
+        if constexpr (WPR > 1) __syncthreads();  // all have read the first sum
+        mean = row_sum(again) / (float)a.n + a.eps * p * p;
     }
-    const float f = 1.0f / sqrtf(sum / (float)a.n + a.eps);
+    const float f = 1.0f / sqrtf(mean);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int c = 8 * (i * TPR + t);
