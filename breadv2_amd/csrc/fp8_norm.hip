@@ -218,6 +218,9 @@ extern "C" int bread_rmsnorm_fp8(const bread_rmsnorm_fp8_t *args, bread_stream_t
     BREAD_REQUIRE(xs >= o.n && rs >= o.n && hs >= o.n && cs >= o.n && ss >= nb && os >= o.n, BREAD_ERR_SHAPE,
                   "a stride is smaller than a row");
     if (o.n_tokens == 0) return BREAD_OK;
+    // (with another stride a row of hidden would lie on rows that others have yet to read)
+    BREAD_REQUIRE(o.n_tokens == 1 || !o.hidden || ((o.hidden != o.x || hs == xs) && (o.hidden != o.residual || hs == rs)),
+                  BREAD_ERR_ARG, "hidden in place of x or residual needs its stride");
     BREAD_REQUIRE(o.x && o.codes && o.scales, BREAD_ERR_ARG, "NULL pointer");
     BREAD_REQUIRE(((uintptr_t)o.codes & 15) == 0 && cs % 16 == 0, BREAD_ERR_ALIGN,
                   "codes must be 16-byte aligned and their stride a multiple of 16");

@@ -161,7 +161,7 @@ int bread_matmul(const void *w, const uint16_t *x, void *y, int rows, int cols, 
  * bread_matmul_fp8, and unquantised for a router.  n is a multiple of 16 up to
  * 32768, n_tokens below 2^22.  Strides in elements, 0: packed.  codes are 16-byte aligned with a
  * stride that is a multiple of 16, the others aligned to their elements.
- * hidden may be x or residual itself; nothing else may overlap.  Results
+ * hidden may be x or residual itself, with its stride; nothing else may overlap.  Results
  * between one row's end and the next row's start are left as they were. */
 typedef struct {
     const void *x;
