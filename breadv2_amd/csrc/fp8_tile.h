@@ -180,15 +180,21 @@ __device__ __forceinline__ void put4(const F8Args &a, int64_t t, int r, const fl
 // blocks and add their sums in the last stage's place.
 //
 // FAST, the 8-bit matrix instructions: they cut products more than 2^13 below the largest of their eight, which is
-// 1.5e-5 to 2.3e-5 of a result: a twentieth of fp16's own rounding, a hundred and seventieth of bf16's.  Not for fp32
-// results, nor for e4m3, whose scales are fp32.  Else the codes are widened to fp16 (exact, and their products sum in fp32).
+// 1.5e-5 to 2.3e-5 of a result (rms): a fourteenth to a ninth of fp16's own rounding, which is 2.1e-4, and a hundredth to a
+// seventieth of bf16's.  Not for fp32 results, nor for e4m3, whose scales are fp32, nor for a few tokens, which wait for
+// loads.  Else the codes are widened to fp16 (exact, and their products sum in fp32).
 //
 // What bounds them.  A compute unit's four SIMDs take an fp16 instruction of 16 x 16 x 32 in 16 cycles, and a widening,
 // a scaled addition or any other vector instruction in 4 to 5; the widenings are 16 (N + TX), the additions 4 N TX of
 // 4 N TX matrix instructions, so a wave's tiles want to be many and square: N, TX = 4 is what 256 registers hold.
 // Measured over long columns, 4096 tokens: exact 1.25 PFLOP/s (the library's bf16 product of 8192^3: 1.37), FAST 1.85.
 // Of an exact stage's 1.78 us (128 x 128 x 128 twice on a compute unit) the matrix instructions alone take 0.94, with the
-// reads of LDS 1.23, with widening and scaling 1.37, and the loads to LDS add 0.42.  Around its stages a tile costs 5 to
+// reads of LDS 1.23, with widening and scaling 1.37, and the loads to LDS add 0.42.  Of a FAST stage's 128 x 128 x 128 the
+// matrix instructions are 512 cycles a SIMD and the scaled additions some 300, but LDS is busy for 768 (at 128 bytes a
+// cycle): four waves of 64 x 64 read 64 KB, and 32 KB are written.  Larger wave tiles would read less.
+// Forms that take tiles in turn keep more than the scalar registers hold: those of groups spill 36 to 92 of them to lanes
+// (92: gated, 128 x 128), those of one matrix 10 to 36; those that take one tile none.  In the loop over the blocks that
+// is five lane reads at most, beside 64 matrix and some 210 vector instructions.  Around its stages a tile costs 5 to
 // 8 us of lookups, first loads and results, or those of the results where a workgroup takes the next one meanwhile.
 // Tried and not kept: three stages (no faster: it is not latency), tokens widened once and shared as fp16 through LDS (the
 // same), the loads spread over a stage's products (slower by 6 to 17 %), columns that begin elsewhere for each tile (5 %:

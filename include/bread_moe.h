@@ -194,12 +194,13 @@ int bread_rmsnorm_fp8(const bread_rmsnorm_fp8_t *args, bread_stream_t stream);
  * rounded before it meets the block's sum: its magnitude has to stay below 2^128
  * (from there on the block counts as infinite, or as NaN where its sum is zero),
  * and below 2^-126 it has fewer bits, by which a block's part of a result is off
- * by 2^-125 at most (a block of zeros then still adds zero).
- * For fp32 and quantised y, and for a few tokens,
- * products are exact; for fp16 and bf16 y and many tokens they are summed by
- * the 8-bit matrix instructions, which cut each product of eight neighbours
- * below 2^-13 of the largest one's leading bit (5e-5 of a sum and less for
- * ordinary values: under half a step of fp16).
+ * by 2^-125 at most (a block of zeros then still adds zero).  For fp32 and
+ * quantised y, and for a few tokens, products are exact; for fp16 and bf16 y and
+ * many tokens they are summed by the 8-bit matrix instructions, which cut each
+ * product of eight neighbours below 2^-13 of the largest one's leading bit (5e-5
+ * of the results' size and less for ordinary values: under half a step of fp16),
+ * so that a token's result may differ in its last bit between calls of few and of
+ * many tokens.
  * cols is a multiple of 16 up to 2^20, rows and n_tokens up to 2^24, rows *
  * n_tokens up to 2^33 and rows * cols up to 2^40.  Strides in elements, 0:
  * packed; x_stride up to 2^22, x_scale_stride up to 2^20.  w, up and x are 16-byte aligned with an
@@ -516,7 +517,7 @@ typedef struct {
  * Products are exact and sums fp32; an expert's result is held in fp32 until
  * the sum is rounded once; products of scales as for bread_matmul_fp8.  The current device is the context's.  An index outside [0, n_experts) is left out and sets bit 32 of the
  * error word (bread_moe_ctx_check).  d_idx and d_w as bread_route_select gives
- * them. */
+ * them.  A few tokens are fastest with an expert_inter of 256, 512 or 1024. */
 int bread_moe_expert_block_fp8(bread_moe_ctx_t *ctx, const bread_fp8_experts_t *experts, const void *d_x,
                                const float *d_x_scale, const void *d_residual, void *d_hidden, int hidden_type,
                                int n_tokens, const int32_t *d_idx, const float *d_w, bread_stream_t stream);
