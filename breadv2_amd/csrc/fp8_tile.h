@@ -9,8 +9,8 @@
 // That product is fp32's: a number below 2^128, with fewer bits below 2^-126 (a sum
 // is below 2^25, so a block's part is off by 2^-125 at most).  The header says so.
 // Blocks beyond by sums in 64 bits were built and not kept: a test a block costs
-// ordinary calls 2 to 5 %, one a tile up to 2 %, and either with a second path for
-// the sums 3 to 20 %, by the registers that it takes.
+// ordinary calls 2 to 5 %, one a tile up to 2 %, and with a second path for the
+// sums it is 1 to 25 %, by the registers that the path takes.
 #pragma once
 
 #include "activate.h"
